@@ -21,7 +21,10 @@ SOURCES = ["crag_scan_gemv.hip", "crag_scan_q16.hip", "crag_scan_qsplit.hip", "c
 INCLUDES = {"crag_scan_q16.hip": ["crag_q16_kloop.inc"],
             "crag_scan_qsplit.hip": ["crag_qsplit_kloop.inc"]}
 ISA_CHECKED = ("crag_scan_q16.hip", "crag_scan_qsplit.hip", "crag_scan_gemv.hip", "crag_scan_qlong.hip")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function"]
+# no packed float32 instructions: hipcc makes them by itself from ordinary float code, and some of their forms have been
+# seen to give wrong results now and then on this machine
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _newer(target, deps):
