@@ -17,9 +17,10 @@ SRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "lib", "libcoderag_hip.so")
 SOURCES = ["crag_scan_gemv.hip", "crag_scan_q16.hip", "crag_scan_qsplit.hip", "crag_scan_qlong.hip",
-           "crag_select.hip", "crag_capi.hip"]
+           "crag_scan_fp4.hip", "crag_embed.hip", "crag_select.hip", "crag_capi.hip"]
 INCLUDES = {"crag_scan_q16.hip": ["crag_q16_kloop.inc"],
-            "crag_scan_qsplit.hip": ["crag_qsplit_kloop.inc"]}
+            "crag_scan_qsplit.hip": ["crag_qsplit_kloop.inc"],
+            "crag_scan_fp4.hip": ["crag_fp4.h"], "crag_select.hip": ["crag_fp4.h"], "crag_capi.hip": ["crag_fp4.h"]}
 ISA_CHECKED = ("crag_scan_q16.hip", "crag_scan_qsplit.hip", "crag_scan_gemv.hip", "crag_scan_qlong.hip")
 # no packed float32 instructions: hipcc makes them by itself from ordinary float code, and some of their forms have been
 # seen to give wrong results now and then on this machine

@@ -11,8 +11,8 @@ from .collection import (GpuCollection, classify_path, f32_to_bf16_bits, hash_na
 from .hybrid_search import ChunkCollection, HybridSearcher, group_requests  # noqa: F401
 from .config import load_retrieval_config  # noqa: F401
 from .api import create_app, get_collection_name, search_route  # noqa: F401
-from .embed import HashingEmbedder  # noqa: F401
+from .embed import HashingEmbedder, TokenEmbedder, embed_bags, ngram_tokens  # noqa: F401
 
 __all__ = ["HybridSearcher", "ChunkCollection", "GpuCollection", "CragError", "search_multi", "search_multi_device", "merge_rerank_device",
            "get_collection_name", "search_route", "create_app", "HashingEmbedder", "classify_path", "hash_names",
-           "f32_to_bf16_bits", "load", "LIB_PATH", "SYMBOLS", "load_retrieval_config", "group_requests"]
+           "TokenEmbedder", "embed_bags", "ngram_tokens", "f32_to_bf16_bits", "load", "LIB_PATH", "SYMBOLS", "load_retrieval_config", "group_requests"]

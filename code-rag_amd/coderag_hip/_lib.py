@@ -12,7 +12,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libcoderag_hip.so")
 
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_FP4 = 0, 1, 2
 METRIC_L2, METRIC_IP = 0, 1
 ENTRY_BYTES = 16
 MAX_TOP_K = 200
@@ -27,6 +27,7 @@ SYMBOLS = [
     "crag_search", "crag_search_multi", "crag_search_multi_hashed", "crag_search_device", "crag_search_multi_device",
     "crag_search_device_noalloc",
     "crag_search_local_device", "crag_merge_rerank_device",
+    "crag_embed_workspace", "crag_embed_forward_device", "crag_embed_backward_device",
     "crag_stats", "crag_set_path", "crag_set_profiling", "crag_get_profile", "crag_debug_dense_scores",
 ]
 
@@ -97,6 +98,11 @@ def load() -> C.CDLL:
     lib.crag_search_device_noalloc.argtypes = [vp, vp, i32, i32, f64, vp, vp, vp, vp, vp, vp, vp]
     lib.crag_search_local_device.argtypes = [vp, vp, i32, i32, vp, vp, vp, vp]
     lib.crag_merge_rerank_device.argtypes = [i32, vp, i32, i32, i32, f64, vp, vp, vp, vp, vp]
+    f32 = C.c_float
+    lib.crag_embed_workspace.argtypes = [i64, i32, i32, i32]
+    lib.crag_embed_workspace.restype = i64
+    lib.crag_embed_forward_device.argtypes = [i32, vp, i64, i32, i32, vp, vp, i64, vp, i32, i32, f32, i32, vp, i32, vp, vp, i64, vp]
+    lib.crag_embed_backward_device.argtypes = [i32, vp, i64, i32, i32, vp, vp, i64, vp, i32, i32, vp, vp, vp, vp, vp, vp, i64, vp]
     lib.crag_stats.argtypes = [vp, vp, i32]
     lib.crag_set_path.argtypes = [vp, i32]
     lib.crag_set_profiling.argtypes = [vp, i32]

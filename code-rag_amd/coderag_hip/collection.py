@@ -63,19 +63,27 @@ def hash_names(names: Sequence) -> Tuple[np.ndarray, np.ndarray]:
     return out, lens
 
 
+DTYPES = {"f32": _lib.DTYPE_F32, "bf16": _lib.DTYPE_BF16, "fp4": _lib.DTYPE_FP4}
+
+
 def _ptr(a) -> Optional[int]:
     return None if a is None else a.ctypes.data
 
 
 class GpuCollection:
+    """dtype: "f32", "bf16", or "fp4" -- rows held in 4 bits with a scale for each 32 elements (include/coderag_hip.h:
+    CRAG_DTYPE_FP4), an eighth of float32's memory and traffic; rows and queries are float32 for it."""
+
     def __init__(self, dim: int, dtype: str = "f32", metric: str = "l2", device: int = 0):
+        if dtype not in DTYPES:
+            raise ValueError(f"dtype must be one of {sorted(DTYPES)}, got {dtype!r}")
         self._lib = _lib.load()
         self.dim = int(dim)
         self.dtype = dtype
         self.metric = metric
         self.device = int(device)
         h = C.c_void_p()
-        check(self._lib.crag_index_create(self.dim, {"f32": 0, "bf16": 1}[dtype], {"l2": 0, "ip": 1}[metric],
+        check(self._lib.crag_index_create(self.dim, DTYPES[dtype], {"l2": 0, "ip": 1}[metric],
                                           self.device, C.byref(h)), "crag_index_create")
         self._h = h
         self._keep = []  # tensors adopted zero-copy must outlive the handle
@@ -113,7 +121,7 @@ class GpuCollection:
         rows = np.asarray(rows)
         if rows.ndim != 2 or rows.shape[1] != self.dim:
             raise ValueError(f"rows must be [n, {self.dim}], got {rows.shape}")
-        if self.dtype == "f32":
+        if self.dtype != "bf16":
             return np.ascontiguousarray(rows, np.float32)
         if rows.dtype == np.uint16:
             return np.ascontiguousarray(rows)
@@ -140,14 +148,14 @@ class GpuCollection:
 
     def _check_tensor(self, t, n=None):
         import torch
-        want = torch.float32 if self.dtype == "f32" else torch.bfloat16
+        want = torch.bfloat16 if self.dtype == "bf16" else torch.float32
         if t.dtype != want or not t.is_cuda or not t.is_contiguous() or t.dim() != 2 or t.shape[1] != self.dim:
             raise ValueError(f"need a contiguous CUDA {want} tensor [n, {self.dim}]")
         if t.device.index != self.device:
             raise ValueError("tensor is on another device")
 
     def add_device(self, rows, name_hash=None, path_class=None):
-        """Device ingest: rows is a CUDA torch tensor in the index dtype; columns are CUDA tensors
+        """Device ingest: rows is a CUDA torch tensor in the index dtype (fp4: float32); columns are CUDA tensors
         (int64/uint64 bit patterns for name_hash, uint8 for path_class)."""
         import torch
         self._check_tensor(rows)
@@ -171,9 +179,10 @@ class GpuCollection:
         self._finalized = False
 
     def rows_host(self, first: int = 0, n: Optional[int] = None) -> np.ndarray:
-        """Rows [first, first + n) copied back from the device: float32 [n, dim], or uint16 bf16 bit patterns."""
+        """Rows [first, first + n) copied back from the device: float32 [n, dim] (of an fp4 collection the values its
+        codes stand for), or uint16 bf16 bit patterns."""
         n = len(self) - first if n is None else int(n)
-        out = np.empty((n, self.dim), np.float32 if self.dtype == "f32" else np.uint16)
+        out = np.empty((n, self.dim), np.uint16 if self.dtype == "bf16" else np.float32)
         check(self._lib.crag_index_get_rows(self._h, int(first), n, out.ctypes.data), "crag_index_get_rows")
         return out
 

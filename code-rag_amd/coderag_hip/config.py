@@ -48,8 +48,8 @@ def load_retrieval_config(path: Optional[str] = None) -> Dict[str, Any]:
     top_k, sb = int(cfg["topK"]), float(cfg["symbolBoost"])
     if not 1 <= top_k <= 200:
         raise ValueError(f"{path}: topK must be in 1..200 (CRAG_MAX_TOP_K), got {top_k}")
-    if cfg["metric"] not in ("l2", "ip") or cfg["dtype"] not in ("f32", "bf16"):
-        raise ValueError(f"{path}: metric must be l2|ip and dtype f32|bf16")
+    if cfg["metric"] not in ("l2", "ip") or cfg["dtype"] not in ("f32", "bf16", "fp4"):
+        raise ValueError(f"{path}: metric must be l2|ip and dtype f32|bf16|fp4")
     cfg["topK"], cfg["symbolBoost"] = top_k, sb
     cfg["searchDefaults"]["top_k"] = int(cfg["searchDefaults"]["top_k"])
     cfg["searchDefaults"]["symbol_boost"] = float(cfg["searchDefaults"]["symbol_boost"])

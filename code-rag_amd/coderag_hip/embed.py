@@ -13,16 +13,25 @@ model; plug the real embedder in for retrieval quality.
 searcher with no arguments (api/main.py:66-72): Chroma's own ONNX MiniLM when chromadb imports, built exactly as
 hybrid_search.py:23 builds it, so that a one-line swap keeps the reference's embeddings; otherwise the hashing
 stand-in, with a warning (once per process) that the results are not semantic.
+
+`TokenEmbedder` is the learned counterpart of the hashing stand-in, on the GPU: a text's tokens (by default the same
+character n-grams, hashed into the table's rows) are looked up, weighted, pooled and L2-normalised by one kernel
+(`embed_bags`, differentiable in the table and the weights, so the table can be trained with torch on a user's own
+question/chunk pairs).  With the identity as its table it computes HashingEmbedder.
 """
 from __future__ import annotations
 
 import warnings
 import zlib
-from typing import Callable, List
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import numpy as np
 
+from . import _lib
+from ._lib import check
+
 _warned = False
+POOL_MODES = {"sum": 0, "mean": 1, "sqrt": 2}
 
 
 def default_embedder() -> Callable[[List[str]], np.ndarray]:
@@ -40,6 +49,18 @@ def default_embedder() -> Callable[[List[str]], np.ndarray]:
     return lambda texts: np.asarray(onnx(list(texts)), np.float32)
 
 
+def ngram_hashes(text, ngram: int = 3) -> List[int]:
+    """CRC-32 of every byte n-gram (1 .. ngram) of the lowered text with a blank at both ends."""
+    b = (" " + str(text).lower() + " ").encode("utf-8", "ignore")
+    return [zlib.crc32(b[j:j + n]) for n in range(1, ngram + 1) for j in range(0, max(len(b) - n + 1, 0))]
+
+
+def ngram_tokens(text, vocab: int, ngram: int = 3) -> Tuple[np.ndarray, np.ndarray]:
+    """(ids int32 = hash % vocab, weights float32 = +-1 by the hash's top bit) of a text's n-grams: HashingEmbedder's."""
+    h = np.array(ngram_hashes(text, ngram), np.int64)
+    return (h % vocab).astype(np.int32), np.where((h >> 31) & 1, np.float32(1.0), np.float32(-1.0)).astype(np.float32)
+
+
 class HashingEmbedder:
     def __init__(self, dim: int = 384, ngram: int = 3):
         self.dim = dim
@@ -48,15 +69,166 @@ class HashingEmbedder:
     def __call__(self, texts: List[str]) -> np.ndarray:
         out = np.zeros((len(texts), self.dim), np.float32)
         for i, t in enumerate(texts):
-            s = " " + str(t).lower() + " "
-            b = s.encode("utf-8", "ignore")
-            for n in range(1, self.ngram + 1):
-                for j in range(0, max(len(b) - n + 1, 0)):
-                    h = zlib.crc32(b[j:j + n])
-                    out[i, h % self.dim] += 1.0 if (h >> 31) & 1 else -1.0
+            for h in ngram_hashes(t, self.ngram):
+                out[i, h % self.dim] += 1.0 if (h >> 31) & 1 else -1.0
             nrm = float(np.linalg.norm(out[i]))
             if nrm > 0:
                 out[i] /= nrm
             else:
                 out[i, 0] = 1.0
         return out
+
+
+# ---- lookups on the GPU ----------------------------------------------------------------------------------------------
+def _check_bags(table, ids, offsets, weights):
+    import torch
+    if table.dim() != 2 or table.dtype not in (torch.float32, torch.bfloat16) or not table.is_cuda or not table.is_contiguous():
+        raise ValueError("table must be a contiguous CUDA float32 or bfloat16 tensor [vocab, dim]")
+    for name, t, dt in (("ids", ids, torch.int32), ("offsets", offsets, torch.int64), ("weights", weights, torch.float32)):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.dtype != dt or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous 1-D {dt} tensor")
+        if t.device != table.device:
+            raise ValueError(f"{name} is on {t.device}, the table on {table.device}")
+    if offsets.numel() < 1:
+        raise ValueError("offsets must hold one more value than there are bags")
+    if weights is not None and weights.numel() != ids.numel():
+        raise ValueError("one weight per id")
+
+
+def _workspace(n_tokens: int, n_bags: int, dim: int, backward: bool, device):
+    import torch
+    size = check(_lib.load().crag_embed_workspace(n_tokens, n_bags, dim, int(backward)), "crag_embed_workspace")
+    return torch.empty(max(int(size), 256), dtype=torch.uint8, device=device)
+
+
+def _dtype_id(t) -> int:
+    import torch
+    return _lib.DTYPE_F32 if t.dtype == torch.float32 else _lib.DTYPE_BF16
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, want_coef):
+    import torch
+    dev, n_bags, (vocab, dim) = table.device, offsets.numel() - 1, table.shape
+    out = torch.empty((n_bags, dim), dtype=out_dtype, device=dev)
+    coef = torch.empty((n_bags,), dtype=torch.float32, device=dev) if want_coef else None
+    ws = _workspace(ids.numel(), n_bags, dim, False, dev)
+    check(_lib.load().crag_embed_forward_device(
+        dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), ids.numel(), offsets.data_ptr(),
+        n_bags, POOL_MODES[mode], float(scale), int(bool(normalize)), out.data_ptr(), _dtype_id(out), _ptr(coef), ws.data_ptr(),
+        ws.numel(), torch.cuda.current_stream(dev).cuda_stream), "crag_embed_forward_device")
+    return out, coef
+
+
+_function = None
+
+
+def _bag_function():
+    """the autograd node (made on first use: this module imports without torch)"""
+    global _function
+    if _function is not None:
+        return _function
+    import torch
+
+    class EmbedBags(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, table, weights, ids, offsets, mode, scale, normalize):
+            y, coef = _forward(table, ids, offsets, weights, mode, scale, normalize, torch.float32, True)
+            ctx.normalize = bool(normalize)
+            ctx.save_for_backward(table, weights, ids, offsets, y, coef)
+            return y
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            table, weights, ids, offsets, y, coef = ctx.saved_tensors
+            dev, n_bags, (vocab, dim) = table.device, offsets.numel() - 1, table.shape
+            grad = grad.contiguous()
+            d_table = torch.empty_like(table) if ctx.needs_input_grad[0] else None
+            d_weights = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
+            ws = _workspace(ids.numel(), n_bags, dim, True, dev)
+            check(_lib.load().crag_embed_backward_device(
+                dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), ids.numel(),
+                offsets.data_ptr(), n_bags, int(ctx.normalize), y.data_ptr(), coef.data_ptr(), grad.data_ptr(), _ptr(d_table),
+                _ptr(d_weights), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
+                "crag_embed_backward_device")
+            return d_table, d_weights, None, None, None, None, None
+
+    _function = EmbedBags
+    return _function
+
+
+def embed_bags(table, ids, offsets, weights=None, mode: str = "mean", scale: float = 1.0, normalize: bool = True, out_dtype=None):
+    """Pooled embedding lookup on the GPU: row b of the result is `scale` times the sum, mean or sum / sqrt(count) (`mode`) of
+    weights[t] * table[ids[t]] over the positions offsets[b] <= t < offsets[b + 1], divided by its norm when `normalize`.
+
+    table: CUDA [vocab, dim] float32 or bfloat16; ids: int32 [T]; offsets: int64 [bags + 1], ascending; weights: float32 [T]
+    or None.  Ids outside [0, vocab) are padding: they contribute nothing and do not count.  An empty bag gives zeros.
+    Returns [bags, dim] in out_dtype (float32).  Runs on the current stream of the table's device, without a
+    synchronisation.  Differentiable (once) in table and weights; the gradient of the table is dense, in its dtype."""
+    import torch
+    _check_bags(table, ids, offsets, weights)
+    if mode not in POOL_MODES:
+        raise ValueError(f"mode must be one of {sorted(POOL_MODES)}, got {mode!r}")
+    out_dtype = torch.float32 if out_dtype is None else out_dtype
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    if torch.is_grad_enabled() and (table.requires_grad or (weights is not None and weights.requires_grad)):
+        return _bag_function().apply(table, weights, ids, offsets, mode, float(scale), bool(normalize)).to(out_dtype)
+    return _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, False)[0]
+
+
+class TokenEmbedder:
+    """texts -> vectors through a table of token vectors on the GPU; an `embed_fn` for HybridSearcher.
+
+    table: array or tensor [vocab, dim], float32 or bfloat16; `tokenize(text) -> (ids, weights)` (weights may be None), by
+    default hashed character n-grams.  `__call__` returns float32 numpy vectors as every embed_fn does; `embed_device` leaves
+    them on the GPU, where GpuCollection.search_device takes them."""
+
+    def __init__(self, table, tokenize: Optional[Callable] = None, device: int = 0, mode: str = "mean", normalize: bool = True):
+        import torch
+        self.device = torch.device("cuda", int(device))
+        t = torch.from_numpy(np.ascontiguousarray(table, np.float32)) if isinstance(table, np.ndarray) else table
+        if t.dim() != 2 or t.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("table must be [vocab, dim], float32 or bfloat16")
+        if mode not in POOL_MODES:
+            raise ValueError(f"mode must be one of {sorted(POOL_MODES)}, got {mode!r}")
+        self.table = t.to(self.device).contiguous()
+        self.vocab, self.dim = self.table.shape
+        self.tokenize = tokenize if tokenize is not None else (lambda text: ngram_tokens(text, self.vocab))
+        self.mode, self.normalize = mode, bool(normalize)
+
+    def bags(self, texts: Sequence[str]):
+        """(ids int32, offsets int64, weights float32 or None) of the texts, on the device; an id outside the table is an error
+        here (embed_bags takes it for padding)."""
+        import torch
+        parts = [self.tokenize(t) for t in texts]
+        ids = [np.asarray(p[0], np.int64).reshape(-1) for p in parts]
+        offsets = np.zeros(len(ids) + 1, np.int64)
+        np.cumsum([len(i) for i in ids], out=offsets[1:])
+        flat = np.concatenate(ids) if ids else np.zeros(0, np.int64)
+        if flat.size and (flat.min() < 0 or flat.max() >= self.vocab):
+            raise ValueError(f"a token id is outside the table's {self.vocab} rows")
+        weights = None
+        if any(p[1] is not None for p in parts):
+            weights = np.concatenate([np.ones(len(i), np.float32) if p[1] is None else np.asarray(p[1], np.float32).reshape(-1)
+                                      for i, p in zip(ids, parts)])
+            if weights.size != flat.size:
+                raise ValueError("one weight per id")
+            weights = torch.from_numpy(weights).to(self.device)
+        return torch.from_numpy(flat.astype(np.int32)).to(self.device), torch.from_numpy(offsets).to(self.device), weights
+
+    def embed_device(self, texts: Sequence[str], out_dtype=None):
+        """CUDA tensor [len(texts), dim], float32 unless out_dtype says bfloat16"""
+        import torch
+        ids, offsets, weights = self.bags(texts)
+        with torch.no_grad():
+            return embed_bags(self.table, ids, offsets, weights, self.mode, 1.0, self.normalize, out_dtype)
+
+    def __call__(self, texts: List[str]) -> np.ndarray:
+        return self.embed_device(list(texts)).cpu().numpy()

@@ -3,7 +3,9 @@
 `data/chroma_db` persistence stands in the reference (indexer/embed_ingest.py:77-105).
 
     <db_path>/<collection_name>/meta.json     {"dim", "dtype", "metric", "count"}
-    <db_path>/<collection_name>/rows.npy      [count, dim] float32, or uint16 bf16 bit patterns
+    <db_path>/<collection_name>/rows.npy      [count, dim] float32, or uint16 bf16 bit patterns (bf16 and fp4
+                                              collections: the values of 4-bit rows are bf16 values, and adding
+                                              them again gives the same codes)
     <db_path>/<collection_name>/chunks.jsonl  one {"id", "meta", "text"} per row (the chunker's
                                               record shape, indexer/chunker.py:270-278)
 
@@ -19,6 +21,7 @@ from typing import Any, Callable, Dict, Iterable, List, Optional
 
 import numpy as np
 
+from .collection import f32_to_bf16_bits
 
 ROWS_PER_SLICE = 262144  # rows moved between disk, host and device at a time
 
@@ -59,9 +62,10 @@ def save_collection(db_path: str, col) -> str:
     n, dim = col.count(), col.gpu.dim
     out = np.lib.format.open_memmap(os.path.join(d, "rows.npy"), mode="w+",
                                     dtype=np.float32 if col.gpu.dtype == "f32" else np.uint16, shape=(n, dim))
+    as_bits = f32_to_bf16_bits if col.gpu.dtype == "fp4" else (lambda rows: rows)
     for lo in range(0, n, ROWS_PER_SLICE):
         m = min(ROWS_PER_SLICE, n - lo)
-        out[lo:lo + m] = col._host_rows(lo, m)
+        out[lo:lo + m] = as_bits(col._host_rows(lo, m))
     out.flush()
     del out
     with open(os.path.join(d, "chunks.jsonl"), "w", encoding="utf-8") as f:
@@ -85,7 +89,10 @@ def load_collection(db_path: str, name: str, device: int = 0):
     def flush():
         nonlocal done
         if ids:
-            col.add(list(ids), np.ascontiguousarray(rows[done:done + len(ids)]), list(metas), list(docs))
+            part = np.ascontiguousarray(rows[done:done + len(ids)])
+            if meta["dtype"] == "fp4":
+                part = (part.astype(np.uint32) << 16).view(np.float32)
+            col.add(list(ids), part, list(metas), list(docs))
             done += len(ids)
             ids.clear()
             metas.clear()

@@ -22,6 +22,7 @@
 
 #include "../../include/coderag_hip.h"
 #include "crag_common.h"
+#include "crag_fp4.h"
 
 namespace {
 
@@ -243,7 +244,12 @@ inline uint16_t f32_to_bf16(float f) {
 
 struct crag_index {
     int dim = 0, dim_pad = 0, dtype = 0, metric = 0, device = 0, chunks = 0;
-    size_t esz = 4;
+    size_t esz = 4;  // bytes per element of a query, and of a row unless the rows are 4-bit
+    // bytes that hold n rows
+    size_t row_storage(int64_t n) const {
+        if (dtype == CRAG_FP4) return (size_t)((n + 31) / 32) * (size_t)crag_fp4_tile_bytes(dim_pad >> 6);
+        return (size_t)n * (size_t)dim_pad * esz;
+    }
     int64_t n_rows = 0, cap_rows = 0;
     int64_t id_base = 0;
     void* rows = nullptr;
@@ -279,11 +285,10 @@ int grow(crag_index* h, int64_t need_rows, bool need_hash, bool need_class) {
         cap = std::max<int64_t>(need_rows, cap + cap / 2);
         cap = std::max<int64_t>(cap, 1024);
     }
-    const size_t row_bytes = (size_t)h->dim_pad * h->esz;
     if (realloc_rows) {
         void* nr = nullptr;
-        HIPCHK(hipMalloc(&nr, (size_t)cap * row_bytes));
-        if (h->n_rows) HIPCHK(hipMemcpy(nr, h->rows, (size_t)h->n_rows * row_bytes, hipMemcpyDeviceToDevice));
+        HIPCHK(hipMalloc(&nr, h->row_storage(cap)));
+        if (h->n_rows) HIPCHK(hipMemcpy(nr, h->rows, h->row_storage(h->n_rows), hipMemcpyDeviceToDevice));
         if (h->rows) (void)hipFree(h->rows);
         h->rows = nr;
     }
@@ -308,6 +313,36 @@ int grow(crag_index* h, int64_t need_rows, bool need_hash, bool need_class) {
     return 0;
 }
 
+// float32 rows -> 4-bit rows behind the ones that are there.  Host rows go through a staging buffer on the device.
+constexpr int64_t FP4_STAGE_BYTES = 64ll << 20;
+struct DevTemp {
+    void* p = nullptr;
+    ~DevTemp() {
+        if (p) (void)hipFree(p);
+    }
+};
+int add_fp4(crag_index* h, const void* rows, int64_t n, hipMemcpyKind kind) {
+    const int64_t row_bytes = (int64_t)h->dim * 4;
+    if (kind == hipMemcpyDeviceToDevice) {
+        if (((uintptr_t)rows & 3) != 0) return fail(CRAG_E_INVALID, "crag_index_add_device: rows must be aligned to their elements");
+        if (crag_launch_fp4_quantize((const float*)rows, n, h->dim, h->dim_pad, h->n_rows, h->rows, nullptr))
+            return fail(CRAG_E_HIP, "4-bit conversion launch failed");
+        HIPCHK(hipStreamSynchronize(nullptr));
+        return 0;
+    }
+    const int64_t per = std::min<int64_t>(n, std::max<int64_t>(1, FP4_STAGE_BYTES / row_bytes));
+    DevTemp stage;
+    HIPCHK(hipMalloc(&stage.p, (size_t)(per * row_bytes)));
+    for (int64_t i = 0; i < n; i += per) {
+        const int64_t m = std::min(per, n - i);
+        HIPCHK(hipMemcpy(stage.p, (const char*)rows + i * row_bytes, (size_t)(m * row_bytes), kind));
+        if (crag_launch_fp4_quantize((const float*)stage.p, m, h->dim, h->dim_pad, h->n_rows + i, h->rows, nullptr))
+            return fail(CRAG_E_HIP, "4-bit conversion launch failed");
+        HIPCHK(hipStreamSynchronize(nullptr));
+    }
+    return 0;
+}
+
 int add_common(crag_index* h, const void* rows, int64_t n, const uint64_t* name_hash, const uint8_t* path_class,
                hipMemcpyKind kind) {
     if (!h || n < 0 || (n > 0 && !rows)) return fail(CRAG_E_INVALID, "crag_index_add: bad arguments");
@@ -318,7 +353,9 @@ int add_common(crag_index* h, const void* rows, int64_t n, const uint64_t* name_
     if (rc) return rc;
     const size_t src_pitch = (size_t)h->dim * h->esz, dst_pitch = (size_t)h->dim_pad * h->esz;
     char* dst = (char*)h->rows + (size_t)h->n_rows * dst_pitch;
-    if (src_pitch == dst_pitch) {
+    if (h->dtype == CRAG_FP4) {
+        if ((rc = add_fp4(h, rows, n, kind))) return rc;
+    } else if (src_pitch == dst_pitch) {
         HIPCHK(hipMemcpy(dst, rows, (size_t)n * dst_pitch, kind));
     } else {
         HIPCHK(hipMemset(dst, 0, (size_t)n * dst_pitch));
@@ -523,6 +560,8 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     //              VALU-bound (6-8 queries 0.90-1.0 / 0.75)
     const int path = h0->force_path;  // 0 auto, 1 GEMV, 2 MFMA, 3 tiled MFMA (tests, bench, tools)
     const bool bf16 = h0->dtype == CRAG_BF16;
+    // 4-bit rows have one scan for every batch size (crag_scan_fp4.hip); several collections, or path 1, take its grouped form
+    const bool fp4 = h0->dtype == CRAG_FP4;
     const bool can_q16 = bf16 && crag_q16_supported(h0->dim_pad), can_qsplit = bf16 && crag_qsplit_supported(h0->dim_pad);
     const bool can_qlong = crag_qlong_supported(h0->dtype, h0->dim_pad);
     int mfma_from;
@@ -531,6 +570,8 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     else if (bf16) mfma_from = CRAG_QLONG_FROM;
     else mfma_from = h0->dim_pad <= 192 ? 5 : CRAG_QLONG_FROM_F32;
     P.mfma = same_handle && (can_q16 || can_qsplit || can_qlong) && (path >= 2 || (path == 0 && B >= mfma_from));
+    if (fp4) P.mfma = same_handle && path != 1;
+    const int group_q = fp4 ? CRAG_FP4_GROUP_Q : CRAG_MAX_GROUP_Q;
 
     const bool qsplit = P.mfma && can_qsplit;  // 1024-element rows: flat buffers, row-major sample
     // (the LDS-tiled scan, crag_scan_qlong.hip: flat buffers and a row-major sample as well)
@@ -574,7 +615,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         int max_nq = 1;
         while (b < B) {
             int e = b + 1;
-            while (e < B && e - b < CRAG_MAX_GROUP_Q && hs[e] == hs[b]) ++e;
+            while (e < B && e - b < group_q && hs[e] == hs[b]) ++e;
             GroupDesc g;
             memset(&g, 0, sizeof(g));
             g.rows = hs[b]->rows;
@@ -594,6 +635,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
             b = e;
         }
         P.nq_template = max_nq <= 1 ? 1 : (max_nq <= 2 ? 2 : (max_nq <= 4 ? 4 : 8));
+        if (fp4) P.nq_template = 2;  // its waves take tiles of 32 rows
         for (int pass = 0; pass < 3; ++pass) P.blocks[pass] = gemv_partition(gd, pass, P.nq_template, h0->n_cus);
     }
     P.n_groups = (int)gd.size();
@@ -607,7 +649,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     if ((rc = ws->desc.ensure(desc_bytes))) return rc;
     if ((rc = ws->tau.ensure(sizeof(float) * (size_t)B))) return rc;
     if ((rc = ws->cntst.ensure(sizeof(uint32_t) * ((size_t)B * CRAG_CNT_STRIDE + (size_t)B)))) return rc;
-    const bool query_minor = P.mfma;  // every MFMA scan writes a query-minor sample: [row][bpad] or tile-major
+    const bool query_minor = P.mfma && !fp4;  // these MFMA scans write a query-minor sample: [row][bpad] or tile-major
     const long long bpad = ((long long)B + 15) / 16 * 16;
     if ((rc = ws->sample.ensure(sizeof(uint32_t) * (size_t)std::max<long long>(B, bpad) * (size_t)P.sample_stride))) return rc;
     const bool merged = !noalloc && ws->merged_bytes != 0;
@@ -661,7 +703,32 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     if (prof && (rc = ws->ensure_events())) return rc;
     MfmaArgs ma;
     ScanArgs ga;
-    if (P.mfma) {
+    Fp4Args fa = {};
+    const float* qres = nullptr;
+    if (fp4) {
+        const bool narrow = !P.mfma || B <= CRAG_FP4_GROUP_Q;
+        const int n_blocks = P.mfma ? crag_fp4_query_blocks(B, h0->dim_pad) : (int)gd.size();
+        const size_t piece_bytes = (size_t)crag_fp4_query_bytes(n_blocks, h0->dim_pad, narrow);
+        if ((rc = ws->qscan.ensure(piece_bytes + sizeof(float) * (size_t)B))) return rc;
+        float* res = (float*)((char*)ws->qscan.p + piece_bytes);
+        if (crag_launch_fp4_split(q_dev, P.mfma ? nullptr : gd_dev, n_blocks, B, h0->dim_pad, h0->metric, narrow, ws->qscan.p, res, st))
+            return fail(CRAG_E_HIP, "query split launch failed");
+        qres = res;
+        fa.queries = ws->qscan.p;
+        fa.metric = h0->metric;
+        fa.tau = tau;
+        fa.sample = sample;
+        fa.sample_stride = P.sample_stride;
+        fa.cand = cand;
+        fa.cand_stride = cand_stride;
+        fa.cnt = cnt;
+        fa.rows = h0->rows;
+        fa.xnorm = h0->xnorm;
+        fa.n_queries = B;
+        fa.groups = P.mfma ? nullptr : gd_dev;
+        fa.n_groups = P.n_groups;
+        h0->stats[P.mfma ? 5 : 6]++;
+    } else if (P.mfma) {
         ma.rows = h0->rows;
         ma.xnorm = h0->xnorm;
         ma.n_rows = h0->n_rows;
@@ -703,12 +770,21 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     }
     auto scan = [&](int pass) -> int {  // GEMV passes (the MFMA scans run the cascade below)
         if (P.blocks[pass] == 0) return 0;  // every row of every group is already behind an earlier level
+        if (fp4) {
+            fa.pass = pass;
+            return crag_launch_scan_fp4_groups(fa, h0->dim_pad, P.blocks[pass], st);
+        }
         return crag_launch_scan_gemv(ga, pass, P.nq_template, P.blocks[pass], st);
     };
     if (prof) HIPCHK(hipEventRecord(ws->ev[0], st));
     double prof_rows = 0.0;  // rows the last (timed) filter launch scans
     if (cascade) {
         auto launch_level = [&](int mode) -> int {
+            if (fp4) {
+                fa.row_begin = ma.row_begin;
+                fa.row_end = ma.row_end;
+                return crag_launch_scan_fp4(fa, h0->dim_pad, mode == 1, h0->n_cus, st);
+            }
             if (segmented) return crag_launch_scan_q16(ma, mode, h0->n_cus, st);
             if (qsplit) return crag_launch_scan_qsplit(ma, mode, h0->n_cus, st);
             return crag_launch_scan_qlong(ma, h0->dtype, mode, h0->n_cus, st);
@@ -723,6 +799,9 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         k.src = sample;
         if (segmented) {
             k.tile_bpad = bpad;  // the two-block scan writes a tile-major sample
+        } else if (!query_minor) {
+            k.q_stride = P.sample_stride;  // the 4-bit scan writes a query's scores one after the other
+            k.e_stride = 1;
         } else {
             k.q_stride = 1;      // the one-block scans write it row-major: [row][bpad]
             k.e_stride = bpad;
@@ -855,6 +934,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     f.n_seg = n_seg;
     f.seg_cap = seg_cap;
     f.cand_stride = cand_stride;
+    f.qres = qres;
     f.qmap = nullptr;
     if ((rc = crag_launch_finalize(f, st))) return fail(CRAG_E_HIP, "finalize launch failed");
     auto merge = [&]() -> int {
@@ -934,7 +1014,10 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
                 ma.row_begin = 0;
                 ma.row_end = h0->n_rows;
                 ma.progress = nullptr;
-                if (segmented ? crag_launch_scan_q16(ma, 1, h0->n_cus, st)
+                fa.row_begin = 0;
+                fa.row_end = h0->n_rows;
+                if (fp4         ? crag_launch_scan_fp4(fa, h0->dim_pad, true, h0->n_cus, st)
+                    : segmented ? crag_launch_scan_q16(ma, 1, h0->n_cus, st)
                     : qsplit  ? crag_launch_scan_qsplit(ma, 1, h0->n_cus, st)
                               : crag_launch_scan_qlong(ma, h0->dtype, 1, h0->n_cus, st))
                     return fail(CRAG_E_HIP, "re-scan launch failed");
@@ -953,7 +1036,12 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
                 HIPCHK(hipMemcpyAsync(ws->keys.p, ws->pinned, bytes2, hipMemcpyHostToDevice, st));
                 ScanArgs ga2 = ga;
                 ga2.groups = (const GroupDesc*)ws->keys.p;
-                if (crag_launch_scan_gemv(ga2, 2, P.nq_template, blocks2, st)) return fail(CRAG_E_HIP, "re-scan launch failed");
+                if (fp4) {
+                    Fp4Args fa2 = fa;
+                    fa2.groups = ga2.groups;
+                    fa2.pass = 2;
+                    if (crag_launch_scan_fp4_groups(fa2, h0->dim_pad, blocks2, st)) return fail(CRAG_E_HIP, "re-scan launch failed");
+                } else if (crag_launch_scan_gemv(ga2, 2, P.nq_template, blocks2, st)) return fail(CRAG_E_HIP, "re-scan launch failed");
             }
             HIPCHK(hipStreamSynchronize(st));  // the pinned staging (descriptors, then the query list) is reused below
             if ((rc = upload_qmap(t1b))) return rc;
@@ -1049,7 +1137,7 @@ int upload_queries(crag_index* h, const float* queries, int B, Workspace* ws, hi
     memset(stage, 0, bytes);
     for (int b = 0; b < B; ++b) {
         const float* src = queries + (size_t)b * h->dim;
-        if (h->dtype == CRAG_F32) {
+        if (h->dtype != CRAG_BF16) {
             memcpy(stage + (size_t)b * h->dim_pad * 4, src, (size_t)h->dim * 4);
         } else {
             uint16_t* dst = (uint16_t*)(stage + (size_t)b * h->dim_pad * 2);
@@ -1257,6 +1345,38 @@ int put_descriptors(const QueryDesc& qd, const GroupDesc* gd, int n_groups, int 
 
 }  // namespace
 
+namespace {
+
+// the caller's current device comes back when the call returns
+struct DeviceGuard {
+    int before = -1, rc = 0;
+    explicit DeviceGuard(int device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (before != device) rc = hipSetDevice(device) == hipSuccess ? 0 : -1;
+        if (rc) (void)hipGetLastError();
+    }
+    ~DeviceGuard() {
+        int now = -1;
+        if (before >= 0 && hipGetDevice(&now) == hipSuccess && now != before) (void)hipSetDevice(before);
+    }
+};
+
+int check_embed(const char* who, const void* table, int64_t vocab, int dim, int dtype, const int32_t* ids, int64_t n, const int64_t* offsets,
+                int n_bags, const void* workspace, int64_t workspace_bytes, bool backward) {
+    const std::string w = who;
+    if (!table || vocab <= 0 || vocab > 0x7fffffff || dim <= 0 || n < 0 || n > 0x7fffffff || n_bags < 0) return fail(CRAG_E_INVALID, w + ": bad arguments");
+    if (dim > CRAG_MAX_EMBED_DIM) return fail(CRAG_E_LIMIT, w + ": more than 2048 elements per row");
+    if (dtype != CRAG_F32 && dtype != CRAG_BF16) return fail(CRAG_E_INVALID, w + ": tables are float32 or bf16");
+    if (((uintptr_t)table & (dtype == CRAG_F32 ? 3 : 1)) != 0) return fail(CRAG_E_INVALID, w + ": the table must be aligned to its elements");
+    if ((n > 0 && !ids) || (n_bags > 0 && !offsets)) return fail(CRAG_E_INVALID, w + ": null buffer");
+    const int64_t need = (int64_t)crag_embed_ws_bytes(n, n_bags, dim, backward);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return fail(CRAG_E_INVALID, w + ": the workspace is smaller than crag_embed_workspace says");
+    if (((uintptr_t)workspace & 255) != 0) return fail(CRAG_E_INVALID, w + ": the workspace must be 256-byte aligned");
+    return 0;
+}
+
+}  // namespace
+
 extern "C" {
 
 int crag_version(void) { return 100; }
@@ -1271,9 +1391,11 @@ int crag_device_count(void) {
 int crag_index_create(int dim, int dtype, int metric, int device, crag_index** out) {
     if (!out) return fail(CRAG_E_INVALID, "crag_index_create: out is NULL");
     *out = nullptr;
-    if (dim <= 0 || (dtype != CRAG_F32 && dtype != CRAG_BF16) || (metric != CRAG_L2 && metric != CRAG_IP))
+    if (dim <= 0 || (dtype != CRAG_F32 && dtype != CRAG_BF16 && dtype != CRAG_FP4) || (metric != CRAG_L2 && metric != CRAG_IP))
         return fail(CRAG_E_INVALID, "crag_index_create: bad dim/dtype/metric");
-    const size_t esz = dtype == CRAG_F32 ? 4 : 2;
+    const size_t esz = dtype == CRAG_BF16 ? 2 : 4;
+    const int fp4_pad = dtype == CRAG_FP4 ? crag_fp4_dim_pad(dim) : 0;
+    if (dtype == CRAG_FP4 && !fp4_pad) return fail(CRAG_E_LIMIT, "crag_index_create: 4-bit rows of more than 2048 elements are not supported");
     const size_t chunks_needed = ((size_t)dim * esz + 15) / 16;
     int chunks = 0;
     for (int c : kChunkSizes)
@@ -1281,7 +1403,7 @@ int crag_index_create(int dim, int dtype, int metric, int device, crag_index** o
             chunks = c;
             break;
         }
-    if (!chunks) return fail(CRAG_E_LIMIT, "crag_index_create: rows longer than 4096 bytes are not supported");
+    if (!chunks && !fp4_pad) return fail(CRAG_E_LIMIT, "crag_index_create: rows longer than 4096 bytes are not supported");
     int ndev = 0;
     HIPCHK(hipGetDeviceCount(&ndev));
     if (device < 0 || device >= ndev) return fail(CRAG_E_INVALID, "crag_index_create: no such device");
@@ -1296,7 +1418,7 @@ int crag_index_create(int dim, int dtype, int metric, int device, crag_index** o
     h->device = device;
     h->esz = esz;
     h->chunks = chunks;
-    h->dim_pad = (int)((size_t)chunks * 16 / esz);
+    h->dim_pad = fp4_pad ? fp4_pad : (int)((size_t)chunks * 16 / esz);
     h->len_present.assign(65536 + 1, 0);
     h->n_cus = prop.multiProcessorCount > 0 ? prop.multiProcessorCount : 256;
     *out = h;
@@ -1354,6 +1476,7 @@ int crag_index_attach_device(crag_index* h, const void* rows_dev, int64_t n, con
     if (!h || !rows_dev || n < 0) return fail(CRAG_E_INVALID, "crag_index_attach_device: bad arguments");
     if (h->n_rows != 0) return fail(CRAG_E_STATE, "crag_index_attach_device: collection already holds rows");
     if (n > CRAG_MAX_ROWS) return fail(CRAG_E_LIMIT, "crag_index_attach_device: a collection holds at most 2^32 - 64 rows");
+    if (h->dtype == CRAG_FP4) return fail(CRAG_E_INVALID, "crag_index_attach_device: 4-bit rows have a layout of their own; add them");
     if (h->dim != h->dim_pad) return fail(CRAG_E_INVALID, "crag_index_attach_device: dim must equal crag_index_dim_pad");
     if (((uintptr_t)rows_dev) & 15) return fail(CRAG_E_INVALID, "crag_index_attach_device: rows must be 16-byte aligned");
     h->rows = const_cast<void*>(rows_dev);
@@ -1373,6 +1496,18 @@ int crag_index_get_rows(const crag_index* h, int64_t first, int64_t n, void* out
         return fail(CRAG_E_INVALID, "crag_index_get_rows: bad arguments");
     if (n == 0) return 0;
     HIPCHK(hipSetDevice(h->device));
+    if (h->dtype == CRAG_FP4) {
+        const int64_t row_bytes = (int64_t)h->dim * 4, per = std::min<int64_t>(n, std::max<int64_t>(1, FP4_STAGE_BYTES / row_bytes));
+        DevTemp stage;
+        HIPCHK(hipMalloc(&stage.p, (size_t)(per * row_bytes)));
+        for (int64_t i = 0; i < n; i += per) {
+            const int64_t m = std::min(per, n - i);
+            if (crag_launch_fp4_dequantize(h->rows, first + i, m, h->dim, h->dim_pad, (float*)stage.p, nullptr))
+                return fail(CRAG_E_HIP, "4-bit read-back launch failed");
+            HIPCHK(hipMemcpy((char*)out_rows + i * row_bytes, stage.p, (size_t)(m * row_bytes), hipMemcpyDeviceToHost));
+        }
+        return 0;
+    }
     const size_t src_pitch = (size_t)h->dim_pad * h->esz, dst_pitch = (size_t)h->dim * h->esz;
     HIPCHK(hipMemcpy2D(out_rows, dst_pitch, (const char*)h->rows + (size_t)first * src_pitch, src_pitch, dst_pitch, (size_t)n,
                        hipMemcpyDeviceToHost));
@@ -1391,7 +1526,8 @@ int crag_index_finalize(crag_index* h) {
     HIPCHK(hipMemset(h->xnorm, 0, sizeof(float) * (nx + 4)));
     float* mx = h->xnorm + nx;
     if (h->n_rows) {
-        int rc = crag_launch_row_norms(h->rows, h->dtype, h->dim_pad, h->n_rows, h->xnorm, mx, nullptr);
+        int rc = h->dtype == CRAG_FP4 ? crag_launch_fp4_row_norms(h->rows, h->dim_pad, h->n_rows, h->xnorm, mx, nullptr)
+                                      : crag_launch_row_norms(h->rows, h->dtype, h->dim_pad, h->n_rows, h->xnorm, mx, nullptr);
         if (rc) return fail(CRAG_E_HIP, "row_norms launch failed");
     }
     HIPCHK(hipMemcpy(&h->max_xnorm, mx, 4, hipMemcpyDeviceToHost));
@@ -1595,11 +1731,28 @@ int crag_debug_dense_scores(crag_index* h, const void* queries_dev, int B, int p
     int rc;
     if ((rc = stage_device_queries(h, queries_dev, B, ws, st, &q))) return rc;
     const long long n = h->n_rows;
-    const long long stride = n;
+    const long long stride = h->dtype == CRAG_FP4 ? (n + 63) / 64 * 64 : n;
     bool rowmajor = false, tiled = false;
     long long bpad = B;
     if ((rc = ws->sample.ensure(sizeof(uint32_t) * (size_t)B * (size_t)std::max<long long>(stride, 1)))) return rc;
-    if (path >= 2) {
+    if (h->dtype == CRAG_FP4) {
+        const bool narrow = B <= CRAG_FP4_GROUP_Q;
+        const int n_blocks = crag_fp4_query_blocks(B, h->dim_pad);
+        const size_t piece_bytes = (size_t)crag_fp4_query_bytes(n_blocks, h->dim_pad, narrow);
+        if ((rc = ws->qscan.ensure(piece_bytes + sizeof(float) * (size_t)B))) return rc;
+        if (crag_launch_fp4_split(q, nullptr, n_blocks, B, h->dim_pad, h->metric, narrow, ws->qscan.p, (float*)((char*)ws->qscan.p + piece_bytes), st))
+            return fail(CRAG_E_HIP, "query split launch failed");
+        Fp4Args a = {};
+        a.queries = ws->qscan.p;
+        a.metric = h->metric;
+        a.sample = (uint32_t*)ws->sample.p;
+        a.sample_stride = stride;
+        a.rows = h->rows;
+        a.xnorm = h->xnorm;
+        a.row_end = n;
+        a.n_queries = B;
+        if (crag_launch_scan_fp4(a, h->dim_pad, false, h->n_cus, st)) return fail(CRAG_E_HIP, "4-bit scan launch failed");
+    } else if (path >= 2) {
         const bool d_bf16 = h->dtype == CRAG_BF16;
         MfmaArgs a;
         memset(&a, 0, sizeof(a));
@@ -1668,14 +1821,14 @@ int crag_debug_dense_scores(crag_index* h, const void* queries_dev, int B, int p
     }
     HIPCHK(hipStreamSynchronize(st));
     // keys -> floats on the host side of the boundary is the caller's job; here we decode on the host
-    std::vector<uint32_t> keys((size_t)(rowmajor ? bpad : B) * (size_t)(tiled ? (n + 31) / 32 * 32 : n));
+    std::vector<uint32_t> keys((size_t)(rowmajor ? bpad : B) * (size_t)(tiled ? (n + 31) / 32 * 32 : rowmajor ? n : stride));
     HIPCHK(hipMemcpy(keys.data(), ws->sample.p, keys.size() * 4, hipMemcpyDeviceToHost));
     std::vector<float> sc((size_t)B * (size_t)n);
     for (int b = 0; b < B; ++b)
         for (long long i = 0; i < n; ++i)
             sc[(size_t)b * n + i] = crag_fkey_inv(tiled      ? keys[((size_t)(i >> 5) * bpad + b) * 32 + (i & 31)]
                                                   : rowmajor ? keys[(size_t)i * bpad + b]
-                                                             : keys[(size_t)b * n + i]);
+                                                             : keys[(size_t)b * stride + i]);
     HIPCHK(hipMemcpy(out_scores_dev, sc.data(), sc.size() * 4, hipMemcpyHostToDevice));
     return 0;
 }
@@ -1699,6 +1852,76 @@ int crag_get_profile(crag_index* h, double* out4, int reset) {
 int crag_set_path(crag_index* h, int path) {
     if (!h || path < 0 || path > 3) return fail(CRAG_E_INVALID, "crag_set_path: bad arguments");
     h->force_path = path;
+    return 0;
+}
+
+int64_t crag_embed_workspace(int64_t n_tokens, int n_bags, int dim, int backward) {
+    if (n_tokens < 0 || n_tokens > 0x7fffffff || n_bags < 0 || dim <= 0) return fail(CRAG_E_INVALID, "crag_embed_workspace: bad arguments");
+    if (dim > CRAG_MAX_EMBED_DIM) return fail(CRAG_E_LIMIT, "crag_embed_workspace: more than 2048 elements per row");
+    return (int64_t)crag_embed_ws_bytes(n_tokens, n_bags, dim, backward != 0);
+}
+
+int crag_embed_forward_device(int device, const void* table_dev, int64_t vocab, int dim, int dtype, const int32_t* ids_dev,
+                              const float* weights_dev, int64_t n_tokens, const int64_t* offsets_dev, int n_bags, int mode, float scale,
+                              int normalize, void* out_dev, int out_dtype, float* coef_dev, void* workspace_dev, int64_t workspace_bytes,
+                              void* stream) {
+    CragEmbedArgs e = {};
+    int rc = check_embed("crag_embed_forward_device", table_dev, vocab, dim, dtype, ids_dev, n_tokens, offsets_dev, n_bags, workspace_dev, workspace_bytes, false);
+    if (rc) return rc;
+    if (mode < CRAG_POOL_SUM || mode > CRAG_POOL_SQRT) return fail(CRAG_E_INVALID, "crag_embed_forward_device: unknown pooling mode");
+    if (out_dtype != CRAG_F32 && out_dtype != CRAG_BF16) return fail(CRAG_E_INVALID, "crag_embed_forward_device: vectors are float32 or bf16");
+    if (n_bags == 0) return 0;
+    if (!out_dev) return fail(CRAG_E_INVALID, "crag_embed_forward_device: null output");
+    e.table = table_dev;
+    e.vocab = vocab;
+    e.dim = dim;
+    e.dtype = dtype;
+    e.ids = ids_dev;
+    e.weights = weights_dev;
+    e.n = n_tokens;
+    e.offsets = (const long long*)offsets_dev;
+    e.n_bags = n_bags;
+    e.mode = mode;
+    e.normalize = normalize;
+    e.scale = scale;
+    e.out = out_dev;
+    e.out_dtype = out_dtype;
+    e.coef = coef_dev;
+    e.workspace = workspace_dev;
+    DeviceGuard g(device);
+    if (g.rc) return fail(CRAG_E_INVALID, "crag_embed_forward_device: no such device");
+    if (crag_launch_embed_forward(e, (hipStream_t)stream)) return fail(CRAG_E_HIP, "embedding lookup launch failed");
+    return 0;
+}
+
+int crag_embed_backward_device(int device, const void* table_dev, int64_t vocab, int dim, int dtype, const int32_t* ids_dev,
+                               const float* weights_dev, int64_t n_tokens, const int64_t* offsets_dev, int n_bags, int normalize,
+                               const float* y_dev, const float* coef_dev, const float* grad_dev, void* d_table_dev, float* d_weights_dev,
+                               void* workspace_dev, int64_t workspace_bytes, void* stream) {
+    CragEmbedArgs e = {};
+    int rc = check_embed("crag_embed_backward_device", table_dev, vocab, dim, dtype, ids_dev, n_tokens, offsets_dev, n_bags, workspace_dev, workspace_bytes, true);
+    if (rc) return rc;
+    if (n_bags > 0 && (!coef_dev || !grad_dev || (normalize && !y_dev))) return fail(CRAG_E_INVALID, "crag_embed_backward_device: null buffer");
+    if (((uintptr_t)d_table_dev & 15) != 0) return fail(CRAG_E_INVALID, "crag_embed_backward_device: the table's gradient must be 16-byte aligned");
+    e.table = table_dev;
+    e.vocab = vocab;
+    e.dim = dim;
+    e.dtype = dtype;
+    e.ids = ids_dev;
+    e.weights = weights_dev;
+    e.n = n_tokens;
+    e.offsets = (const long long*)offsets_dev;
+    e.n_bags = n_bags;
+    e.normalize = normalize;
+    e.y = y_dev;
+    e.coef = const_cast<float*>(coef_dev);
+    e.grad = grad_dev;
+    e.d_table = d_table_dev;
+    e.d_weights = d_weights_dev;
+    e.workspace = workspace_dev;
+    DeviceGuard g(device);
+    if (g.rc) return fail(CRAG_E_INVALID, "crag_embed_backward_device: no such device");
+    if (crag_launch_embed_backward(e, (hipStream_t)stream)) return fail(CRAG_E_HIP, "embedding gradient launch failed");
     return 0;
 }
 

@@ -9,6 +9,7 @@
 
 #define CRAG_F32 0
 #define CRAG_BF16 1
+#define CRAG_FP4 2  // rows in 4 bits (crag_fp4.h); queries are float32
 #define CRAG_L2 0
 #define CRAG_IP 1
 
@@ -199,6 +200,7 @@ struct FinalizeArgs {
     const uint32_t* segcnt;           // segmented candidate buffer (see MfmaArgs) when n_seg > 0; then cnt is unused
     int n_seg, seg_cap;
     long long cand_stride;            // slots per query in cand (CRAG_CAND_CAP when flat)
+    const float* qres;                // 4-bit rows: norm of what the scan's pieces leave of each query; null elsewhere
     const int* qmap;                  // null: block b serves query b; else block b serves query qmap[b] (fallback passes)
 };
 int crag_launch_finalize(const FinalizeArgs& a, hipStream_t s);
@@ -232,6 +234,85 @@ struct ExactSelectArgs {
     unsigned int* cnt;
 };
 int crag_launch_exact_select(const ExactSelectArgs& a, hipStream_t s);
+
+// 4-bit rows (crag_scan_fp4.hip)
+struct Fp4Args {
+    const void* queries;  // pieces (crag_launch_fp4_split)
+    int metric;
+    const float* tau;
+    uint32_t* sample;  // [B][sample_stride] ordered-float keys
+    long long sample_stride;
+    unsigned long long* cand;  // flat buffers: [B][cand_stride], counts in cnt
+    long long cand_stride;
+    uint32_t* cnt;
+    // one collection (crag_launch_scan_fp4): rows [row_begin, row_end), row_begin a multiple of 32
+    const void* rows;
+    const float* xnorm;
+    long long row_begin, row_end;
+    int n_queries, wave_queries, query_groups;  // the latter two are the launcher's
+    // several collections (crag_launch_scan_fp4_groups): query block g holds the queries of group g, at most 16
+    const GroupDesc* groups;
+    int n_groups, pass;
+};
+#define CRAG_FP4_GROUP_Q 16  // most queries of the narrow form
+int crag_fp4_dim_pad(int dim);  // 0: too long
+int crag_fp4_query_blocks(int B, int dim_pad);
+long long crag_fp4_query_bytes(int n_blocks, int dim_pad, bool narrow);
+// residual[q]: norm of what the pieces of query q leave over
+int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_blocks, int B, int dim_pad, int metric, bool narrow, void* out,
+                          float* residual, hipStream_t s);
+int crag_launch_scan_fp4(const Fp4Args& a, int dim_pad, bool filter, int n_cus, hipStream_t s);
+int crag_launch_scan_fp4_groups(const Fp4Args& a, int dim_pad, int blocks, hipStream_t s);
+int crag_launch_fp4_quantize(const float* src, long long n, int dim, int dim_pad, long long first, void* dst, hipStream_t s);
+int crag_launch_fp4_dequantize(const void* rows, long long first, long long n, int dim, int dim_pad, float* out, hipStream_t s);
+int crag_launch_fp4_row_norms(const void* rows, int dim_pad, long long n, float* xnorm, float* max_out, hipStream_t s);
+
+// pooled embedding lookups and their gradient (crag_embed.hip)
+#define CRAG_POOL_SUM 0
+#define CRAG_POOL_MEAN 1
+#define CRAG_POOL_SQRT 2
+#define CRAG_MAX_EMBED_DIM 2048
+struct CragEmbedArgs {
+    const void* table;  // [vocab][dim], dtype
+    long long vocab;
+    int dim, dtype;
+    const int* ids;            // [n]
+    const float* weights;      // [n], may be null (ones)
+    long long n;
+    const long long* offsets;  // [n_bags + 1]
+    int n_bags, mode, normalize;
+    float scale;
+    // forward
+    void* out;  // [n_bags][dim], out_dtype
+    int out_dtype;
+    float* coef;  // [n_bags], may be null: what the backward pass scales a bag's gradient by
+    // backward
+    const float *y, *grad;  // [n_bags][dim]; y only read when normalize
+    void* d_table;          // [vocab][dim], dtype; may be null
+    float* d_weights;       // [n], may be null
+    void* workspace;
+};
+// a segmented sum of gathered rows (k_segsum): the same arguments for both directions
+struct CragSegArgs {
+    const void* src;   // rows that are gathered: the table, or the bags' gradients
+    long long n;       // positions
+    long long n_share; // groups of lanes, each walks `share` positions
+    int share, lpr, dim, vocab, n_seg;
+    const int* ids;            // forward
+    const float* weights;
+    const long long* offsets;  // forward
+    const uint32_t *keys, *perm;  // backward: sorted tokens and their positions
+    const int* bag;               // backward: bag of a position
+    float* partial;    // [n_share][2][dim]: sum of a segment that began in front of the share, of one that goes on behind it
+    int *partial_seg, *partial_count;  // [n_share][2]
+    void* out;
+    int out_dtype, mode, normalize;
+    float scale;
+    float* coef;
+};
+size_t crag_embed_ws_bytes(long long n, int n_bags, int dim, bool backward);
+int crag_launch_embed_forward(const CragEmbedArgs& e, hipStream_t s);
+int crag_launch_embed_backward(const CragEmbedArgs& e, hipStream_t s);
 
 // Kernels that take more than 64 KiB of dynamic LDS opt in once per (kernel, device): the attribute belongs
 // to the device that is current, and one process may hold collections on several devices.  `done` is the

@@ -1,0 +1,547 @@
+// Products of queries with 4-bit rows (layout: crag_fp4.h), for every batch size, and the kernels that lay rows and
+// queries out for them.
+//
+// Replaces the k-NN half of `col.query(query_texts=[q], n_results=2*top_k)` at retriever/hybrid_search.py:60-64 of the
+// reference on collections that hold a quarter of the bf16 rows' bytes.
+//
+// The matrix instructions multiply E2M1 codes with E2M3 codes, each group of 32 with its own power of two, and add in
+// float32: v_mfma_scale_f32_32x32x64_f8f6f4, 32 rows x 32 columns x 64 elements.  The stored rows ARE its A operand.  A
+// float32 query becomes the sum of two E2M3 pieces: the first is the nearest representable one, the second that of what
+// the first left over.  What both leave over, r = q - q1 - q2, is at most 2^-9 of a group's largest element; its norm
+// is computed per query, and |<r, x>| <= |r| max|x| enters the exactness certificate of the selection, which re-scores
+// the nearest rows from the float32 query in float64.  So results do not depend on the pieces at all, only how many rows
+// have to be re-scored does.
+// score s = |x|^2 - 2<q,x> (l2: the accumulators start at |x|^2, the pieces are those of -2q) or -<q,x> (ip).
+#include <algorithm>
+#include <utility>
+
+#include "crag_fp4.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) int i32x8_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+#define GLOBAL_AS __attribute__((address_space(1)))
+
+template <int N, typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    static_for_impl<N>(f, std::make_integer_sequence<int, N>{});
+}
+
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+// `CK` K steps of a tile of 32 rows as a wave holds them
+template <int CK>
+struct Codes {
+    u32x4_t c[CK];
+    __device__ __forceinline__ void load(const GLOBAL_AS unsigned char* tile, int step, int lane) {
+#pragma unroll
+        for (int k = 0; k < CK; ++k) c[k] = *(const GLOBAL_AS u32x4_t*)(tile + ((step + k) * 64 + lane) * 16);
+    }
+};
+template <int KS>
+struct RowScales {
+    uint32_t w[crag_fp4_sw(KS)];
+    __device__ __forceinline__ void load(const GLOBAL_AS unsigned char* tile, int lane) {
+        const GLOBAL_AS uint32_t* s = (const GLOBAL_AS uint32_t*)(tile + 1024 * KS) + lane * crag_fp4_sw(KS);
+#pragma unroll
+        for (int i = 0; i < crag_fp4_sw(KS); ++i) w[i] = s[i];
+    }
+};
+
+// 32 columns as a wave holds them
+template <int KS, int P>
+struct Query {
+    i32x8_t piece[KS * P];
+    uint32_t scale[crag_fp4_qsw(KS, P)];
+    __device__ __forceinline__ void load(const unsigned char* q, int lane) {
+#pragma unroll
+        for (int i = 0; i < KS * P; ++i) {
+            const u32x2_t* p = (const u32x2_t*)(q + ((long long)i * 64 + lane) * 24);
+            const u32x2_t a = p[0], b = p[1], c = p[2];
+            piece[i] = (i32x8_t){(int)a.x, (int)a.y, (int)b.x, (int)b.y, (int)c.x, (int)c.y, 0, 0};
+        }
+        const uint32_t* s = (const uint32_t*)(q + 64ll * 24 * KS * P) + lane * crag_fp4_qsw(KS, P);
+#pragma unroll
+        for (int w = 0; w < crag_fp4_qsw(KS, P); ++w) scale[w] = s[w];
+    }
+};
+
+template <int KS, int P, int QB, int STEP, int CK>
+__device__ __forceinline__ void products(const Codes<CK>& t, const RowScales<KS>& rs, const Query<KS, P> (&q)[QB], f32x16_t (&acc)[QB]) {
+    static_for<CK>([&](auto kc) {
+        constexpr int j = kc, k = STEP + j;
+        const i32x8_t a = {(int)t.c[j].x, (int)t.c[j].y, (int)t.c[j].z, (int)t.c[j].w, 0, 0, 0, 0};
+        static_for<P>([&](auto pc) {
+            constexpr int i = k * P + pc;
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+                acc[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[b].piece[i], acc[b], 4 /* A: E2M1 */, 2 /* B: E2M3 */, k % 4,
+                                                                         (int)rs.w[k / 4], i % 4, (int)q[b].scale[i / 4]);
+        });
+    });
+}
+
+// Lane l's accumulators: column l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4 of the tile (row0: the lane's first).
+// Rows behind the last one are filtered here; a threshold that is NaN (columns past the batch) lets nothing through.
+__device__ __forceinline__ void keep_survivors(const f32x16_t& s, float tau, int q, long long row0, long long row_end, const Fp4Args& a) {
+    float m = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = fminf(m, s[i]);
+    if (m <= tau) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const long long row = row0 + 8 * (i >> 2) + (i & 3);
+            if (s[i] <= tau && row < row_end) {
+                const uint32_t pos = atomicAdd(&a.cnt[CRAG_CNT(q)], 1u);
+                if (pos < CRAG_CAND_CAP) a.cand[q * a.cand_stride + pos] = ((unsigned long long)crag_fkey(s[i]) << 32) | (uint32_t)row;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void keep_all(const f32x16_t& s, int q, long long row0, const Fp4Args& a) {
+    if (q < 0) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)  // (rows behind the last one land in the sample's padding, which is a multiple of 64 rows)
+        *(u32x4_t*)(a.sample + q * a.sample_stride + row0 + 8 * r) =
+            (u32x4_t){crag_fkey(s[4 * r]), crag_fkey(s[4 * r + 1]), crag_fkey(s[4 * r + 2]), crag_fkey(s[4 * r + 3])};
+}
+
+// K steps a wave loads ahead: a whole tile, or what the registers of long rows leave room for
+constexpr int chunk_steps(int ks) { return ks <= 8 ? ks : (ks == 12 ? 6 : (ks == 32 ? 4 : 8)); }
+
+// Tiles first, first + step, ... < last.  P = 2: a column is a query.  P = 1: columns c and 16 + c are the pieces of query c.
+template <int KS, int P, int QB, bool FILTER>
+__device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, long long first, long long step, long long last, long long row_end,
+                                     const Fp4Args& a, const Query<KS, P> (&q)[QB], const float (&tau)[QB], const int (&qid)[QB], int lane) {
+    constexpr int CK = chunk_steps(KS), NCH = KS / CK;
+    static_assert(KS % CK == 0, "whole chunks");
+    const GLOBAL_AS unsigned char* rows = (const GLOBAL_AS unsigned char*)rows_;
+    const GLOBAL_AS float* xnorm = (const GLOBAL_AS float*)xnorm_;
+    const bool l2 = a.metric == CRAG_L2;
+    const bool start = l2 && (P == 2 || (lane & 16) == 0);  // the accumulators that begin at |x|^2
+    if (first >= last) return;
+    const GLOBAL_AS unsigned char* tile = rows + first * crag_fp4_tile_bytes(KS);
+    Codes<CK> cur;
+    RowScales<KS> rs;
+    f32x4_t xn[4];
+    auto load_norms = [&](long long t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            xn[r] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            if (start) xn[r] = *(const GLOBAL_AS f32x4_t*)(xnorm + t * 32 + 8 * r + (lane >> 5) * 4);
+        }
+    };
+    cur.load(tile, 0, lane);
+    rs.load(tile, lane);
+    load_norms(first);
+    for (long long t = first; t < last; t += step) {
+        const long long tn = t + step < last ? t + step : t;
+        const GLOBAL_AS unsigned char* tile_n = rows + tn * crag_fp4_tile_bytes(KS);
+        f32x16_t acc[QB];
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][i] = xn[i >> 2][i & 3];
+        RowScales<KS> rs_n;
+        rs_n.load(tile_n, lane);
+        load_norms(tn);
+        static_for<NCH>([&](auto cc) {
+            constexpr int c = cc;
+            Codes<CK> next;
+            if constexpr (c + 1 < NCH) next.load(tile, (c + 1) * CK, lane);
+            else next.load(tile_n, 0, lane);
+            products<KS, P, QB, c * CK, CK>(cur, rs, q, acc);
+            cur = next;
+        });
+        rs = rs_n;
+        tile = tile_n;
+        const long long row0 = t * 32 + (lane >> 5) * 4;
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            if constexpr (P == 1) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[b][i] += __shfl_xor(acc[b][i], 16);
+            }
+            if constexpr (FILTER) keep_survivors(acc[b], tau[b], qid[b], row0, row_end, a);
+            else keep_all(acc[b], qid[b], row0, a);
+        }
+    }
+}
+
+// One collection, more than 16 queries: rows [row_begin, row_end) for all of them.  A workgroup's waves take `wave_queries`
+// sets of 32 QB queries and 4 / wave_queries streams of tiles; workgroups on one stream that serve other queries sit on the
+// same XCD and share its L2.
+template <int KS, int QB, bool FILTER>
+__global__ __launch_bounds__(256, 1) void k_scan_fp4(Fp4Args a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wq = a.wave_queries, wr = 4 / wq;
+    const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int qg = slot % a.query_groups;
+    const long long stream = ((long long)(slot / a.query_groups) * 8 + xcd) * wr + wave / wq;
+    const long long streams = (long long)(gridDim.x / a.query_groups) * wr;
+    const int blk = (qg * wq + wave % wq) * QB;
+    Query<KS, 2> q[QB];
+    float tau[QB];
+    int qid[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        q[b].load((const unsigned char*)a.queries + (blk + b) * crag_fp4_qblock_bytes(KS, 2), lane);
+        const int id = (blk + b) * 32 + (lane & 31);
+        qid[b] = id < a.n_queries ? id : -1;
+        tau[b] = FILTER && id < a.n_queries ? a.tau[id] : __builtin_nanf("");
+    }
+    walk<KS, 2, QB, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + stream, streams, (a.row_end + 31) >> 5, a.row_end, a, q, tau, qid, lane);
+}
+
+// Up to 16 queries on one collection (groups == null), or several collections with groups of up to 16 queries each
+// (GroupDesc, as the float32 and bf16 scans have them).
+template <int KS, bool FILTER>
+__global__ __launch_bounds__(256) void k_scan_fp4_narrow(Fp4Args a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bid = blockIdx.x, c = lane & 31;
+    Query<KS, 1> q[1];
+    if (!a.groups) {
+        q[0].load((const unsigned char*)a.queries, lane);
+        const int qid[1] = {c < 16 && c < a.n_queries ? c : -1};
+        const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[c] : __builtin_nanf("")};
+        walk<KS, 1, 1, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + (long long)bid * 4 + wave, (long long)gridDim.x * 4, (a.row_end + 31) >> 5,
+                               a.row_end, a, q, tau, qid, lane);
+        return;
+    }
+    int g = 0;
+    for (int hi = a.n_groups; hi - g > 1;) {  // the last group whose first block is <= bid
+        const int mid = (g + hi) >> 1;
+        if (a.groups[mid].blk_first[a.pass] <= bid) g = mid; else hi = mid;
+    }
+    const GroupDesc& G = a.groups[g];
+    const long long row_end = a.pass == 0 ? G.n_sample : (a.pass == 1 ? G.n_mid : G.n_rows);
+    q[0].load((const unsigned char*)a.queries + g * crag_fp4_qblock_bytes(KS, 1), lane);
+    const int qid[1] = {c < 16 && c < G.nq ? G.q_first + c : -1};
+    const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[G.q_first + c] : __builtin_nanf("")};
+    const long long first = (long long)(bid - G.blk_first[a.pass]) * 4 + wave;
+    walk<KS, 1, 1, FILTER>(G.rows, G.xnorm, (G.from[a.pass] >> 5) + first, (long long)G.n_blk[a.pass] * 4, (row_end + 31) >> 5, row_end, a, q, tau, qid,
+                           lane);
+}
+
+// ---- queries: float32 -> two E2M3 pieces ---------------------------------------------------------------------------------
+// nearest E2M3 value of t (|t| <= 7.5), its code
+__device__ __forceinline__ float e2m3(float t, uint32_t* code) {
+    const float m = fabsf(t);
+    float r;
+    uint32_t c;
+    if (m < 2.f) {
+        const float k = rintf(m * 8.f);
+        r = k * 0.125f;
+        c = (uint32_t)k;
+    } else if (m < 4.f) {
+        const float k = rintf(m * 4.f);
+        r = k * 0.25f;
+        c = (uint32_t)k + 8u;
+    } else {
+        const float k = rintf(m * 2.f);
+        r = k * 0.5f;
+        c = (uint32_t)k + 16u;
+    }
+    *code = c | (t < 0.f ? 32u : 0u);
+    return t < 0.f ? -r : r;
+}
+
+// One wave per query slot; lane l splits group l (dim_pad / 32 <= 64 groups).  Wide: slot = query, 32 to a block.  Narrow:
+// 16 slots to a block; with `groups`, block g holds the queries of group g.
+__global__ __launch_bounds__(64) void k_fp4_split(const float* __restrict__ queries, const GroupDesc* __restrict__ groups, int n_queries,
+                                                  int dim_pad, int metric, int narrow, unsigned char* __restrict__ out, float* __restrict__ residual) {
+    const int per = narrow ? 16 : 32, pieces = narrow ? 1 : 2;
+    const int blk = blockIdx.x / per, col = blockIdx.x % per, lane = threadIdx.x;
+    int q;
+    if (groups) q = col < groups[blk].nq ? groups[blk].q_first + col : -1;
+    else q = (int)blockIdx.x < n_queries ? (int)blockIdx.x : -1;
+    const int ks = dim_pad >> 6, n_grp = dim_pad >> 5;
+    unsigned char* base = out + blk * crag_fp4_qblock_bytes(ks, pieces);
+    double left = 0.0;
+    if (lane < n_grp) {
+        float v[32];
+        bool finite = true;
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+            if (q >= 0) x = *(const f32x4_t*)(queries + (long long)q * dim_pad + lane * 32 + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[j + k] = -x[k];
+                finite = finite && fabsf(x[k]) <= 1.329227995784916e36f;  // 2^120: beyond it nothing is split, and everything left over
+                big = fmaxf(big, fabsf(x[k]));
+            }
+        }
+        const int k = lane >> 1, half = (lane & 1) * 32;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            int ex;
+            const float m = frexpf(big, &ex);
+            int e = ex - (m > 0.9375f ? 2 : 3);  // the smallest with big <= 7.5 * 2^e
+            e = e < -120 || !finite ? -120 : e;
+            const float down = ldexpf(1.f, -e), up = ldexpf(1.f, e);
+            uint32_t w[6] = {0, 0, 0, 0, 0, 0};
+            float rest = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                uint32_t c = 0;
+                if (finite) {
+                    const float r = e2m3(v[j] * down, &c);
+                    v[j] -= r * up;
+                    rest = fmaxf(rest, fabsf(v[j]));
+                }
+                const int bit = 6 * j;
+                w[bit >> 5] |= c << (bit & 31);
+                if ((bit & 31) > 26) w[(bit >> 5) + 1] |= c >> (32 - (bit & 31));
+            }
+            big = rest;
+            const int i = narrow ? k : 2 * k + p, at = half + (narrow ? 16 * p + col : col);
+            u32x2_t* o = (u32x2_t*)(base + ((long long)i * 64 + at) * 24);
+            o[0] = (u32x2_t){w[0], w[1]};
+            o[1] = (u32x2_t){w[2], w[3]};
+            o[2] = (u32x2_t){w[4], w[5]};
+            // -2q is -q with a scale twice as large
+            base[64ll * 24 * ks * pieces + (long long)at * 4 * crag_fp4_qsw(ks, pieces) + i] = (unsigned char)(e + 127 + (metric == CRAG_L2 ? 1 : 0));
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) left += (double)v[j] * (double)v[j];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) left += __shfl_xor(left, o);
+    if (lane == 0 && q >= 0) residual[q] = nextafterf((float)sqrt(left), __builtin_inff());
+}
+
+// ---- rows ------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t e2m1(float v) {  // |v| <= 7, nearest code, ties to the even one
+    const float m = fabsf(v);
+    const uint32_t c = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.f);
+    return c | (v < 0.f ? 8u : 0u);
+}
+
+// eight lanes per group of 32: float32 rows [n][dim] -> rows first .. first + n of the tiles
+template <bool VEC>
+__global__ __launch_bounds__(256) void k_fp4_quantize(const float* __restrict__ src, long long n, int dim, int dim_pad, long long first,
+                                                      unsigned char* __restrict__ dst) {
+    const int n_grp = dim_pad >> 5;
+    const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) >> 3;
+    const int part = threadIdx.x & 7;
+    const long long i = unit / n_grp;
+    const int grp = (int)(unit - i * n_grp);
+    const bool on = i < n;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int e0 = grp * 32 + part * 4;
+    if (on) {
+        if constexpr (VEC) {
+            if (e0 < dim) {
+                const f32x4_t x = *(const f32x4_t*)(src + i * dim + e0);
+                v[0] = x[0]; v[1] = x[1]; v[2] = x[2]; v[3] = x[3];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (e0 + k < dim) v[k] = src[i * dim + e0 + k];
+        }
+    }
+    float big = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    int bad = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bad |= fabsf(v[k]) <= 3.4028234663852886e38f ? 0 : 1;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        big = fmaxf(big, __shfl_xor(big, o));
+        bad |= __shfl_xor(bad, o);
+    }
+    int ex;
+    const float m = frexpf(big, &ex);
+    int e = ex - (m > 0.875f ? 2 : 3);
+    e = e < CRAG_FP4_EXP_MIN ? CRAG_FP4_EXP_MIN : (e > CRAG_FP4_EXP_MAX ? CRAG_FP4_EXP_MAX : e);
+    const float down = ldexpf(1.f, -e);
+    uint32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c |= (bad ? 0u : e2m1(v[k] * down)) << (4 * k);
+    // lane 0 of the eight gathers the 16 bytes
+    const uint32_t w = c | (__shfl_down(c, 1, 8) << 16);
+    const uint32_t w1 = __shfl_down(w, 2, 8), w2 = __shfl_down(w, 4, 8), w3 = __shfl_down(w, 6, 8);
+    if (on && part == 0) {
+        long long at, sc;
+        crag_fp4_place(dim_pad, first + i, grp, &at, &sc);
+        *(u32x4_t*)(dst + at) = (u32x4_t){w, w1, w2, w3};
+        dst[sc] = bad ? 255 : (unsigned char)(e + 127);
+    }
+}
+
+// rows first .. first + n back to float32 [n][dim]: a thread per group of 32
+__global__ __launch_bounds__(256) void k_fp4_dequantize(const unsigned char* __restrict__ rows, long long first, long long n, int dim, int dim_pad,
+                                                        float* __restrict__ out) {
+    const int n_grp = (dim + 31) / 32;
+    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long i = unit / n_grp;
+    if (i >= n) return;
+    const int grp = (int)(unit - i * n_grp);
+    long long at, sc;
+    crag_fp4_place(dim_pad, first + i, grp, &at, &sc);
+    const u32x4_t w = *(const u32x4_t*)(rows + at);
+    const float s = crag_fp4_scale(rows[sc]);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (grp * 32 + j < dim) out[i * dim + grp * 32 + j] = crag_fp4_value((w[j >> 3] >> (4 * (j & 7))) & 15u, s);
+}
+
+// |x|^2 per row and their maximum: a wave per tile, summed in float64
+__global__ __launch_bounds__(256) void k_fp4_row_norms(const unsigned char* __restrict__ rows, int dim_pad, long long n, float* __restrict__ xnorm,
+                                                       unsigned int* __restrict__ max_bits) {
+    const int lane = threadIdx.x & 63, ks = dim_pad >> 6;
+    const long long waves = (long long)gridDim.x * 4;
+    float wmax = 0.f;
+    for (long long t = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); t * 32 < n; t += waves) {
+        const long long row = t * 32 + (lane & 31);
+        double acc = 0.0;
+        for (int k = 0; k < ks; ++k) {
+            long long at, sc;
+            crag_fp4_place(dim_pad, row, k * 2 + (lane >> 5), &at, &sc);
+            const u32x4_t w = *(const u32x4_t*)(rows + at);
+            const float s = crag_fp4_scale(rows[sc]);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const double v = (double)crag_fp4_value((w[j >> 3] >> (4 * (j & 7))) & 15u, s);
+                acc += v * v;
+            }
+        }
+        acc += __shfl_xor(acc, 32);
+        if (row < n) {
+            const float f = (float)acc;
+            if (lane < 32) xnorm[row] = f;
+            wmax = fmaxf(wmax, f == f ? f : __builtin_inff());
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) wmax = fmaxf(wmax, __shfl_xor(wmax, o));
+    if (lane == 0) atomicMax(max_bits, __builtin_bit_cast(unsigned int, wmax));
+}
+
+// sets of 32 queries a wave holds: what its registers take beside the rows in flight
+constexpr int max_qb(int ks) { return ks <= 12 ? 2 : 1; }
+int wide_qb(int B, int ks) { return B <= 32 ? 1 : max_qb(ks); }
+int wide_waves(int B, int ks) {
+    const int sets = (B + 32 * wide_qb(B, ks) - 1) / (32 * wide_qb(B, ks));
+    return sets >= 3 ? 4 : sets;
+}
+
+template <int KS>
+int launch_wide(const Fp4Args& a, int qb, int blocks, bool filter, hipStream_t s) {
+    if (qb == 1) {
+        if (filter) hipLaunchKernelGGL((k_scan_fp4<KS, 1, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_scan_fp4<KS, 1, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    } else {
+        if (filter) hipLaunchKernelGGL((k_scan_fp4<KS, max_qb(KS), true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_scan_fp4<KS, max_qb(KS), false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    }
+    return (int)hipGetLastError();
+}
+template <int KS>
+int launch_narrow(const Fp4Args& a, int blocks, bool filter, hipStream_t s) {
+    if (filter) hipLaunchKernelGGL((k_scan_fp4_narrow<KS, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_scan_fp4_narrow<KS, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    return (int)hipGetLastError();
+}
+#define CRAG_FP4_KS(X) X(2) X(4) X(6) X(8) X(12) X(16) X(24) X(32)
+#define CRAG_FP4_DISPATCH(dim_pad, call) \
+    switch ((dim_pad) >> 6) {            \
+        CRAG_FP4_KS(call)                \
+    }                                    \
+    return -1;
+
+}  // namespace
+
+int crag_fp4_dim_pad(int dim) {
+#define X(K) \
+    if (dim <= 64 * K) return 64 * K;
+    CRAG_FP4_KS(X)
+#undef X
+    return 0;
+}
+
+// query blocks of the single-collection scan for B queries (the wide form's waves take whole sets of them)
+int crag_fp4_query_blocks(int B, int dim_pad) {
+    if (B <= CRAG_FP4_GROUP_Q) return 1;
+    const int per = wide_qb(B, dim_pad >> 6) * wide_waves(B, dim_pad >> 6);
+    return ((B + 31) / 32 + per - 1) / per * per;
+}
+long long crag_fp4_query_bytes(int n_blocks, int dim_pad, bool narrow) { return n_blocks * crag_fp4_qblock_bytes(dim_pad >> 6, narrow ? 1 : 2); }
+
+int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_blocks, int B, int dim_pad, int metric, bool narrow, void* out,
+                          float* residual, hipStream_t s) {
+    hipLaunchKernelGGL(k_fp4_split, dim3((unsigned)n_blocks * (narrow ? 16u : 32u)), dim3(64), 0, s, (const float*)queries, groups, B, dim_pad, metric,
+                       narrow ? 1 : 0, (unsigned char*)out, residual);
+    return (int)hipGetLastError();
+}
+
+int crag_launch_scan_fp4(const Fp4Args& args, int dim_pad, bool filter, int n_cus, hipStream_t s) {
+    Fp4Args a = args;
+    a.groups = nullptr;
+    if (a.row_end <= a.row_begin) return 0;
+    const int ks = dim_pad >> 6, B = a.n_queries;
+    const long long tiles = ((a.row_end + 31) >> 5) - (a.row_begin >> 5);
+    if (B <= CRAG_FP4_GROUP_Q) {
+        const int blocks = (int)std::min<long long>((tiles + 3) / 4, 2ll * n_cus);
+#define X(K) \
+    case K: return launch_narrow<K>(a, blocks, filter, s);
+        CRAG_FP4_DISPATCH(dim_pad, X)
+#undef X
+    }
+    const int qb = wide_qb(B, ks), sets = (B + 32 * qb - 1) / (32 * qb);
+    a.wave_queries = wide_waves(B, ks);
+    a.query_groups = (sets + a.wave_queries - 1) / a.wave_queries;
+    const int wr = 4 / a.wave_queries;
+    // streams of tiles: a multiple of eight (one share per XCD), no more than there are tiles
+    long long streams = std::max<long long>(1, n_cus / a.query_groups);
+    streams = std::min(streams, (tiles + wr - 1) / wr);
+    streams = (streams + 7) / 8 * 8;
+    const int blocks = (int)(streams * a.query_groups);
+#define X(K) \
+    case K: return launch_wide<K>(a, qb, blocks, filter, s);
+    CRAG_FP4_DISPATCH(dim_pad, X)
+#undef X
+}
+
+int crag_launch_scan_fp4_groups(const Fp4Args& a, int dim_pad, int blocks, hipStream_t s) {
+    if (blocks <= 0) return 0;
+#define X(K) \
+    case K: return launch_narrow<K>(a, blocks, a.pass != 0, s);
+    CRAG_FP4_DISPATCH(dim_pad, X)
+#undef X
+}
+
+int crag_launch_fp4_quantize(const float* src, long long n, int dim, int dim_pad, long long first, void* dst, hipStream_t s) {
+    if (n <= 0) return 0;
+    const bool vec = dim % 4 == 0 && ((uintptr_t)src & 15) == 0;
+    const long long rows_at_once = (1ll << 30) / (dim_pad >> 5);  // keeps the grid within 32 bits
+    for (long long i = 0; i < n; i += rows_at_once) {
+        const long long m = std::min(rows_at_once, n - i), blocks = (m * (dim_pad >> 5) * 8 + 255) / 256;
+        if (vec) hipLaunchKernelGGL(k_fp4_quantize<true>, dim3((unsigned)blocks), dim3(256), 0, s, src + i * dim, m, dim, dim_pad, first + i, (unsigned char*)dst);
+        else hipLaunchKernelGGL(k_fp4_quantize<false>, dim3((unsigned)blocks), dim3(256), 0, s, src + i * dim, m, dim, dim_pad, first + i, (unsigned char*)dst);
+    }
+    return (int)hipGetLastError();
+}
+
+int crag_launch_fp4_dequantize(const void* rows, long long first, long long n, int dim, int dim_pad, float* out, hipStream_t s) {
+    if (n <= 0) return 0;
+    const long long blocks = (n * ((dim + 31) / 32) + 255) / 256;
+    hipLaunchKernelGGL(k_fp4_dequantize, dim3((unsigned)blocks), dim3(256), 0, s, (const unsigned char*)rows, first, n, dim, dim_pad, out);
+    return (int)hipGetLastError();
+}
+
+int crag_launch_fp4_row_norms(const void* rows, int dim_pad, long long n, float* xnorm, float* max_out, hipStream_t s) {
+    if (n <= 0) return 0;
+    const long long blocks = std::min<long long>(8192, ((n + 31) / 32 + 3) / 4);
+    hipLaunchKernelGGL(k_fp4_row_norms, dim3((unsigned)blocks), dim3(256), 0, s, (const unsigned char*)rows, dim_pad, n, xnorm, (unsigned int*)max_out);
+    return (int)hipGetLastError();
+}

@@ -14,11 +14,12 @@
 //                                           fallback tier 2: canonical distance of every row + radix select, batched
 //                                           over the failed queries, no host round trip between the passes
 #include "crag_common.h"
+#include "crag_fp4.h"
 
 namespace {
 
 __device__ __forceinline__ double load_elem_f64(const void* p, int dtype, long long idx) {
-    if (dtype == CRAG_F32) return (double)((const float*)p)[idx];
+    if (dtype != CRAG_BF16) return (double)((const float*)p)[idx];  // float32, and the queries of 4-bit rows
     uint32_t u = ((uint32_t)((const unsigned short*)p)[idx]) << 16;
     return (double)__builtin_bit_cast(float, u);
 }
@@ -336,8 +337,37 @@ __device__ __forceinline__ double canon_lane_t(const void* row, const void* q, i
 }
 __device__ __forceinline__ double canon_lane(const void* row, const void* q, int dtype, int dim, int j, int metric,
                                              long long row_off) {
-    return dtype == CRAG_F32 ? canon_lane_t<CRAG_F32>(row, q, dim, j, metric, row_off)
+    return dtype != CRAG_BF16 ? canon_lane_t<CRAG_F32>(row, q, dim, j, metric, row_off)
                              : canon_lane_t<CRAG_BF16>(row, q, dim, j, metric, row_off);
+}
+
+// the same partial sum of a 4-bit row in the tiles of crag_fp4.h: of a group's four words of eight codes, lane j takes
+// code j of each
+__device__ __forceinline__ double canon_lane_fp4(const void* rows, const float* q, int dim, int dim_pad, long long row, int j, int metric) {
+    double acc = 0.0;
+    for (int g = 0; g * 32 < dim; ++g) {
+        long long at, sc;
+        crag_fp4_place(dim_pad, row, g, &at, &sc);
+        const uint4 c = *(const uint4*)((const unsigned char*)rows + at);
+        const float s = crag_fp4_scale(((const unsigned char*)rows)[sc]);
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int d = g * 32 + 8 * u + j;
+            if (d < dim) {
+                const double a = (double)q[d], b = (double)crag_fp4_value((w[u] >> (4 * j)) & 15u, s);
+                double p;
+                if (metric == CRAG_L2) {
+                    const double t = __dsub_rn(a, b);
+                    p = __dmul_rn(t, t);
+                } else {
+                    p = __dmul_rn(a, b);
+                }
+                acc = __dadd_rn(acc, p);
+            }
+        }
+    }
+    return acc;
 }
 
 __device__ __forceinline__ double combine8(double acc) {
@@ -429,7 +459,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         __syncthreads();
         bitonic_sort_u64(skeys, P);
     }
-    const size_t esz = a.dtype == CRAG_F32 ? 4 : 2;
+    const size_t esz = a.dtype == CRAG_BF16 ? 2 : 4;
     const void* qv = (const char*)a.queries + (size_t)q * a.dim_pad * esz;
 
     // |q|^2 in fp64 (error bound only)
@@ -471,9 +501,10 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     // 128-KiB region is free now), so the order-defining add chains read LDS instead of chasing 2-byte loads
     {
         unsigned char* stage_q = (unsigned char*)(skeys + 1024);  // m + 1 <= CRAG_MAX_M + 1 <= 1024 keys stay live
-        unsigned char* stage_r = stage_q + 4096;                  // dim_pad * esz <= 4096
-        const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;
-        int rpr = (int)((sizeof(unsigned long long) * (CRAG_CAND_CAP - 1024) - 4096) / (size_t)row_bytes);
+        const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;  // (4-bit rows are staged as float32)
+        const int q_bytes = row_bytes > 4096 ? row_bytes : 4096;
+        unsigned char* stage_r = stage_q + q_bytes;
+        int rpr = (int)((sizeof(unsigned long long) * (CRAG_CAND_CAP - 1024) - q_bytes) / (size_t)row_bytes);
         if (rpr > 128) rpr = 128;  // 1024 threads / 8 lanes
         for (int c = tid; c < chunks; c += 1024) ((uint4*)stage_q)[c] = ((const uint4*)qv)[c];
         for (int base = 0; base < m; base += rpr) {
@@ -483,22 +514,44 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             // which makes it a generic pointer to the compiler, and FLAT loads are waited for one at a time
             typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
             const __attribute__((address_space(1))) u32x4_t* grows = (const __attribute__((address_space(1))) u32x4_t*)D.rows;
-            const int total = nr * chunks;
-            for (int idx0 = tid; idx0 < total; idx0 += 4 * 1024) {
-                u32x4_t v[4];
+            if (a.dtype == CRAG_FP4) {
+                // one group of 32 codes per thread, decoded into 128 bytes of float32
+                const int n_grp = a.dim_pad >> 5, total = nr * n_grp;
+                const __attribute__((address_space(1))) unsigned char* grow = (const __attribute__((address_space(1))) unsigned char*)D.rows;
+                for (int idx = tid; idx < total; idx += 1024) {
+                    const int r = idx / n_grp, g = idx - r * n_grp;
+                    long long at, sc;
+                    crag_fp4_place(a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), g, &at, &sc);
+                    const u32x4_t c = *(const __attribute__((address_space(1))) u32x4_t*)(grow + at);
+                    const float s = crag_fp4_scale(grow[sc]);
+                    float4* o = (float4*)(stage_r + (size_t)r * row_bytes + g * 128);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int idx = idx0 + u * 1024;
-                    if (idx < total) {
-                        const int r = idx / chunks, c = idx - r * chunks;
-                        const uint32_t row = (uint32_t)(skeys[base + r] & 0xffffffffull);
-                        v[u] = grows[(long long)row * chunks + c];
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t w = c[u];
+                        o[2 * u] = make_float4(crag_fp4_value(w & 15u, s), crag_fp4_value((w >> 4) & 15u, s), crag_fp4_value((w >> 8) & 15u, s),
+                                               crag_fp4_value((w >> 12) & 15u, s));
+                        o[2 * u + 1] = make_float4(crag_fp4_value((w >> 16) & 15u, s), crag_fp4_value((w >> 20) & 15u, s),
+                                                   crag_fp4_value((w >> 24) & 15u, s), crag_fp4_value(w >> 28, s));
                     }
                 }
+            } else {
+                const int total = nr * chunks;
+                for (int idx0 = tid; idx0 < total; idx0 += 4 * 1024) {
+                    u32x4_t v[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int idx = idx0 + u * 1024;
-                    if (idx < total) ((u32x4_t*)stage_r)[idx] = v[u];
+                    for (int u = 0; u < 4; ++u) {
+                        const int idx = idx0 + u * 1024;
+                        if (idx < total) {
+                            const int r = idx / chunks, c = idx - r * chunks;
+                            const uint32_t row = (uint32_t)(skeys[base + r] & 0xffffffffull);
+                            v[u] = grows[(long long)row * chunks + c];
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int idx = idx0 + u * 1024;
+                        if (idx < total) ((u32x4_t*)stage_r)[idx] = v[u];
+                    }
                 }
             }
             __syncthreads();
@@ -573,15 +626,17 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             const double u = 5.9604644775390625e-08;  // 2^-24
             const double X = (double)D.max_xnorm;
             const double qx = sqrt(qn * X);
+            // 4-bit rows: the scan multiplied pieces of the query (crag_scan_fp4.hip); <what they leave over, x> is at most this
+            const double rest = a.qres ? (double)a.qres[q] * sqrt(X) * 1.0000001 + 1e-34 : 0.0;
             double eps, lb;
             if (a.metric == CRAG_L2) {
                 // every partial sum of a scan is bounded by |x|^2 + 2 |q||x|: the 16x16x32 scan starts its accumulators
                 // at |x|^2 (crag_scan_q16.hip); the others add |x|^2 last, which this bound covers as well
                 eps = 2.0 * u * ((double)(a.dim_pad + 4) * (2.0 * qx + X) + 3.0 * X + 1e-30);
-                lb = sM + qn - eps - 1e-12 * (qn + X);
+                lb = sM + qn - eps - 2.0 * rest - 1e-12 * (qn + X);
             } else {
                 eps = 2.0 * u * ((double)(a.dim_pad + 4) * qx + 1e-30);
-                lb = 1.0 + sM - eps - 1e-12 * (1.0 + qx);
+                lb = 1.0 + sM - eps - rest - 1e-12 * (1.0 + qx);
             }
             float lbf = (float)lb;
             if ((double)lbf > lb) lbf = nextafterf(lbf, -__builtin_inff());
@@ -698,7 +753,7 @@ __global__ __launch_bounds__(1024) void k_rescore_wide(FinalizeArgs a, unsigned 
     }
     if (c > CRAG_CAND_CAP) c = CRAG_CAND_CAP;  // (an overflowed query goes to tier 2 anyway)
     unsigned long long* __restrict__ cq = cand_rw + (long long)q * a.cand_stride;
-    const size_t esz = a.dtype == CRAG_F32 ? 4 : 2;
+    const size_t esz = a.dtype == CRAG_BF16 ? 2 : 4;
     const void* qv = (const char*)a.queries + (size_t)q * a.dim_pad * esz;
     const int j = tid & 7;
     for (int i0 = 0; i0 < c; i0 += 128) {  // the trip count is block-uniform: combine8 shuffles among all lanes
@@ -709,7 +764,8 @@ __global__ __launch_bounds__(1024) void k_rescore_wide(FinalizeArgs a, unsigned 
         if (i < c) {
             slot = seg ? seg_slot(seg_off, a.n_seg, a.seg_cap, i) : i;
             row = (uint32_t)(cq[slot] & 0xffffffffull);
-            acc = canon_lane(D.rows, qv, a.dtype, a.dim, j, a.metric, (long long)row * a.dim_pad);
+            acc = a.dtype == CRAG_FP4 ? canon_lane_fp4(D.rows, (const float*)qv, a.dim, a.dim_pad, (long long)row, j, a.metric)
+                                      : canon_lane(D.rows, qv, a.dtype, a.dim, j, a.metric, (long long)row * a.dim_pad);
         }
         acc = combine8(acc);
         if (i < c && j == 0) {
@@ -737,7 +793,7 @@ __global__ __launch_bounds__(256) void k_tau_refine(FinalizeArgs a, float* __res
         return;
     }
     const QueryDesc D = a.qd[q];
-    const size_t esz = a.dtype == CRAG_F32 ? 4 : 2;
+    const size_t esz = a.dtype == CRAG_BF16 ? 2 : 4;
     const void* qv = (const char*)a.queries + (size_t)q * a.dim_pad * esz;
     double part = 0.0;
     for (int d = tid; d < a.dim; d += 256) {
@@ -755,13 +811,14 @@ __global__ __launch_bounds__(256) void k_tau_refine(FinalizeArgs a, float* __res
         const double u = 5.9604644775390625e-08;  // 2^-24
         const double X = (double)D.max_xnorm;
         const double qx = sqrt(qn * X);
+        const double rest = a.qres ? (double)a.qres[q] * sqrt(X) * 1.0000001 + 1e-34 : 0.0;  // as in k_finalize
         double t;
         if (a.metric == CRAG_L2) {
             const double eps = 2.0 * u * ((double)(a.dim_pad + 4) * (2.0 * qx + X) + 3.0 * X + 1e-30);
-            t = (double)d0 - qn + 1.01 * eps + 2e-12 * (qn + X);
+            t = (double)d0 - qn + 1.01 * (eps + 2.0 * rest) + 2e-12 * (qn + X);
         } else {
             const double eps = 2.0 * u * ((double)(a.dim_pad + 4) * qx + 1e-30);
-            t = (double)d0 - 1.0 + 1.01 * eps + 2e-12 * (1.0 + qx);
+            t = (double)d0 - 1.0 + 1.01 * (eps + rest) + 2e-12 * (1.0 + qx);
         }
         float tf = (float)t;
         if ((double)tf < t) tf = nextafterf(tf, __builtin_inff());
@@ -785,7 +842,7 @@ __global__ __launch_bounds__(256) void k_exact_keys_b(const QueryDesc* __restric
     const long long n = qd[q].n_rows;
     if (r >= n) return;
     const void* __restrict__ rows = qd[q].rows;
-    const size_t esz = dtype == CRAG_F32 ? 4 : 2;
+    const size_t esz = dtype == CRAG_BF16 ? 2 : 4;
     const void* query = (const char*)queries + (size_t)q * dim_pad * esz;  // staged: stride dim_pad, zero-padded
     double acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     // eight elements per step through 16-byte loads (rows and staged queries are zero-padded to dim_pad, a multiple of
@@ -797,7 +854,20 @@ __global__ __launch_bounds__(256) void k_exact_keys_b(const QueryDesc* __restric
     const uint4* __restrict__ qv4 = (const uint4*)query;
     for (int d0 = 0; d0 < dim; d0 += 8) {
         double x[8], y[8];
-        if (dtype == CRAG_F32) {
+        if (dtype == CRAG_FP4) {  // eight codes = one word of the group
+            long long at, sc;
+            crag_fp4_place(dim_pad, r, d0 >> 5, &at, &sc);
+            const __attribute__((address_space(1))) unsigned char* grow = (const __attribute__((address_space(1))) unsigned char*)rows;
+            const uint32_t w = *(const __attribute__((address_space(1))) uint32_t*)(grow + at + ((d0 >> 3) & 3) * 4);
+            const float s = crag_fp4_scale(grow[sc]);
+            const uint4 a0 = qv4[d0 >> 2], a1 = qv4[(d0 >> 2) + 1];
+            const uint32_t aw[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = (double)__builtin_bit_cast(float, aw[j]);
+                y[j] = (double)crag_fp4_value((w >> (4 * j)) & 15u, s);
+            }
+        } else if (dtype == CRAG_F32) {
             const uint4 a0 = qv4[d0 >> 2], a1 = qv4[(d0 >> 2) + 1];
             const u32x4_t b0 = rv[d0 >> 2], b1 = rv[(d0 >> 2) + 1];
             const uint32_t aw[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};

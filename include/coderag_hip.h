@@ -22,6 +22,8 @@
  *                                                          (device buffers)
  *   row-sharded corpus over the GPUs of one node           crag_search_local_device +
  *     (no reference counterpart; north_star)               crag_merge_rerank_device
+ *   the embedding function in front of the search           crag_embed_forward_device,
+ *     (retriever/hybrid_search.py:23,60-64)                 crag_embed_backward_device
  *
  * Conventions: every function returns 0 on success or a negative CRAG_E_* code; no C++
  * exception crosses this boundary; the caller allocates every in/out buffer; the library owns
@@ -41,6 +43,12 @@ extern "C" {
 
 #define CRAG_DTYPE_F32 0
 #define CRAG_DTYPE_BF16 1
+/* rows held in 4 bits: E2M1 codes with one power-of-two scale per 32 elements (4.25 bits an element), up to 2048 elements.
+ * Rows and queries cross this boundary as float32; the library converts rows when they are added (each scale the smallest
+ * that keeps its group within 7 units, each element the nearest code) and never rounds a query: searches are exact -- by
+ * (float32 distance, id) -- with respect to the rows as they are held, which crag_index_get_rows returns.  Such a
+ * collection answers bit for bit like a float32 collection that was given crag_index_get_rows' rows. */
+#define CRAG_DTYPE_FP4 2
 #define CRAG_METRIC_L2 0 /* squared L2: Chroma's default space, what the reference uses */
 #define CRAG_METRIC_IP 1 /* Chroma "ip": 1 - <q,x> */
 
@@ -75,7 +83,7 @@ int crag_index_set_id_base(crag_index* h, int64_t id_base);
 
 /*
  * Append n rows from HOST memory.  rows: [n][dim] in the index dtype (bf16 = uint16 bit
- * patterns).  name_hash[n] (crag_hash_name of the lowered chunk name, 0 = no name),
+ * patterns, fp4 = float32).  name_hash[n] (crag_hash_name of the lowered chunk name, 0 = no name),
  * name_len[n] (UTF-8 byte length of the lowered name) and path_class[n] (0 neutral,
  * 1 penalised, 2 boosted; hybrid_search.py:105-111) may each be NULL.
  */
@@ -86,7 +94,7 @@ int crag_index_add_device(crag_index* h, const void* rows_dev, int64_t n, const 
                           const uint8_t* path_class_dev);
 /*
  * Zero-copy: adopt caller-owned DEVICE arrays as the whole collection (they must outlive the
- * handle).  Requires dim == crag_index_dim_pad and 16-byte aligned rows.
+ * handle).  Requires dim == crag_index_dim_pad and 16-byte aligned rows.  Not for CRAG_DTYPE_FP4.
  */
 int crag_index_attach_device(crag_index* h, const void* rows_dev, int64_t n, const uint64_t* name_hash_dev,
                              const uint8_t* path_class_dev);
@@ -96,7 +104,8 @@ int crag_index_attach_device(crag_index* h, const void* rows_dev, int64_t n, con
  */
 int crag_index_set_symbols(crag_index* h, const uint64_t* hashes, const uint16_t* lens, int64_t n);
 /*
- * Copy rows [first, first + n) back to HOST memory as [n][dim] in the index dtype (bf16 = uint16 bit patterns):
+ * Copy rows [first, first + n) back to HOST memory as [n][dim] in the index dtype (bf16 = uint16 bit patterns, fp4 =
+ * float32, the values that the codes stand for; adding them again gives the same codes):
  * what persistence writes to disk, so that no second copy of the embeddings has to live in host memory.
  */
 int crag_index_get_rows(const crag_index* h, int64_t first, int64_t n, void* out_rows);
@@ -121,7 +130,7 @@ int crag_symbol_hashes(const crag_index* h, const char* q_lower_utf8, int64_t le
 /*
  * HybridSearcher.search for a batch of B queries against ONE collection, host buffers.
  *   queries      [B][dim] float32 (cast to the index dtype, round-to-nearest-even, like the
- *                oracle does)
+ *                oracle does; taken as they are by float32 and fp4 collections)
  *   qtext/qtext_off  concatenated UTF-8 of query.lower() per query and B+1 offsets, or NULL
  *                (no symbol boost)
  *   out_ids      [B][top_k] int64 row ids, -1 beyond out_counts[b]
@@ -151,7 +160,7 @@ int crag_search_multi_hashed(crag_index* const* hs, const float* queries, int B,
                              const uint64_t* q_hashes, const int32_t* q_hash_off, int64_t* out_ids,
                              double* out_scores, float* out_dist, int32_t* out_counts);
 /*
- * Device-buffer form: queries_dev [B][dim] ALREADY in the index dtype; q_hashes_dev /
+ * Device-buffer form: queries_dev [B][dim] ALREADY in the index dtype (fp4: float32); q_hashes_dev /
  * q_hash_off_dev (sorted symbol hashes per query, B+1 offsets) may be NULL; outputs are device
  * arrays shaped as above.  Work is enqueued on `stream` (a hipStream_t, NULL = default stream);
  * the call returns after the results are complete and verified (it synchronises the stream,
@@ -212,6 +221,46 @@ int crag_search_local_device(crag_index* h, const void* queries_dev, int B, int 
 int crag_merge_rerank_device(int device, const void* entries_dev, int G, int B, int top_k, double symbol_boost,
                              int64_t* out_ids_dev, double* out_scores_dev, float* out_dist_dev,
                              int32_t* out_counts_dev, void* stream);
+
+/* ---- pooled embedding lookups ----------------------------------------------------------- */
+/*
+ * What turns a text's tokens into the vector that is searched for: a bag of token ids (words, word pieces, hashed
+ * n-grams) becomes the scaled, optionally L2-normalised sum of its tokens' table rows.
+ *
+ *   p_b = scale * c_b * sum over t in bag b of weights[t] * table[ids[t]]     c_b = 1, 1 / n_b or 1 / sqrt(n_b)
+ *   out_b = p_b / |p_b| when normalize (0 where p_b is 0), else p_b
+ *
+ * n_b counts the bag's tokens with an id in [0, vocab).  Ids outside it (padding) contribute nothing, and get no gradient.
+ * Bag b is positions [offsets[b], offsets[b + 1]): offsets_dev holds n_bags + 1 ascending values, and positions in
+ * front of the first or behind the last belong to no bag.  An empty bag gives zeros.
+ *   table_dev     [vocab][dim] float32 or bf16, row-major; dim <= 2048
+ *   weights_dev   [n_tokens], NULL = ones
+ *   out_dev       [n_bags][dim], out_dtype float32 or bf16.  Sums are float32 (norms float64); one rounding at the end
+ *   coef_dev      [n_bags], may be NULL: what the backward call needs of this one
+ * n_tokens < 2^31.  Both calls are asynchronous on `stream`, allocate nothing and may be captured into a graph; everything
+ * they need beside the buffers is in the caller's workspace (crag_embed_workspace bytes, 256-byte aligned), which belongs to
+ * the call until the stream has passed it: calls that can run at once need one each.  They use no atomics on sums: the same
+ * inputs give the same bits.
+ */
+#define CRAG_POOL_SUM 0
+#define CRAG_POOL_MEAN 1
+#define CRAG_POOL_SQRT 2
+int64_t crag_embed_workspace(int64_t n_tokens, int n_bags, int dim, int backward);
+int crag_embed_forward_device(int device, const void* table_dev, int64_t vocab, int dim, int dtype, const int32_t* ids_dev,
+                              const float* weights_dev, int64_t n_tokens, const int64_t* offsets_dev, int n_bags, int mode,
+                              float scale, int normalize, void* out_dev, int out_dtype, float* coef_dev, void* workspace_dev,
+                              int64_t workspace_bytes, void* stream);
+/*
+ * Gradients of the lookup above for grad_dev [n_bags][dim] (of out, float32):
+ *   y_dev          the forward call's out in float32 (only read when normalize), coef_dev its coefficients
+ *   d_table_dev    [vocab][dim] in the table's dtype, 16-byte aligned; written whole (zeros where no token occurs); may be NULL.
+ *                  A token's occurrences are sorted by position and added in that order in float32
+ *   d_weights_dev  [n_tokens] float32, may be NULL
+ */
+int crag_embed_backward_device(int device, const void* table_dev, int64_t vocab, int dim, int dtype, const int32_t* ids_dev,
+                               const float* weights_dev, int64_t n_tokens, const int64_t* offsets_dev, int n_bags, int normalize,
+                               const float* y_dev, const float* coef_dev, const float* grad_dev, void* d_table_dev,
+                               float* d_weights_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
 
 /* ---- introspection (tests, bench) ------------------------------------------------------ */
 /* counters since the last reset: [0] searches, [1] queries, [2] fallback queries (came back from the cascade without

@@ -1,0 +1,313 @@
+"""GPU tests of the pooled embedding lookup and its gradient against a plain implementation in 64 bits.
+
+Tolerances, derived: a float32 sum of n products is off by at most (n + 2) u sum|w E| with u = 2^-24 (one rounding per
+product-and-add, a few for joined parts and the scale); norms and quotients are float64; a bf16 result adds half a step,
+2^-8 relative.  The same holds for a token's gradient over its occurrences, plus what dp itself is off by."""
+import numpy as np
+import pytest
+
+import coderag_hip as ch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def make(bags, mean, dim, vocab, seed, dtype="f32", weighted=True, pads=False, hot=0.0):
+    import torch
+    r = np.random.default_rng(seed)
+    lens = r.integers(0, 2 * mean + 1, bags)
+    offsets = np.zeros(bags + 1, np.int64)
+    np.cumsum(lens, out=offsets[1:])
+    t = int(offsets[-1])
+    ids = r.integers(0, vocab, t)
+    if hot:
+        ids[r.random(t) < hot] = vocab // 2
+    if pads and t:
+        ids[r.random(t) < 0.2] = -1
+        ids[r.random(t) < 0.05] = vocab
+        ids[r.random(t) < 0.02] = 2 ** 31 - 1
+    w = r.standard_normal(t).astype(np.float32) if weighted else None
+    table = torch.from_numpy(r.standard_normal((vocab, dim)).astype(np.float32))
+    if dtype == "bf16":
+        table = table.bfloat16()
+    return table, ids.astype(np.int32), offsets, w
+
+
+def plain(table, ids, offsets, w, mode, scale, normalize, grad=None):
+    """(y, dE, dw) in float64 on the CPU, and the bounds of a float32 computation"""
+    import torch
+    e = table.double().numpy()
+    bags, (vocab, dim) = len(offsets) - 1, e.shape
+    w64 = np.ones(len(ids)) if w is None else w.astype(np.float64)
+    ok = (ids >= 0) & (ids < vocab)
+    y, yb = np.zeros((bags, dim)), np.zeros((bags, dim))
+    coef = np.zeros(bags)
+    for b in range(bags):
+        p = np.arange(offsets[b], offsets[b + 1])
+        p = p[ok[p]]
+        n = max(len(p), 1)
+        f = scale * {"sum": 1.0, "mean": 1.0 / n, "sqrt": n ** -0.5}[mode]
+        terms = w64[p, None] * e[ids[p]]
+        s, mag = terms.sum(0), np.abs(terms).sum(0)
+        err = (n + 2) * U * mag
+        if normalize:
+            norm = np.linalg.norm(s)
+            if norm > 0 and f != 0:
+                y[b] = np.sign(f) * s / norm
+                yb[b] = err / norm + np.abs(y[b]) * (np.linalg.norm(err) / norm + 2 * U)
+                coef[b] = np.sign(f) / norm
+        else:
+            y[b], yb[b], coef[b] = f * s, abs(f) * (err + 2 * U * np.abs(s)), f
+    if grad is None:
+        return y, yb
+    g = grad.double().numpy()
+    dp, dpb = np.zeros((bags, dim)), np.zeros((bags, dim))
+    for b in range(bags):
+        if normalize:
+            gy = g[b] @ y[b]
+            dp[b] = coef[b] * (g[b] - y[b] * gy)
+            off = np.abs(g[b]) @ yb[b]
+            rel = np.linalg.norm(yb[b]) + 3 * U          # of the coefficient: the norm's error is within y's
+            dpb[b] = abs(coef[b]) * (yb[b] * abs(gy) + np.abs(y[b]) * off) * 1.01 + rel * np.abs(dp[b])
+        else:
+            dp[b] = coef[b] * g[b]
+            dpb[b] = 3 * U * np.abs(dp[b])
+    bag = np.repeat(np.arange(bags), np.diff(offsets))
+    de, deb = np.zeros_like(e), np.zeros_like(e)
+    cnt = np.zeros(vocab)
+    t = np.nonzero(ok)[0]
+    np.add.at(de, ids[t], w64[t, None] * dp[bag[t]])
+    np.add.at(cnt, ids[t], 1)
+    np.add.at(deb, ids[t], np.abs(w64[t, None]) * (dpb[bag[t]] + U * np.abs(dp[bag[t]])))
+    mag = np.zeros_like(e)
+    np.add.at(mag, ids[t], np.abs(w64[t, None] * dp[bag[t]]))
+    deb += (cnt[:, None] + 2) * U * mag
+    dw, dwb = np.zeros(len(ids)), np.zeros(len(ids))
+    dw[t] = (dp[bag[t]] * e[ids[t]]).sum(1)
+    dwb[t] = ((dpb[bag[t]] + (dim + 2) * U * np.abs(dp[bag[t]])) * np.abs(e[ids[t]])).sum(1)
+    return (y, yb), (de, deb), (dw, dwb)
+
+
+def within(got, want, bound, bf16=False):
+    got = got.detach().double().cpu().numpy()
+    assert np.isfinite(got).all()
+    if bf16:
+        bound = bound + 2.0 ** -8 * (np.abs(want) + bound)
+    bad = np.abs(got - want) > bound * 1.0001 + 1e-37
+    assert not bad.any(), (np.argwhere(bad)[:3], np.abs(got - want).max())
+
+
+def gpu(table, ids, offsets, w):
+    import torch
+    return table.cuda(), torch.from_numpy(ids).cuda(), torch.from_numpy(offsets).cuda(), None if w is None else torch.from_numpy(w).cuda()
+
+
+SHAPES = [(1, 0, 8, 5), (1, 1, 1, 1), (3, 4, 7, 10), (1, 60, 384, 1000), (1, 3000, 384, 5000), (40, 33, 384, 300), (700, 3, 33, 100), (64, 200, 768, 2000),
+          (9, 100, 1023, 50), (17, 50, 2048, 64), (5, 40, 2047, 40), (2000, 1, 12, 30), (129, 77, 516, 4000), (30, 500, 6, 7), (4, 2500, 130, 100000)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bags,mean,dim,vocab", SHAPES)
+def test_lookup(bags, mean, dim, vocab, dtype):
+    import torch
+    for k, (mode, scale, normalize, weighted, pads) in enumerate([("mean", 1.0, True, True, False), ("sum", -0.5, False, True, True),
+                                                                  ("sqrt", 3.0, False, False, True), ("sqrt", -2.0, True, False, False)]):
+        case = make(bags, mean, dim, vocab, 10 * k + dim, dtype, weighted, pads)
+        y, bound = plain(*case, mode, scale, normalize)
+        dev = gpu(*case)
+        got = ch.embed_bags(*dev, mode=mode, scale=scale, normalize=normalize)
+        within(got, y, bound)
+        assert torch.equal(got, ch.embed_bags(*dev, mode=mode, scale=scale, normalize=normalize))
+        within(ch.embed_bags(*dev, mode=mode, scale=scale, normalize=normalize, out_dtype=torch.bfloat16), y, bound, bf16=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bags,mean,dim,vocab", SHAPES)
+def test_gradients(bags, mean, dim, vocab, dtype):
+    import torch
+    for k, (mode, scale, normalize, weighted, pads, hot) in enumerate([("mean", 1.0, True, True, False, 0.3), ("sum", -0.5, False, True, True, 0.0),
+                                                                       ("sqrt", 2.0, True, False, True, 0.9)]):
+        case = make(bags, mean, dim, vocab, 100 + 10 * k + dim, dtype, weighted, pads, hot)
+        grad = torch.from_numpy(np.random.default_rng(k).standard_normal((bags, dim)).astype(np.float32))
+        (y, yb), (de, deb), (dw, dwb) = plain(*case, mode, scale, normalize, grad)
+        table, ids, offsets, w = gpu(*case)
+        table.requires_grad_(True)
+        leaves = (table,)
+        if w is not None:
+            w.requires_grad_(True)
+            leaves = (table, w)
+        out = ch.embed_bags(table, ids, offsets, w, mode=mode, scale=scale, normalize=normalize)
+        within(out, y, yb)
+        got = torch.autograd.grad(out, leaves, grad.cuda(), retain_graph=True)
+        assert got[0].dtype == table.dtype
+        within(got[0], de, deb, bf16=dtype == "bf16")
+        if w is not None:
+            within(got[1], dw, dwb)
+        for a, b in zip(got, torch.autograd.grad(out, leaves, grad.cuda())):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+def test_large_sort_with_every_number_of_passes(normalize):
+    """more positions than one workgroup sorts; vocabularies that need one to three digits"""
+    import torch
+    for vocab in (200, 256, 30000, 70000):
+        case = make(300, 60, 16, vocab, vocab, hot=0.2, pads=True)
+        grad = torch.from_numpy(np.random.default_rng(1).standard_normal((300, 16)).astype(np.float32))
+        _, (de, deb), (dw, dwb) = plain(*case, "mean", 1.0, normalize, grad)
+        table, ids, offsets, w = gpu(*case)
+        assert ids.numel() > 8192
+        table.requires_grad_(True)
+        w.requires_grad_(True)
+        out = ch.embed_bags(table, ids, offsets, w, normalize=normalize)
+        d_table, d_w = torch.autograd.grad(out, (table, w), grad.cuda())
+        within(d_table, de, deb)
+        within(d_w, dw, dwb)
+
+
+def test_gradients_against_differences():
+    """the loss's change along a direction, by central differences of the 64-bit formula"""
+    import torch
+    table, ids, offsets, w = make(20, 15, 24, 60, 3)
+    r = np.random.default_rng(5)
+    grad = torch.from_numpy(r.standard_normal((20, 24)).astype(np.float32))
+    dt, dw = r.standard_normal((60, 24)), r.standard_normal(len(ids))
+    for normalize in (True, False):
+        h = 1e-5
+
+        def loss(sign):
+            t = torch.from_numpy(table.double().numpy() + sign * h * dt)
+            y, _ = plain(t, ids, offsets, w.astype(np.float64) + sign * h * dw, "mean", 1.0, normalize)
+            return float((y * grad.double().numpy()).sum())
+
+        diff = (loss(1) - loss(-1)) / (2 * h)
+        tb, i, o, ww = gpu(table, ids, offsets, w)
+        tb.requires_grad_(True)
+        ww.requires_grad_(True)
+        g = torch.autograd.grad(ch.embed_bags(tb, i, o, ww, normalize=normalize), (tb, ww), grad.cuda())
+        got = float((g[0].double().cpu().numpy() * dt).sum() + (g[1].double().cpu().numpy() * dw).sum())
+        assert abs(got - diff) <= 1e-4 * max(1.0, abs(diff))    # h^2 of the differences, 24 * 60 float32 values
+
+
+def test_hashing_embedder_is_a_lookup_in_the_identity():
+    texts = ["function parseQuery(q) { return q.split('&') }", "a", "", "größe 名前", "class A extends B"] + ["x" * 500]
+    want = ch.HashingEmbedder(dim=96)(texts)
+    got = ch.TokenEmbedder(np.eye(96, dtype=np.float32))(texts)
+    assert np.array_equal(got != 0, want != 0)
+    assert np.abs(got - want).max() <= 3 * U * np.abs(want).max()     # whole-number sums, one norm and one quotient each
+
+
+def test_positions_outside_every_bag_zero_bags_and_zero_rows():
+    import torch
+    table = torch.randn((10, 20), device="cuda", requires_grad=True)
+    ids = torch.arange(8, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([2, 4, 4, 6], device="cuda")
+    y = ch.embed_bags(table, ids, offsets, mode="sum", normalize=False)
+    assert torch.equal(y[0], table[2] + table[3]) and not y[1].any() and torch.equal(y[2], table[4] + table[5])
+    (d,) = torch.autograd.grad(y.sum(), table)
+    assert d[2:6].eq(1).all() and not d[:2].any() and not d[6:].any()
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    none = ch.embed_bags(table, ids, torch.zeros(1, dtype=torch.int64, device="cuda"), w)
+    assert none.shape == (0, 20)
+    d, dw = torch.autograd.grad(none.sum(), (table, w))
+    assert not d.any() and not dw.any()
+    empty = ch.embed_bags(table, ids[:0], torch.zeros(4, dtype=torch.int64, device="cuda"))
+    assert not empty.any()
+    (d,) = torch.autograd.grad(empty.sum(), table)
+    assert not d.any()
+    zeros = torch.zeros((10, 20), device="cuda", requires_grad=True)   # p = 0: y = 0, and no gradient
+    y = ch.embed_bags(zeros, ids, offsets)
+    assert not y.any()
+    (d,) = torch.autograd.grad(y, zeros, torch.ones_like(y))
+    assert not d.any()
+
+
+def test_unaligned_table_other_stream_and_infinities():
+    import torch
+    big = torch.randn(1 + 50 * 36, device="cuda")
+    table = big[1:].view(50, 36)               # 4-byte aligned rows
+    r = np.random.default_rng(1)
+    ids = torch.from_numpy(r.integers(0, 50, 400).astype(np.int32)).cuda()
+    offsets = torch.arange(0, 401, 40, device="cuda")
+    want = ch.embed_bags(table.clone(), ids, offsets)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = ch.embed_bags(table, ids, offsets)
+    st.synchronize()
+    assert (got - want).abs().max() <= 100 * U      # other lanes hold the row: sums in the same order, norms in another
+    t = table.clone()
+    t[7, 3] = float("inf")
+    y = ch.embed_bags(t, ids, offsets, normalize=False)
+    hit = torch.tensor([bool((ids[40 * b:40 * b + 40] == 7).any()) for b in range(10)], device="cuda")
+    assert torch.equal(torch.isinf(y[:, 3]), hit) and torch.isfinite(y[:, :3]).all()
+
+
+def test_captured_lookup_and_gradient():
+    import torch
+    case = make(40, 300, 384, 2000, 8)
+    table, ids, offsets, w = gpu(*case)
+    table.requires_grad_(True)
+    w.requires_grad_(True)
+    grad = torch.randn((40, 384), device="cuda")
+
+    def step():
+        y = ch.embed_bags(table, ids, offsets, w)
+        return (y,) + torch.autograd.grad(y, (table, w), grad)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.cuda.graph(other):
+        out2 = step()
+    for k in range(4):
+        with torch.no_grad():
+            table.add_(0.25)
+            grad.mul_(-1.5)
+        want = step()
+        graph.replay()
+        other.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(out, want, out2):
+            assert torch.equal(a, b) and torch.equal(c, b), k
+        del want
+
+
+def test_training_through_a_search_batch():
+    """the lookup inside a loss of a user's own: gradients of question and chunk bags through one table add up"""
+    import torch
+    table, ids, offsets, w = gpu(*make(32, 20, 48, 200, 2))
+    table.requires_grad_(True)
+    q = ch.embed_bags(table, ids, offsets, w)
+    c = ch.embed_bags(table, ids.flip(0).contiguous(), offsets, mode="sqrt")
+    loss = torch.logsumexp(q @ c.t() * 5, 1).sum() - 5 * (q * c).sum()
+    loss.backward()
+    q2, c2 = q.detach().requires_grad_(True), c.detach().requires_grad_(True)
+    l2 = torch.logsumexp(q2 @ c2.t() * 5, 1).sum() - 5 * (q2 * c2).sum()
+    l2.backward()
+    host = table.detach().cpu()
+    _, (d1, b1), _ = plain(host, ids.cpu().numpy(), offsets.cpu().numpy(), w.cpu().numpy(), "mean", 1.0, True, q2.grad.cpu())
+    _, (d2, b2), _ = plain(host, ids.flip(0).cpu().numpy(), offsets.cpu().numpy(), None, "sqrt", 1.0, True, c2.grad.cpu())
+    within(table.grad, d1 + d2, b1 + b2 + U * (np.abs(d1) + np.abs(d2)))
+
+
+def test_workspace_size_is_checked():
+    import torch
+    lib = ch.load()
+    table = torch.randn((10, 8), device="cuda")
+    ids, off = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 4], device="cuda")
+    out, ws = torch.empty((1, 8), device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    need = lib.crag_embed_workspace(4, 1, 8, 0)
+    args = [0, table.data_ptr(), 10, 8, 0, ids.data_ptr(), None, 4, off.data_ptr(), 1, 0, 1.0, 0, out.data_ptr(), 0, None, ws.data_ptr(), need, None]
+    assert lib.crag_embed_forward_device(*args) == 0
+    torch.cuda.synchronize()
+    assert torch.allclose(out[0], 4 * table[0])
+    for i, bad in ((17, need - 1), (16, None), (1, None), (2, 0), (3, 0), (3, 2049), (4, 2), (5, None), (7, -1), (8, None), (10, 7), (13, None), (14, 2), (0, 99)):
+        wrong = list(args)
+        wrong[i] = bad
+        assert lib.crag_embed_forward_device(*wrong) < 0, i

@@ -1,0 +1,291 @@
+"""GPU tests of collections whose rows are held in 4 bits: the rows as they are held against a plain restatement of the
+conversion, and every search entry point against the oracle on those rows (bit for bit: ids, scores, distances)."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+import coderag_hip as ch
+from oracle import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+
+
+def held(rows):
+    """float32 [n, d] -> the values a 4-bit collection holds: groups of 32, the smallest power of two that keeps the largest
+    magnitude within 7, the nearest level (a tie to the level with the even index)"""
+    n, d = rows.shape
+    x = np.zeros((n, -(-d // 32) * 32), np.float64)
+    x[:, :d] = rows
+    x = x.reshape(n, -1, 32)
+    big = np.abs(x).max(-1)
+    e = np.full(big.shape, -125.0)
+    nz = big > 0
+    e[nz] = np.clip(np.ceil(np.log2(big[nz] / 7)), -125, 125)
+    # log2 may round across a power of two: settle both sides exactly
+    e = np.where((e > -125) & (big <= 7 * 2.0 ** (e - 1)), e - 1, e)
+    e = np.where((e < 125) & (big > 7 * 2.0 ** e), e + 1, e)
+    v = np.abs(x) / 2.0 ** e[..., None]
+    dist = np.abs(v[..., None] - LEVELS)
+    best = dist.min(-1, keepdims=True)
+    tie = dist == best
+    even = tie & (np.arange(8) % 2 == 0)
+    idx = np.where(even.any(-1), even.argmax(-1), tie.argmax(-1))
+    out = np.sign(x) * LEVELS[idx] * 2.0 ** e[..., None]
+    return out.reshape(n, -1)[:, :d].astype(np.float32)
+
+
+def unit(n, d, seed):
+    r = np.random.default_rng(seed)
+    x = r.standard_normal((n, d)).astype(np.float32)
+    return x / np.linalg.norm(x, axis=1, keepdims=True)
+
+
+def collection(rows, metric="l2", classes=None, path="auto", base=0):
+    col = ch.GpuCollection(rows.shape[1], "fp4", metric)
+    if len(rows):
+        col.add(rows, path_class=classes)
+    col.set_id_base(base)
+    col.finalize()
+    col.set_path(path)
+    return col
+
+
+def agree(got, want, where=""):
+    ids, sc, di, cn = (np.asarray(x) for x in got)
+    for b, (wi, ws, wd) in enumerate(want):
+        k = len(wi)
+        assert int(cn[b]) == k, (where, b, int(cn[b]), k)
+        assert np.array_equal(ids[b, :k], wi), (where, b, ids[b, :k], wi)
+        assert np.array_equal(sc[b, :k], ws), (where, b)
+        assert np.array_equal(di[b, :k].view(np.uint32), np.asarray(wd, np.float32).view(np.uint32)), (where, b)
+        assert np.all(ids[b, k:] == -1)
+
+
+def numpy_of(out):
+    return [t.cpu().numpy() for t in out]
+
+
+@pytest.mark.parametrize("d", [1, 31, 32, 33, 100, 128, 384, 500, 768, 1024, 1536, 2048])
+def test_rows_are_held_as_defined(d):
+    rng = np.random.default_rng(d)
+    rows = (rng.standard_normal((75, d)) * np.exp(rng.uniform(-20, 20, (75, 1)))).astype(np.float32)
+    rows[3] = 0
+    rows[4] = rng.choice([0, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, 6, 7, -7, -5, -.25], d)        # ties, and the scale's border
+    rows[5] = rng.choice([3.5, -3.5, 3.4999998, 3.5000002], d)
+    rows[6] = 1e-39
+    rows[7] = 1.5e17 * rng.choice([-1, 1], d)
+    rows[8] *= np.float32(2.0 ** -100)
+    col = ch.GpuCollection(d, "fp4")
+    for lo, hi in ((0, 1), (1, 34), (34, 64), (64, 75)):
+        col.add(rows[lo:hi])
+    got = col.rows_host()
+    assert np.array_equal(got, held(rows))
+    assert np.array_equal(col.rows_host(30, 40), got[30:70])
+    again = ch.GpuCollection(d, "fp4")
+    again.add(got)
+    assert np.array_equal(again.rows_host(), got)
+    import torch
+    dev = ch.GpuCollection(d, "fp4")
+    t = torch.from_numpy(rows).cuda()
+    dev.add_device(t[:33])
+    dev.add_device(t[33:])          # starts at any element's alignment
+    assert np.array_equal(dev.rows_host(), got)
+
+
+@pytest.mark.parametrize("metric", ["l2", "ip"])
+@pytest.mark.parametrize("d,n,b", [(384, 4100, 1), (384, 4100, 16), (384, 333, 17), (500, 1000, 40), (768, 97, 130), (1024, 640, 64), (1536, 65, 3),
+                                   (2048, 70, 35)])
+def test_scan_scores_are_within_the_certificates_bound(d, n, b, metric):
+    import torch
+    rows, q = unit(n, d, 1), unit(b, d, 2)
+    q[0] *= 37.0
+    col = collection(rows, metric)
+    x = col.rows_host().astype(np.float64)
+    got = col.debug_dense_scores(torch.from_numpy(q).cuda()).cpu().numpy().astype(np.float64)
+    dots = q.astype(np.float64) @ x.T
+    want = (x * x).sum(1) - 2 * dots if metric == "l2" else -dots
+    # two pieces with 4-bit significands leave at most 2^-9 of a group's largest element of each of its elements; float32
+    # sums of the padded length with factor two for the matrix instruction's own order
+    big = np.abs(np.pad(q, ((0, 0), (0, -d % 32)))).reshape(b, -1, 32).max(-1)
+    rest = np.sqrt((32 * (big * 2.0 ** -9) ** 2).sum(1))
+    xm = np.sqrt((x * x).sum(1).max())
+    eps = 2 * 2.0 ** -24 * (col.dim_pad + 4) * (2 * np.linalg.norm(q, axis=1) * xm + xm * xm)
+    bound = (2 if metric == "l2" else 1) * rest * xm + eps
+    assert np.all(np.abs(got - want).max(1) <= bound)
+
+
+@pytest.mark.parametrize("path", ["auto", "gemv"])
+@pytest.mark.parametrize("d,n,b,top_k,metric", [
+    (384, 1, 1, 10, "l2"), (384, 5, 3, 10, "ip"), (384, 31, 16, 1, "l2"), (384, 33, 17, 200, "l2"), (384, 20001, 1, 10, "l2"),
+    (384, 9000, 33, 10, "ip"), (100, 12345, 7, 25, "l2"), (768, 20000, 65, 10, "l2"), (768, 30000, 16, 100, "l2"),
+    (1024, 9001, 130, 10, "ip"), (1024, 20011, 3, 200, "l2"), (1536, 8500, 20, 10, "l2"), (2048, 8300, 2, 10, "l2"),
+    (2048, 1000, 40, 5, "ip"), (17, 40000, 300, 10, "l2"), (500, 70001, 9, 50, "l2"), (256, 33000, 260, 10, "l2"), (512, 9999, 18, 10, "l2")])
+def test_search_is_the_oracles_on_the_held_rows(coracle, d, n, b, top_k, metric, path):
+    rows = unit(n, d, n + d)
+    q = unit(b, d, 7)
+    q[: b // 2] = 0.8 * rows[np.random.default_rng(3).integers(0, n, b // 2)] + 0.1 * q[: b // 2]
+    classes = (np.arange(n) % 3).astype(np.uint8)
+    col = collection(rows, metric, classes, path)
+    want = coracle.search_numeric(col.rows_host(), q, classes, None, top_k, 2.0, metric)
+    agree(col.search(q, top_k), want, "host")
+    import torch
+    agree(numpy_of(col.search_device(torch.from_numpy(q).cuda(), top_k)), want, "device")
+    assert col.stats()["exact_scan"] == 0
+
+
+def test_a_4bit_collection_answers_like_a_float32_one_with_its_rows():
+    import torch
+    rows = unit(60000, 384, 5)
+    q = torch.from_numpy(unit(200, 384, 6)).cuda()
+    col = collection(rows)
+    ref = ch.GpuCollection(384, "f32")
+    ref.add(col.rows_host())
+    for a, b in zip(col.search_device(q, 50), ref.search_device(q, 50)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("b", [1, 20])
+def test_duplicates_ties_and_zero_rows_go_through_the_fallback_tiers(coracle, b):
+    for rows in (np.zeros((30000, 64), np.float32), np.repeat(unit(3, 64, 1), 9000, 0), np.repeat(unit(6000, 64, 1), 5, 0)):
+        col = collection(rows)
+        q = unit(b, 64, 2)
+        want = coracle.search_numeric(col.rows_host(), q, np.zeros(len(rows), np.uint8), None, 20, 2.0, "l2")
+        agree(col.search(q, 20), want)
+
+
+def test_empty_collection_and_refusals():
+    import torch
+    col = collection(np.zeros((0, 96), np.float32))
+    ids, sc, di, cn = col.search(unit(3, 96, 1), 5)
+    assert not cn.any() and (ids == -1).all()
+    with pytest.raises(ch.CragError, match="layout of their own"):
+        ch.GpuCollection(128, "fp4").attach_device(torch.zeros((4, 128), device="cuda"))
+    with pytest.raises(ch.CragError, match="2048"):
+        ch.GpuCollection(2049, "fp4")
+    with pytest.raises(ValueError):
+        col.add_device(torch.zeros((4, 96), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        col.search_device(torch.zeros((4, 96), dtype=torch.bfloat16, device="cuda"))
+    for bad in (np.nan, np.inf):
+        rows = unit(40, 96, 1)
+        rows[33, 95] = bad
+        c = ch.GpuCollection(96, "fp4")
+        c.add(rows)
+        assert np.isnan(c.rows_host()[33, 64:]).all()
+        with pytest.raises(ch.CragError, match="NaN or an infinite"):
+            c.finalize()
+    f32 = ch.GpuCollection(96, "f32")
+    f32.add(unit(40, 96, 1))
+    f32.finalize()
+    with pytest.raises(ch.CragError, match="differ"):
+        ch.search_multi([col, f32], unit(2, 96, 1))
+
+
+def test_queries_of_any_size(coracle):
+    rows = unit(9000, 160, 1)
+    col = collection(rows)
+    q = unit(6, 160, 2)
+    q[0] = 0
+    q[1] *= np.float32(1e-30)
+    q[2] *= np.float32(3e8)
+    q[3] *= np.float32(1e37)
+    want = coracle.search_numeric(col.rows_host(), q, np.zeros(9000, np.uint8), None, 10, 2.0, "l2")
+    agree(col.search(q, 10), want)
+    q[4, 3], q[5, 159] = np.nan, np.inf
+    _, _, _, cn = col.search(q, 10)
+    assert cn[4] == 0 and cn[5] == 0 and cn[0] == 10
+
+
+@pytest.mark.parametrize("metric", ["l2", "ip"])
+def test_many_collections_in_one_call(coracle, metric):
+    import torch
+    sizes = [1, 40, 9000, 31, 20000, 8192, 0, 40000]
+    cols = [collection(unit(n, 384, n) if n else np.zeros((0, 384), np.float32), metric, (np.arange(n) % 3).astype(np.uint8) if n else None, base=100 * i)
+            for i, n in enumerate(sizes)]
+    order = [0, 1, 2, 2, 2, 3, 4, 5, 6, 7, 7, 0] + [4] * 20
+    q = unit(len(order), 384, 9)
+    want = []
+    for b, c in enumerate(order):
+        n = sizes[c]
+        if n == 0:
+            want.append((np.zeros(0, np.int64), np.zeros(0), np.zeros(0, np.float32)))
+            continue
+        w = coracle.search_numeric(cols[c].rows_host(), q[b:b + 1], (np.arange(n) % 3).astype(np.uint8), None, 10, 2.0, metric)[0]
+        want.append((np.asarray(w[0]) + 100 * c, w[1], w[2]))
+    handles = [cols[c] for c in order]
+    agree(ch.search_multi(handles, q, 10), want, "host")
+    agree(numpy_of(ch.search_multi_device(handles, torch.from_numpy(q).cuda(), 10)), want, "device")
+
+
+def test_noalloc_and_sharded_entry_points(coracle):
+    import torch
+    rows, q = unit(25000, 384, 1), unit(64, 384, 2)
+    col = collection(rows)
+    qd = torch.from_numpy(q).cuda()
+    want = numpy_of(col.search_device(qd, 20))
+    out = [torch.empty((64, 20), dtype=t, device="cuda") for t in (torch.int64, torch.float64, torch.float32)] + [torch.empty(64, dtype=torch.int32, device="cuda")]
+    rc = ch.load().crag_search_device_noalloc(col.handle, qd.data_ptr(), 64, 20, C.c_double(2.0), None, None, *[t.data_ptr() for t in out], None)
+    assert rc == 0
+    torch.cuda.synchronize()
+    for a, b in zip(numpy_of(out), want):
+        assert np.array_equal(a, b)
+    parts, entries = [(0, 7001), (7001, 25000)], []
+    for lo, hi in parts:
+        c = collection(rows[lo:hi], base=lo)
+        e = torch.empty((64, 40, 16), dtype=torch.uint8, device="cuda")
+        entries.append(c.search_local_device(qd, 20, e))
+    got = ch.merge_rerank_device(0, torch.stack(entries), 2, 64, 20, 2.0)
+    for a, b in zip(numpy_of(got), want):
+        assert np.array_equal(a, b)
+
+
+def test_two_threads_and_a_stream_of_the_callers():
+    import torch
+    col = collection(unit(30000, 384, 1))
+    qs = [torch.from_numpy(unit(b, 384, b)).cuda() for b in (1, 16, 33, 100)]
+    want = [numpy_of(col.search_device(q, 10)) for q in qs]
+    bad = []
+
+    def work(i):
+        st = torch.cuda.Stream()
+        for _ in range(5):
+            with torch.cuda.stream(st):
+                got = numpy_of(col.search_device(qs[i], 10))
+            bad.extend(1 for a, b in zip(got, want[i]) if not np.array_equal(a, b))
+
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
+def test_text_to_results_with_token_embeddings_and_4bit_rows(tmp_path, coracle):
+    """the path they are for: texts -> looked-up vectors -> 4-bit rows -> search, saved, loaded, searched again"""
+    rng = np.random.default_rng(4)
+    table = rng.standard_normal((5000, 384)).astype(np.float32)
+    ef = ch.TokenEmbedder(table)
+    hs = ch.HybridSearcher(db_path=str(tmp_path), embed_fn=ef, dtype="fp4")
+    words = ["parse", "token", "array", "merge", "cache", "query", "index", "render", "split", "count"]
+    texts = [" ".join(rng.choice(words, 12)) + f" {i}" for i in range(300)]
+    col = hs.create_collection("c", 384)
+    col.add([f"id{i}" for i in range(300)], ef(texts), [{"name": f"fn{i}", "path": f"pkg/src/f{i}.js"} for i in range(300)], texts)
+    res = hs.search(texts[17], top_k=5, collection_name="c")
+    assert res[0]["id"] == "id17"
+    want = coracle.search_numeric(col.gpu.rows_host(), ef([texts[17]]), np.full(300, 2, np.uint8), None, 5, 2.0, "l2")[0]
+    assert [r["id"] for r in res] == [f"id{i}" for i in want[0]]
+    assert [r["score"] for r in res] == list(want[1])
+    dev = col.gpu.search_device(ef.embed_device([texts[17]]), 5)
+    assert np.array_equal(dev[0].cpu().numpy()[0], want[0])
+    from coderag_hip import store
+    store.save_collection(str(tmp_path), col)
+    back = store.load_collection(str(tmp_path), "c")
+    assert back.gpu.dtype == "fp4" and np.array_equal(back.gpu.rows_host(), col.gpu.rows_host())
+    hs2 = ch.HybridSearcher(db_path=str(tmp_path), embed_fn=ef)
+    assert hs2.search(texts[17], top_k=5, collection_name="c") == res

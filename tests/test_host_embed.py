@@ -1,0 +1,62 @@
+"""CPU tests of the lookups' and the 4-bit rows' host side: tokens, refusals that need no device, workspace sizes."""
+import numpy as np
+import pytest
+
+import coderag_hip as ch
+from coderag_hip import embed
+
+
+def test_ngram_tokens_are_the_hashing_embedders():
+    for text in ("asciiToArray(string)", "", "größe", 12):
+        ids, w = ch.ngram_tokens(text, 384)
+        assert ids.dtype == np.int32 and w.dtype == np.float32 and ids.shape == w.shape
+        v = np.zeros(384)
+        np.add.at(v, ids, w)
+        want = ch.HashingEmbedder()([text])[0]
+        assert np.allclose(v / np.linalg.norm(v), want, atol=1e-6)
+
+
+def test_workspace_sizes():
+    lib = ch.load()
+    for n, b, d in ((0, 0, 1), (1, 1, 384), (10 ** 6, 1000, 384), (2 ** 31 - 1, 1, 8), (5000, 3, 2048), (5000, 3, 2047)):
+        fwd, bwd = lib.crag_embed_workspace(n, b, d, 0), lib.crag_embed_workspace(n, b, d, 1)
+        assert 0 < fwd <= bwd
+    for bad in ((-1, 1, 8), (2 ** 31, 1, 8), (1, -1, 8), (1, 1, 0), (1, 1, 2049)):
+        assert lib.crag_embed_workspace(*bad, 0) < 0
+
+
+def test_forward_and_backward_refuse_before_touching_a_device():
+    lib = ch.load()
+    good = [0, 256, 10, 8, 0, 256, None, 4, 256, 1, 0, 1.0, 0, 256, 0, None, 256, 1 << 30, None]
+    for i, bad in ((1, None), (1, 257), (2, 0), (2, 2 ** 31), (3, 0), (3, 2049), (4, 2), (5, None), (7, -1), (8, None), (9, -1), (10, 3), (13, None), (14, 2),
+                   (16, None), (16, 128), (17, 16)):
+        wrong = list(good)
+        wrong[i] = bad
+        assert lib.crag_embed_forward_device(*wrong) < 0, (i, bad)
+    good = [0, 256, 10, 8, 0, 256, None, 4, 256, 1, 1, 256, 256, 256, 256, None, 256, 1 << 30, None]
+    for i, bad in ((1, None), (2, 0), (3, 2049), (4, 3), (11, None), (12, None), (13, None), (14, 264), (16, None), (17, 16)):
+        wrong = list(good)
+        wrong[i] = bad
+        assert lib.crag_embed_backward_device(*wrong) < 0, (i, bad)
+
+
+def test_embed_bags_refuses_wrong_tensors():
+    import torch
+    t = torch.zeros((4, 8))
+    with pytest.raises(ValueError, match="table"):
+        ch.embed_bags(t, torch.zeros(2, dtype=torch.int32), torch.tensor([0, 2]))
+
+
+def test_pool_modes_and_dtypes_match_the_header():
+    assert embed.POOL_MODES == {"sum": 0, "mean": 1, "sqrt": 2}
+    with pytest.raises(ValueError, match="dtype"):
+        ch.GpuCollection(8, "int4")
+
+
+def test_config_takes_4bit_collections(tmp_path):
+    p = tmp_path / "r.yaml"
+    p.write_text("dtype: fp4\n")
+    assert ch.load_retrieval_config(str(p))["dtype"] == "fp4"
+    p.write_text("dtype: fp3\n")
+    with pytest.raises(ValueError):
+        ch.load_retrieval_config(str(p))
