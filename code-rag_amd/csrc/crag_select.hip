@@ -341,29 +341,45 @@ __device__ __forceinline__ double canon_lane(const void* row, const void* q, int
                              : canon_lane_t<CRAG_BF16>(row, q, dim, j, metric, row_off);
 }
 
-// the same partial sum of a 4-bit row in the tiles of crag_fp4.h: of a group's four words of eight codes, lane j takes
-// code j of each
-__device__ __forceinline__ double canon_lane_fp4(const void* rows, const float* q, int dim, int dim_pad, long long row, int j, int metric) {
+// The same partial sum of a 4-bit row in the tiles of crag_fp4.h, q in LDS or in global memory: of a group's four words of
+// eight codes, lane j takes code j of each.  The eight lanes of a row read the same 16 bytes (one request), eight groups
+// ahead of their use; nothing of the row is staged, because every element is used once.
+template <typename QPtr>
+__device__ __forceinline__ double canon_lane_fp4(const void* rows_, QPtr q, int dim, int dim_pad, long long row, int j, int metric) {
+    typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+    typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+    const __attribute__((address_space(1))) unsigned char* rows = (const __attribute__((address_space(1))) unsigned char*)rows_;
     double acc = 0.0;
-    for (int g = 0; g * 32 < dim; ++g) {
-        long long at, sc;
-        crag_fp4_place(dim_pad, row, g, &at, &sc);
-        const uint4 c = *(const uint4*)((const unsigned char*)rows + at);
-        const float s = crag_fp4_scale(((const unsigned char*)rows)[sc]);
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    for (int g0 = 0; g0 * 32 < dim; g0 += 8) {
+        u32x4_t c[8];
+        uint32_t s[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int d = g * 32 + 8 * u + j;
-            if (d < dim) {
-                const double a = (double)q[d], b = (double)crag_fp4_value((w[u] >> (4 * j)) & 15u, s);
-                double p;
-                if (metric == CRAG_L2) {
-                    const double t = __dsub_rn(a, b);
-                    p = __dmul_rn(t, t);
-                } else {
-                    p = __dmul_rn(a, b);
+        for (int u = 0; u < 8; ++u) {
+            if ((g0 + u) * 32 < dim) {
+                long long at, sc;
+                crag_fp4_place(dim_pad, row, g0 + u, &at, &sc);
+                c[u] = *(const __attribute__((address_space(1))) u32x4_t*)(rows + at);
+                s[u] = rows[sc];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float scale = crag_fp4_scale(s[u]);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int d = (g0 + u) * 32 + 8 * v + j;
+                if (d < dim) {
+                    const f32x2_t two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u][v] >> (4 * j), scale, 0);  // exact
+                    const double a = (double)q[d], b = (double)two.x;
+                    double p;
+                    if (metric == CRAG_L2) {
+                        const double t = __dsub_rn(a, b);
+                        p = __dmul_rn(t, t);
+                    } else {
+                        p = __dmul_rn(a, b);
+                    }
+                    acc = __dadd_rn(acc, p);
                 }
-                acc = __dadd_rn(acc, p);
             }
         }
     }
@@ -501,11 +517,11 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     // 128-KiB region is free now), so the order-defining add chains read LDS instead of chasing 2-byte loads
     {
         unsigned char* stage_q = (unsigned char*)(skeys + 1024);  // m + 1 <= CRAG_MAX_M + 1 <= 1024 keys stay live
-        const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;  // (4-bit rows are staged as float32)
+        const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;  // (of 4-bit rows only the query is staged)
         const int q_bytes = row_bytes > 4096 ? row_bytes : 4096;
         unsigned char* stage_r = stage_q + q_bytes;
         int rpr = (int)((sizeof(unsigned long long) * (CRAG_CAND_CAP - 1024) - q_bytes) / (size_t)row_bytes);
-        if (rpr > 128) rpr = 128;  // 1024 threads / 8 lanes
+        if (rpr > 128 || a.dtype == CRAG_FP4) rpr = 128;  // 1024 threads / 8 lanes; 4-bit rows are read where they lie
         for (int c = tid; c < chunks; c += 1024) ((uint4*)stage_q)[c] = ((const uint4*)qv)[c];
         for (int base = 0; base < m; base += rpr) {
             const int nr = m - base < rpr ? m - base : rpr;
@@ -514,27 +530,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             // which makes it a generic pointer to the compiler, and FLAT loads are waited for one at a time
             typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
             const __attribute__((address_space(1))) u32x4_t* grows = (const __attribute__((address_space(1))) u32x4_t*)D.rows;
-            if (a.dtype == CRAG_FP4) {
-                // one group of 32 codes per thread, decoded into 128 bytes of float32
-                const int n_grp = a.dim_pad >> 5, total = nr * n_grp;
-                const __attribute__((address_space(1))) unsigned char* grow = (const __attribute__((address_space(1))) unsigned char*)D.rows;
-                for (int idx = tid; idx < total; idx += 1024) {
-                    const int r = idx / n_grp, g = idx - r * n_grp;
-                    long long at, sc;
-                    crag_fp4_place(a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), g, &at, &sc);
-                    const u32x4_t c = *(const __attribute__((address_space(1))) u32x4_t*)(grow + at);
-                    const float s = crag_fp4_scale(grow[sc]);
-                    float4* o = (float4*)(stage_r + (size_t)r * row_bytes + g * 128);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const uint32_t w = c[u];
-                        o[2 * u] = make_float4(crag_fp4_value(w & 15u, s), crag_fp4_value((w >> 4) & 15u, s), crag_fp4_value((w >> 8) & 15u, s),
-                                               crag_fp4_value((w >> 12) & 15u, s));
-                        o[2 * u + 1] = make_float4(crag_fp4_value((w >> 16) & 15u, s), crag_fp4_value((w >> 20) & 15u, s),
-                                                   crag_fp4_value((w >> 24) & 15u, s), crag_fp4_value(w >> 28, s));
-                    }
-                }
-            } else {
+            if (a.dtype != CRAG_FP4) {
                 const int total = nr * chunks;
                 for (int idx0 = tid; idx0 < total; idx0 += 4 * 1024) {
                     u32x4_t v[4];
@@ -557,7 +553,10 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             __syncthreads();
             const int r = tid >> 3, j = tid & 7;
             double acc = 0.0;
-            if (r < nr) acc = canon_lane(stage_r, stage_q, a.dtype, a.dim, j, a.metric, (long long)r * a.dim_pad);
+            if (r < nr)
+                acc = a.dtype == CRAG_FP4
+                          ? canon_lane_fp4(D.rows, (const float*)stage_q, a.dim, a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), j, a.metric)
+                          : canon_lane(stage_r, stage_q, a.dtype, a.dim, j, a.metric, (long long)r * a.dim_pad);
             acc = combine8(acc);
             if (r < nr && j == 0) {
                 const double dist = a.metric == CRAG_L2 ? acc : __dsub_rn(1.0, acc);
