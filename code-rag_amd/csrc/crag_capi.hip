@@ -580,7 +580,8 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     // MFMA scan runs the multi-level cascade in which a level continues where the previous one
     // stopped.  (A one-block scan for bf16 rows up to 768 elements served two queries at top-10 until round 2;
     // the two-block cascade was within 1 % of it there, same box, and it went.)
-    const bool segmented = P.mfma && can_q16;
+    const int fp4_seg = fp4 && P.mfma ? crag_fp4_segments(B, h0->dim_pad, h0->n_cus) : 0;
+    const bool segmented = P.mfma && (can_q16 || fp4_seg > 0);
     const bool cascade = P.mfma;
     // ---- descriptors ----
     SmallVec<QueryDesc, 64> qd;
@@ -670,7 +671,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     unsigned long long* cand = nullptr;
     // no memset of the counters: level 0's selection (k_kth) writes every query's counter -- flat or per segment --
     // when it seeds the buffers, and k_finalize writes every query's status
-    const int n_seg = segmented ? crag_q16_segments(B, h0->n_cus) : 0;
+    const int n_seg = fp4 ? fp4_seg : (segmented ? crag_q16_segments(B, h0->n_cus) : 0);
     // physical room for twice CRAG_CAND_CAP per query (a segment holds >= 32): the COUNT must stay <= CAP
     const int seg_cap = segmented ? std::max(32, 2 * CRAG_CAND_CAP / n_seg) : 0;
     const long long cand_stride = segmented ? (long long)n_seg * seg_cap : (long long)CRAG_CAND_CAP;
@@ -686,7 +687,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         if (every < 1 || every > 128 || (every & (every - 1))) every = CRAG_PACE_EVERY_DEFAULT;
         return ((e ? atoi(e) : CRAG_AHEAD_MAX_DEFAULT) & 0xff) | ((every - 1) << 8);  // MfmaArgs::ahead_max: tiles | mask << 8
     }();
-    const bool paced = segmented && B > 256 && (ahead_max & 0xff) > 0;
+    const bool paced = segmented && !fp4 && B > 256 && (ahead_max & 0xff) > 0;
     const size_t prog_words = paced ? (size_t)CRAG_PROGRESS_WORDS(h0->n_cus) : 0;
     uint32_t* progress = nullptr;
     if (segmented) {
@@ -722,6 +723,9 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         fa.cand = cand;
         fa.cand_stride = cand_stride;
         fa.cnt = cnt;
+        fa.segcnt = segcnt;
+        fa.n_seg = n_seg;
+        fa.seg_cap = seg_cap;
         fa.rows = h0->rows;
         fa.xnorm = h0->xnorm;
         fa.n_queries = B;
@@ -797,11 +801,11 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         KthArgs k;
         memset(&k, 0, sizeof(k));
         k.src = sample;
-        if (segmented) {
-            k.tile_bpad = bpad;  // the two-block scan writes a tile-major sample
-        } else if (!query_minor) {
+        if (!query_minor) {
             k.q_stride = P.sample_stride;  // the 4-bit scan writes a query's scores one after the other
             k.e_stride = 1;
+        } else if (segmented) {
+            k.tile_bpad = bpad;  // the two-block scan writes a tile-major sample
         } else {
             k.q_stride = 1;      // the one-block scans write it row-major: [row][bpad]
             k.e_stride = bpad;

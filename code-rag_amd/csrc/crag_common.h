@@ -245,6 +245,9 @@ struct Fp4Args {
     unsigned long long* cand;  // flat buffers: [B][cand_stride], counts in cnt
     long long cand_stride;
     uint32_t* cnt;
+    // crag_fp4_segments > 0: segmented buffers instead (MfmaArgs), two segments per stream of tiles
+    uint32_t* segcnt;
+    int n_seg, seg_cap;
     // one collection (crag_launch_scan_fp4): rows [row_begin, row_end), row_begin a multiple of 32
     const void* rows;
     const float* xnorm;
@@ -261,6 +264,7 @@ long long crag_fp4_query_bytes(int n_blocks, int dim_pad, bool narrow);
 // residual[q]: norm of what the pieces of query q leave over
 int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_blocks, int B, int dim_pad, int metric, bool narrow, void* out,
                           float* residual, hipStream_t s);
+int crag_fp4_segments(int B, int dim_pad, int n_cus);
 int crag_launch_scan_fp4(const Fp4Args& a, int dim_pad, bool filter, int n_cus, hipStream_t s);
 int crag_launch_scan_fp4_groups(const Fp4Args& a, int dim_pad, int blocks, hipStream_t s);
 int crag_launch_fp4_quantize(const float* src, long long n, int dim, int dim_pad, long long first, void* dst, hipStream_t s);

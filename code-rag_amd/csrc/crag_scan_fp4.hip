@@ -105,6 +105,24 @@ __device__ __forceinline__ void keep_survivors(const f32x16_t& s, float tau, int
         }
     }
 }
+// The same into a segment of the query's candidate buffer that only this lane appends to: no atomic whose answer the wave
+// would wait for.  `count` may pass the segment's room: the selection then takes the query for overflowed.
+__device__ __forceinline__ void keep_survivors_own(const f32x16_t& s, float tau, long long row0, long long row_end, unsigned long long* __restrict__ seg,
+                                                   int seg_cap, uint32_t& count) {
+    float m = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = fminf(m, s[i]);
+    if (m <= tau) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const long long row = row0 + 8 * (i >> 2) + (i & 3);
+            if (s[i] <= tau && row < row_end) {
+                if (count < (uint32_t)seg_cap) seg[count] = ((unsigned long long)crag_fkey(s[i]) << 32) | (uint32_t)row;
+                ++count;
+            }
+        }
+    }
+}
 __device__ __forceinline__ void keep_all(const f32x16_t& s, int q, long long row0, const Fp4Args& a) {
     if (q < 0) return;
 #pragma unroll
@@ -198,6 +216,119 @@ __global__ __launch_bounds__(256, 1) void k_scan_fp4(Fp4Args a) {
         tau[b] = FILTER && id < a.n_queries ? a.tau[id] : __builtin_nanf("");
     }
     walk<KS, 2, QB, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + stream, streams, (a.row_end + 31) >> 5, a.row_end, a, q, tau, qid, lane);
+}
+
+// The same with four sets of queries per workgroup: the rows' tiles come through a ring in LDS, one copy for the four waves,
+// brought there by loads that write LDS directly and run up to RING - 1 tiles ahead.  The registers hold nothing but the
+// queries, the accumulators and the operands on their way, so two blocks of 32 queries fit for rows of up to 1024 elements
+// and each tile read from LDS feeds twice the products.
+template <int KS>
+struct Ring {
+    static constexpr int CHUNKS = KS + (crag_fp4_sw(KS) * 256 + 1023) / 1024;  // 1-KiB pieces of a tile
+    static constexpr int SLOT = CHUNKS * 1024 + 128;                            // ... and |x|^2 of its rows
+    static constexpr int LOADS = (CHUNKS + 1 + 3) / 4;                          // per wave: the same number in each, see issue()
+    static constexpr int SLOTS = 155 * 1024 / SLOT < 8 ? 155 * 1024 / SLOT : 8;
+    static constexpr int BYTES = SLOT * SLOTS;
+};
+
+// Wave w brings pieces w, w + 4, ... of a tile to LDS offset `slot`.  Waves with fewer pieces repeat their last one, so that
+// every wave has LOADS loads per tile in flight and one counted wait serves all.
+template <int KS>
+__device__ __forceinline__ void issue(const GLOBAL_AS unsigned char* tile, const GLOBAL_AS float* xnorm, uint32_t slot, int wave, int lane) {
+    using R = Ring<KS>;
+#pragma unroll
+    for (int i = 0; i < R::LOADS; ++i) {
+        int c = wave + 4 * i;
+        c = c > R::CHUNKS ? R::CHUNKS : c;  // piece CHUNKS: the norms
+        const int bytes = c == R::CHUNKS ? 128 : (c == R::CHUNKS - 1 ? (int)crag_fp4_tile_bytes(KS) - 1024 * (R::CHUNKS - 1) : 1024);
+        const GLOBAL_AS unsigned char* from = c == R::CHUNKS ? (const GLOBAL_AS unsigned char*)xnorm : tile + c * 1024;
+        const uint32_t to = __builtin_amdgcn_readfirstlane(slot + c * 1024);
+        if (lane * 16 < bytes)  // m0 is the LDS address of lane 0; an instruction must lie between its write and its use
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from + lane * 16) : "memory");
+    }
+}
+
+template <int KS, int QB, bool FILTER>
+__global__ __launch_bounds__(256, 1) void k_scan_fp4_ring(Fp4Args a) {
+    using R = Ring<KS>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int xcd = blockIdx.x & 7, slot_ = blockIdx.x >> 3;
+    const int qg = slot_ % a.query_groups;
+    const long long stream = (long long)(slot_ / a.query_groups) * 8 + xcd, streams = gridDim.x / a.query_groups;
+    const GLOBAL_AS unsigned char* rows = (const GLOBAL_AS unsigned char*)a.rows;
+    const GLOBAL_AS float* xnorm = (const GLOBAL_AS float*)a.xnorm;
+    const long long first = (a.row_begin >> 5) + stream, last = (a.row_end + 31) >> 5;
+    if (first >= last) return;  // the whole workgroup
+    const int n = (int)((last - first + streams - 1) / streams);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    auto bring = [&](int i) {
+        const long long t = first + i * streams;
+        issue<KS>(rows + t * crag_fp4_tile_bytes(KS), xnorm + t * 32, lds0 + (uint32_t)(i % R::SLOTS) * R::SLOT, wave, lane);
+    };
+    const int blk = (qg * 4 + wave) * QB;
+    Query<KS, 2> q[QB];
+    float tau[QB];
+    int qid[QB];
+    unsigned long long* seg[QB] = {};
+    uint32_t* segcnt[QB] = {};
+    uint32_t count[QB] = {};
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        q[b].load((const unsigned char*)a.queries + (blk + b) * crag_fp4_qblock_bytes(KS, 2), lane);
+        const int id = (blk + b) * 32 + (lane & 31);
+        qid[b] = id < a.n_queries ? id : -1;
+        tau[b] = FILTER && id < a.n_queries ? a.tau[id] : __builtin_nanf("");
+        if constexpr (FILTER) {
+            // two lanes of one wave hold a query's scores of this stream's tiles: a segment for each
+            const int sg = (int)stream * 2 + (lane >> 5);
+            const long long q_ = qid[b] < 0 ? 0 : qid[b];
+            seg[b] = a.cand + q_ * a.cand_stride + (long long)sg * a.seg_cap;
+            segcnt[b] = a.segcnt + q_ * a.n_seg + sg;
+            count[b] = qid[b] < 0 ? 0 : *segcnt[b];
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // from here on the counter holds the ring's loads
+    for (int i = 0; i < R::SLOTS - 1 && i < n; ++i) bring(i);
+    const bool l2 = a.metric == CRAG_L2;
+    for (int i = 0; i < n; ++i) {
+        // tile i has arrived (only the SLOTS - 2 tiles behind it may be on their way; at the end there are fewer), and every
+        // wave is done with tile i - 1, whose slot the next load takes
+        if (i + R::SLOTS - 1 <= n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R::SLOTS - 2) * R::LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (i + R::SLOTS - 1 < n) bring(i + R::SLOTS - 1);
+        const unsigned char* slot = smem + (i % R::SLOTS) * R::SLOT;
+        RowScales<KS> rs;
+#pragma unroll
+        for (int w = 0; w < crag_fp4_sw(KS); ++w) rs.w[w] = ((const uint32_t*)(slot + 1024 * KS))[lane * crag_fp4_sw(KS) + w];
+        f32x16_t acc[QB];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            f32x4_t xn = *(const f32x4_t*)(slot + 1024 * R::CHUNKS + 32 * r + (lane >> 5) * 16);
+            if (!l2) xn = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < QB; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[b][4 * r + j] = xn[j];
+        }
+        static_for<KS>([&](auto kc) {
+            constexpr int k = kc;
+            Codes<1> c;
+            c.c[0] = *(const u32x4_t*)(slot + k * 1024 + lane * 16);
+            products<KS, 2, QB, k, 1>(c, rs, q, acc);
+        });
+        const long long row0 = (first + i * streams) * 32 + (lane >> 5) * 4;
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            if constexpr (FILTER) keep_survivors_own(acc[b], tau[b], row0, a.row_end, seg[b], a.seg_cap, count[b]);
+            else keep_all(acc[b], qid[b], row0, a);
+        }
+    }
+    if constexpr (FILTER) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+            if (qid[b] >= 0) *segcnt[b] = count[b];
+    }
 }
 
 // Up to 16 queries on one collection (groups == null), or several collections with groups of up to 16 queries each
@@ -427,16 +558,27 @@ __global__ __launch_bounds__(256) void k_fp4_row_norms(const unsigned char* __re
     if (lane == 0) atomicMax(max_bits, __builtin_bit_cast(unsigned int, wmax));
 }
 
-// sets of 32 queries a wave holds: what its registers take beside the rows in flight
+// blocks of 32 queries a wave holds: what its registers take beside the rows in flight
 constexpr int max_qb(int ks) { return ks <= 12 ? 2 : 1; }
-int wide_qb(int B, int ks) { return B <= 32 ? 1 : max_qb(ks); }
+constexpr int ring_qb(int ks) { return ks <= 16 ? 2 : 1; }
+// with more than two sets of queries a workgroup's four waves take one each and share the rows through LDS
+bool use_ring(int B, int ks) { return B > 64 * ring_qb(ks); }
+int wide_qb(int B, int ks) { return use_ring(B, ks) ? ring_qb(ks) : (B <= 32 ? 1 : max_qb(ks)); }
 int wide_waves(int B, int ks) {
     const int sets = (B + 32 * wide_qb(B, ks) - 1) / (32 * wide_qb(B, ks));
     return sets >= 3 ? 4 : sets;
 }
 
+template <int KS, bool FILTER>
+int launch_ring(const Fp4Args& a, int blocks, hipStream_t s) {
+    static std::atomic<uint64_t> lds_ok;
+    crag_allow_dynamic_lds((const void*)k_scan_fp4_ring<KS, ring_qb(KS), FILTER>, Ring<KS>::BYTES, lds_ok);
+    hipLaunchKernelGGL((k_scan_fp4_ring<KS, ring_qb(KS), FILTER>), dim3((unsigned)blocks), dim3(256), Ring<KS>::BYTES, s, a);
+    return (int)hipGetLastError();
+}
 template <int KS>
 int launch_wide(const Fp4Args& a, int qb, int blocks, bool filter, hipStream_t s) {
+    if (use_ring(a.n_queries, KS)) return filter ? launch_ring<KS, true>(a, blocks, s) : launch_ring<KS, false>(a, blocks, s);
     if (qb == 1) {
         if (filter) hipLaunchKernelGGL((k_scan_fp4<KS, 1, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((k_scan_fp4<KS, 1, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -484,6 +626,16 @@ int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_bl
     return (int)hipGetLastError();
 }
 
+// candidate segments per query that the scan of B queries appends to; 0: flat buffers and atomic counters
+static long long ring_streams(int B, int ks, int n_cus) {
+    const int sets = (B + 32 * ring_qb(ks) - 1) / (32 * ring_qb(ks)), groups = (sets + 3) / 4;
+    return std::max(8, std::min(512, n_cus / groups) / 8 * 8);  // a multiple of eight: one share per XCD
+}
+int crag_fp4_segments(int B, int dim_pad, int n_cus) {
+    const int ks = dim_pad >> 6;
+    return use_ring(B, ks) ? (int)ring_streams(B, ks, n_cus) * 2 : 0;
+}
+
 int crag_launch_scan_fp4(const Fp4Args& args, int dim_pad, bool filter, int n_cus, hipStream_t s) {
     Fp4Args a = args;
     a.groups = nullptr;
@@ -505,6 +657,7 @@ int crag_launch_scan_fp4(const Fp4Args& args, int dim_pad, bool filter, int n_cu
     long long streams = std::max<long long>(1, n_cus / a.query_groups);
     streams = std::min(streams, (tiles + wr - 1) / wr);
     streams = (streams + 7) / 8 * 8;
+    if (use_ring(B, ks)) streams = std::min<long long>(ring_streams(B, ks, n_cus), (tiles + 7) / 8 * 8);
     const int blocks = (int)(streams * a.query_groups);
 #define X(K) \
     case K: return launch_wide<K>(a, qb, blocks, filter, s);
