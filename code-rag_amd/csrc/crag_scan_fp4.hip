@@ -109,21 +109,28 @@ __device__ __forceinline__ void keep_survivors(const f32x16_t& s, float tau, int
 // would wait for.  `count` may pass the segment's room: the selection then takes the query for overflowed.
 __device__ __forceinline__ void keep_survivors_own(const f32x16_t& s, float tau, long long row0, long long row_end, unsigned long long* __restrict__ seg,
                                                    int seg_cap, uint32_t& count) {
-    float m = s[0];
+    float m[4];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) m = fminf(m, s[i]);
-    if (m <= tau) {
+    for (int r = 0; r < 4; ++r) m[r] = fminf(fminf(s[4 * r], s[4 * r + 1]), fminf(s[4 * r + 2], s[4 * r + 3]));
+    if (fminf(fminf(m[0], m[1]), fminf(m[2], m[3])) <= tau) {
+        int room = row_end - row0 < 32 ? (int)(row_end - row0) : 32;
+        asm volatile("" : "+v"(room));  // keeps the comparisons with it in here: hoisted, they would run for every tile
+        const uint32_t row = (uint32_t)row0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const long long row = row0 + 8 * (i >> 2) + (i & 3);
-            if (s[i] <= tau && row < row_end) {
-                if (count < (uint32_t)seg_cap) seg[count] = ((unsigned long long)crag_fkey(s[i]) << 32) | (uint32_t)row;
-                ++count;
+        for (int r = 0; r < 4; ++r)
+            if (m[r] <= tau) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (s[4 * r + j] <= tau && 8 * r + j < room) {
+                        if (count < (uint32_t)seg_cap) seg[count] = ((unsigned long long)crag_fkey(s[4 * r + j]) << 32) | (row + 8 * r + j);
+                        ++count;
+                    }
             }
-        }
     }
 }
-__device__ __forceinline__ void keep_all(const f32x16_t& s, int q, long long row0, const Fp4Args& a) {
+__device__ __forceinline__ void keep_all(const f32x16_t& s_, int q, long long row0, const Fp4Args& a) {
+    f32x16_t s = s_;
+    asm volatile("" : "+v"(s));  // the products stay in front of the branch: inside, all their operands would wait for it
     if (q < 0) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r)  // (rows behind the last one land in the sample's padding, which is a multiple of 64 rows)
@@ -218,28 +225,29 @@ __global__ __launch_bounds__(256, 1) void k_scan_fp4(Fp4Args a) {
     walk<KS, 2, QB, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + stream, streams, (a.row_end + 31) >> 5, a.row_end, a, q, tau, qid, lane);
 }
 
-// The same with four sets of queries per workgroup: the rows' tiles come through a ring in LDS, one copy for the four waves,
-// brought there by loads that write LDS directly and run up to RING - 1 tiles ahead.  The registers hold nothing but the
-// queries, the accumulators and the operands on their way, so two blocks of 32 queries fit for rows of up to 1024 elements
-// and each tile read from LDS feeds twice the products.
+// The same for large batches: the rows' tiles come through a ring in LDS, one copy for all waves of the workgroup, brought
+// there by loads that write LDS directly, half a ring ahead.  The waves meet once per half: a wave that has survivors to
+// write does not hold the others up at every tile.  With nothing else in the registers two waves with 32 queries each fit a
+// SIMD for rows of up to 1024 elements, and one's comparisons run in the shadow of the other's matrix instructions.
 template <int KS>
 struct Ring {
     static constexpr int CHUNKS = KS + (crag_fp4_sw(KS) * 256 + 1023) / 1024;  // 1-KiB pieces of a tile
     static constexpr int SLOT = CHUNKS * 1024 + 128;                            // ... and |x|^2 of its rows
-    static constexpr int LOADS = (CHUNKS + 1 + 3) / 4;                          // per wave: the same number in each, see issue()
-    static constexpr int SLOTS = 155 * 1024 / SLOT < 8 ? 155 * 1024 / SLOT : 8;
+    static constexpr int WAVES = KS <= 16 ? 8 : 4;
+    static constexpr int LOADS = (CHUNKS + WAVES) / WAVES;  // per wave, at most
+    static constexpr int HALF = 77 * 1024 / SLOT < 4 ? 77 * 1024 / SLOT : 4;    // tiles between two barriers; the next ones are on their way
+    static constexpr int SLOTS = 2 * HALF;
     static constexpr int BYTES = SLOT * SLOTS;
 };
 
-// Wave w brings pieces w, w + 4, ... of a tile to LDS offset `slot`.  Waves with fewer pieces repeat their last one, so that
-// every wave has LOADS loads per tile in flight and one counted wait serves all.
+// Wave w brings pieces w, w + WAVES, ... of a tile to LDS offset `slot`.
 template <int KS>
-__device__ __forceinline__ void issue(const GLOBAL_AS unsigned char* tile, const GLOBAL_AS float* xnorm, uint32_t slot, int wave, int lane) {
+__device__ __forceinline__ void issue(const GLOBAL_AS unsigned char* tile, const GLOBAL_AS float* xnorm, uint32_t slot, bool norms, int wave, int lane) {
     using R = Ring<KS>;
 #pragma unroll
     for (int i = 0; i < R::LOADS; ++i) {
-        int c = wave + 4 * i;
-        c = c > R::CHUNKS ? R::CHUNKS : c;  // piece CHUNKS: the norms
+        const int c = wave + R::WAVES * i;
+        if (c > R::CHUNKS || (c == R::CHUNKS && !norms)) break;  // piece CHUNKS: the norms
         const int bytes = c == R::CHUNKS ? 128 : (c == R::CHUNKS - 1 ? (int)crag_fp4_tile_bytes(KS) - 1024 * (R::CHUNKS - 1) : 1024);
         const GLOBAL_AS unsigned char* from = c == R::CHUNKS ? (const GLOBAL_AS unsigned char*)xnorm : tile + c * 1024;
         const uint32_t to = __builtin_amdgcn_readfirstlane(slot + c * 1024);
@@ -248,9 +256,10 @@ __device__ __forceinline__ void issue(const GLOBAL_AS unsigned char* tile, const
     }
 }
 
-template <int KS, int QB, bool FILTER>
-__global__ __launch_bounds__(256, 1) void k_scan_fp4_ring(Fp4Args a) {
+template <int KS, bool FILTER>
+__global__ __launch_bounds__(64 * Ring<KS>::WAVES, Ring<KS>::WAVES / 4) void k_scan_fp4_ring(Fp4Args a) {
     using R = Ring<KS>;
+    constexpr int QB = 1;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int xcd = blockIdx.x & 7, slot_ = blockIdx.x >> 3;
@@ -262,11 +271,14 @@ __global__ __launch_bounds__(256, 1) void k_scan_fp4_ring(Fp4Args a) {
     if (first >= last) return;  // the whole workgroup
     const int n = (int)((last - first + streams - 1) / streams);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+    const bool l2 = a.metric == CRAG_L2;
+    if (!l2 && threadIdx.x < 32)  // the accumulators start at zero: no load writes these
+        for (int i = 0; i < R::SLOTS; ++i) *(float*)(smem + i * R::SLOT + 1024 * R::CHUNKS + 4 * threadIdx.x) = 0.f;
     auto bring = [&](int i) {
         const long long t = first + i * streams;
-        issue<KS>(rows + t * crag_fp4_tile_bytes(KS), xnorm + t * 32, lds0 + (uint32_t)(i % R::SLOTS) * R::SLOT, wave, lane);
+        issue<KS>(rows + t * crag_fp4_tile_bytes(KS), xnorm + t * 32, lds0 + (uint32_t)(i % R::SLOTS) * R::SLOT, l2, wave, lane);
     };
-    const int blk = (qg * 4 + wave) * QB;
+    const int blk = qg * R::WAVES + wave;
     Query<KS, 2> q[QB];
     float tau[QB];
     int qid[QB];
@@ -288,15 +300,13 @@ __global__ __launch_bounds__(256, 1) void k_scan_fp4_ring(Fp4Args a) {
             count[b] = qid[b] < 0 ? 0 : *segcnt[b];
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // from here on the counter holds the ring's loads
-    for (int i = 0; i < R::SLOTS - 1 && i < n; ++i) bring(i);
-    const bool l2 = a.metric == CRAG_L2;
+    for (int i = 0; i < R::HALF && i < n; ++i) bring(i);
     for (int i = 0; i < n; ++i) {
-        // tile i has arrived (only the SLOTS - 2 tiles behind it may be on their way; at the end there are fewer), and every
-        // wave is done with tile i - 1, whose slot the next load takes
-        if (i + R::SLOTS - 1 <= n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R::SLOTS - 2) * R::LOADS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (i + R::SLOTS - 1 < n) bring(i + R::SLOTS - 1);
+        if (i % R::HALF == 0) {
+            // this half of the ring has arrived, and every wave is done with the other one, which the next loads take
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            for (int j = i + R::HALF; j < i + R::SLOTS && j < n; ++j) bring(j);
+        }
         const unsigned char* slot = smem + (i % R::SLOTS) * R::SLOT;
         RowScales<KS> rs;
 #pragma unroll
@@ -304,8 +314,7 @@ __global__ __launch_bounds__(256, 1) void k_scan_fp4_ring(Fp4Args a) {
         f32x16_t acc[QB];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            f32x4_t xn = *(const f32x4_t*)(slot + 1024 * R::CHUNKS + 32 * r + (lane >> 5) * 16);
-            if (!l2) xn = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            const f32x4_t xn = *(const f32x4_t*)(slot + 1024 * R::CHUNKS + 32 * r + (lane >> 5) * 16);
 #pragma unroll
             for (int b = 0; b < QB; ++b)
 #pragma unroll
@@ -560,10 +569,10 @@ __global__ __launch_bounds__(256) void k_fp4_row_norms(const unsigned char* __re
 
 // blocks of 32 queries a wave holds: what its registers take beside the rows in flight
 constexpr int max_qb(int ks) { return ks <= 12 ? 2 : 1; }
-constexpr int ring_qb(int ks) { return ks <= 16 ? 2 : 1; }
-// with more than two sets of queries a workgroup's four waves take one each and share the rows through LDS
-bool use_ring(int B, int ks) { return B > 64 * ring_qb(ks); }
-int wide_qb(int B, int ks) { return use_ring(B, ks) ? ring_qb(ks) : (B <= 32 ? 1 : max_qb(ks)); }
+// with more queries than half of a ring workgroup's, they share the rows through LDS
+constexpr int ring_queries(int ks) { return ks <= 16 ? 256 : 128; }
+bool use_ring(int B, int ks) { return B > ring_queries(ks) / 2; }
+int wide_qb(int B, int ks) { return B <= 32 ? 1 : max_qb(ks); }
 int wide_waves(int B, int ks) {
     const int sets = (B + 32 * wide_qb(B, ks) - 1) / (32 * wide_qb(B, ks));
     return sets >= 3 ? 4 : sets;
@@ -572,8 +581,9 @@ int wide_waves(int B, int ks) {
 template <int KS, bool FILTER>
 int launch_ring(const Fp4Args& a, int blocks, hipStream_t s) {
     static std::atomic<uint64_t> lds_ok;
-    crag_allow_dynamic_lds((const void*)k_scan_fp4_ring<KS, ring_qb(KS), FILTER>, Ring<KS>::BYTES, lds_ok);
-    hipLaunchKernelGGL((k_scan_fp4_ring<KS, ring_qb(KS), FILTER>), dim3((unsigned)blocks), dim3(256), Ring<KS>::BYTES, s, a);
+    static_assert(ring_queries(KS) == 32 * Ring<KS>::WAVES, "queries of a workgroup");
+    crag_allow_dynamic_lds((const void*)k_scan_fp4_ring<KS, FILTER>, Ring<KS>::BYTES, lds_ok);
+    hipLaunchKernelGGL((k_scan_fp4_ring<KS, FILTER>), dim3((unsigned)blocks), dim3(64 * Ring<KS>::WAVES), Ring<KS>::BYTES, s, a);
     return (int)hipGetLastError();
 }
 template <int KS>
@@ -614,6 +624,7 @@ int crag_fp4_dim_pad(int dim) {
 // query blocks of the single-collection scan for B queries (the wide form's waves take whole sets of them)
 int crag_fp4_query_blocks(int B, int dim_pad) {
     if (B <= CRAG_FP4_GROUP_Q) return 1;
+    if (use_ring(B, dim_pad >> 6)) return (B + ring_queries(dim_pad >> 6) - 1) / ring_queries(dim_pad >> 6) * (ring_queries(dim_pad >> 6) / 32);
     const int per = wide_qb(B, dim_pad >> 6) * wide_waves(B, dim_pad >> 6);
     return ((B + 31) / 32 + per - 1) / per * per;
 }
@@ -628,7 +639,7 @@ int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_bl
 
 // candidate segments per query that the scan of B queries appends to; 0: flat buffers and atomic counters
 static long long ring_streams(int B, int ks, int n_cus) {
-    const int sets = (B + 32 * ring_qb(ks) - 1) / (32 * ring_qb(ks)), groups = (sets + 3) / 4;
+    const int groups = (B + ring_queries(ks) - 1) / ring_queries(ks);
     return std::max(8, std::min(512, n_cus / groups) / 8 * 8);  // a multiple of eight: one share per XCD
 }
 int crag_fp4_segments(int B, int dim_pad, int n_cus) {
@@ -650,14 +661,17 @@ int crag_launch_scan_fp4(const Fp4Args& args, int dim_pad, bool filter, int n_cu
 #undef X
     }
     const int qb = wide_qb(B, ks), sets = (B + 32 * qb - 1) / (32 * qb);
-    a.wave_queries = wide_waves(B, ks);
-    a.query_groups = (sets + a.wave_queries - 1) / a.wave_queries;
-    const int wr = 4 / a.wave_queries;
-    // streams of tiles: a multiple of eight (one share per XCD), no more than there are tiles
-    long long streams = std::max<long long>(1, n_cus / a.query_groups);
-    streams = std::min(streams, (tiles + wr - 1) / wr);
-    streams = (streams + 7) / 8 * 8;
-    if (use_ring(B, ks)) streams = std::min<long long>(ring_streams(B, ks, n_cus), (tiles + 7) / 8 * 8);
+    long long streams;  // of tiles: a multiple of eight (one share per XCD), no more than there are tiles
+    if (use_ring(B, ks)) {
+        a.query_groups = (B + ring_queries(ks) - 1) / ring_queries(ks);
+        streams = std::min<long long>(ring_streams(B, ks, n_cus), (tiles + 7) / 8 * 8);
+    } else {
+        a.wave_queries = wide_waves(B, ks);
+        a.query_groups = (sets + a.wave_queries - 1) / a.wave_queries;
+        const int wr = 4 / a.wave_queries;
+        streams = std::min<long long>(std::max(1, n_cus / a.query_groups), (tiles + wr - 1) / wr);
+        streams = (streams + 7) / 8 * 8;
+    }
     const int blocks = (int)(streams * a.query_groups);
 #define X(K) \
     case K: return launch_wide<K>(a, qb, blocks, filter, s);
