@@ -212,6 +212,14 @@ def _rows(n, d, g):
     return x.div_(x.norm(dim=-1, keepdim=True))
 
 
+def _framework():
+    import sys
+    if "code-rag_amd" not in sys.path:
+        sys.path.insert(0, "code-rag_amd")
+    import coderag_hip
+    return coderag_hip
+
+
 def prepare(case, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     if case["op"] in ("search", "multi"):
@@ -227,10 +235,7 @@ def prepare(case, seed):
         queries = _unit(rows[at] + torch.randn((case["queries"], d), generator=g, device="cuda") * (0.7 / math.sqrt(d)))
         state = {"case": case, "queries": queries}
         if own:
-            import sys
-            if "code-rag_amd" not in sys.path:
-                sys.path.insert(0, "code-rag_amd")
-            import coderag_hip as ch
+            ch = _framework()
             state["cols"] = []
             for k in range(cols):
                 col = ch.GpuCollection(d, "fp4", case["metric"])
@@ -270,7 +275,7 @@ def prepare(case, seed):
 def run(state):
     case = state["case"]
     if own:
-        import coderag_hip as ch
+        ch = _framework()
         if case["op"] == "search":
             return state["cols"][0].search_device(state["queries"], top_k=case["top_k"])
         if case["op"] == "multi":
