@@ -1875,7 +1875,7 @@ int crag_embed_forward_device(int device, const void* table_dev, int64_t vocab, 
     if (mode < CRAG_POOL_SUM || mode > CRAG_POOL_SQRT) return fail(CRAG_E_INVALID, "crag_embed_forward_device: unknown pooling mode");
     if (out_dtype != CRAG_F32 && out_dtype != CRAG_BF16) return fail(CRAG_E_INVALID, "crag_embed_forward_device: vectors are float32 or bf16");
     if (n_bags == 0) return 0;
-    if (!out_dev) return fail(CRAG_E_INVALID, "crag_embed_forward_device: null output");
+    if (!out_dev || ((uintptr_t)out_dev & 15) != 0) return fail(CRAG_E_INVALID, "crag_embed_forward_device: the output must be a 16-byte aligned buffer");
     e.table = table_dev;
     e.vocab = vocab;
     e.dim = dim;

@@ -301,6 +301,7 @@ struct CragSegArgs {
     const void* src;   // rows that are gathered: the table, or the bags' gradients
     long long n;       // positions
     long long n_share; // groups of lanes, each walks `share` positions
+    long long sum_blocks;  // backward: the blocks behind them clear the rows of tokens that do not occur
     int share, lpr, dim, vocab, n_seg;
     const int* ids;            // forward
     const float* weights;
@@ -308,7 +309,9 @@ struct CragSegArgs {
     const uint32_t *keys, *perm;  // backward: sorted tokens and their positions
     const int* bag;               // backward: bag of a position
     float* partial;    // [n_share][2][dim]: sum of a segment that began in front of the share, of one that goes on behind it
-    int *partial_seg, *partial_count;  // [n_share][2]
+    int *partial_seg, *partial_count;  // [n_share][2]: backward, forward
+    float* sums;       // forward: [n_seg][dim] plain sums of the bags that lie in one share, and how many tokens each has
+    int* sums_count;
     void* out;
     int out_dtype, mode, normalize;
     float scale;

@@ -8,12 +8,11 @@
 // Both sums are one operation, a segmented sum of gathered, weighted rows: forward the segments are the bags and the rows
 // come from the table; backward the segments are the runs of equal tokens among the occurrences sorted by (token,
 // position) and the rows are the bags' dp.  k_segsum walks equal shares of the positions whatever the segments' lengths;
-// a segment that crosses a share's border leaves partial sums that k_segjoin adds in the order of the positions.  No
-// atomics: the same inputs give the same bits.
+// a segment that crosses a share's border leaves partial sums that k_embed_finish (forward) and k_segjoin (backward) add in
+// the order of the positions.  No atomics on sums: the same inputs give the same bits.
 //
 // Stands in front of retriever/hybrid_search.py:60-64 of the reference, which embeds the query text before the search.
 #include <algorithm>
-#include <initializer_list>
 
 #include "crag_common.h"
 
@@ -30,58 +29,55 @@ __device__ __forceinline__ uint32_t f32_bf16(float f) {  // round to nearest eve
     return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
 }
 
-// VEC consecutive elements of a row (aligned to VEC elements or 16 bytes)
+// VEC consecutive elements of a row as they lie in memory (aligned to VEC elements or 16 bytes)
 template <int DT, int VEC>
-__device__ __forceinline__ void load_vec(const void* p, long long i, float (&x)[VEC]) {
-    if constexpr (DT == CRAG_F32) {
-        const float* f = (const float*)p + i;
-        if constexpr (VEC % 4 == 0) {
-#pragma unroll
-            for (int j = 0; j < VEC; j += 4) {
-                const f32x4_t v = *(const f32x4_t*)(f + j);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[j + k] = v[k];
-            }
-        } else if constexpr (VEC == 2) {
-            const f32x2_t v = *(const f32x2_t*)f;
-            x[0] = v[0];
-            x[1] = v[1];
+struct Raw {
+    static constexpr int WORDS = DT == CRAG_F32 ? VEC : (VEC + 1) / 2;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const void* p, long long i) {
+        if constexpr (DT == CRAG_BF16 && VEC == 1) {
+            w[0] = ((const unsigned short*)p)[i];
         } else {
-            x[0] = *f;
-        }
-    } else {
-        const unsigned short* h = (const unsigned short*)p + i;
-        if constexpr (VEC == 8) {
-            const u32x4_t v = *(const u32x4_t*)h;
+            const uint32_t* u = (const uint32_t*)((const char*)p + i * (DT == CRAG_F32 ? 4 : 2));
+            if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                x[2 * k] = bf16_f32(v[k] & 0xffffu);
-                x[2 * k + 1] = bf16_f32(v[k] >> 16);
+                for (int j = 0; j < WORDS; j += 4) {
+                    const u32x4_t v = *(const u32x4_t*)(u + j);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[j + k] = v[k];
+                }
+            } else if constexpr (WORDS == 2) {
+                const uint2 v = *(const uint2*)u;
+                w[0] = v.x;
+                w[1] = v.y;
+            } else {
+                w[0] = *u;
             }
-        } else if constexpr (VEC == 2) {
-            const uint32_t v = *(const uint32_t*)h;
-            x[0] = bf16_f32(v & 0xffffu);
-            x[1] = bf16_f32(v >> 16);
-        } else if constexpr (VEC == 4) {
-            const uint2 v = *(const uint2*)h;
-            x[0] = bf16_f32(v.x & 0xffffu);
-            x[1] = bf16_f32(v.x >> 16);
-            x[2] = bf16_f32(v.y & 0xffffu);
-            x[3] = bf16_f32(v.y >> 16);
-        } else {
-            x[0] = bf16_f32(*h);
         }
     }
-}
-template <int VEC>
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int k = 0; k < WORDS; ++k) w[k] = 0;
+    }
+    __device__ __forceinline__ float get(int k) const {
+        if constexpr (DT == CRAG_F32) return __builtin_bit_cast(float, w[k]);
+        else return __builtin_bit_cast(float, k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    }
+};
+// STREAM: past the caches
+template <int VEC, bool STREAM = false>
 __device__ __forceinline__ void store_vec(void* p, int dt, long long i, const float (&x)[VEC]) {
+    auto put = [](auto v, auto* to) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+        else *to = v;
+    };
     if (dt == CRAG_F32) {
         float* f = (float*)p + i;
         if constexpr (VEC % 4 == 0) {
 #pragma unroll
-            for (int k = 0; k < VEC; k += 4) *(f32x4_t*)(f + k) = (f32x4_t){x[k], x[k + 1], x[k + 2], x[k + 3]};
+            for (int k = 0; k < VEC; k += 4) put((f32x4_t){x[k], x[k + 1], x[k + 2], x[k + 3]}, (f32x4_t*)(f + k));
         } else if constexpr (VEC == 2) {
-            *(f32x2_t*)f = (f32x2_t){x[0], x[1]};
+            put((f32x2_t){x[0], x[1]}, (f32x2_t*)f);
         } else {
             *f = x[0];
         }
@@ -96,8 +92,30 @@ __device__ __forceinline__ void store_vec(void* p, int dt, long long i, const fl
     }
 }
 
-// A row is held by `lpr` lanes (8 .. 64, a power of two), NV pieces of VEC elements in each: lane `sub` holds elements
-// (n * lpr + sub) * VEC ..., n < NV.
+// A row of `dim` elements is held by `lpr` lanes (8 .. 64, a power of two), NV pieces of VEC elements in each: lane `sub` holds
+// elements (n * lpr + sub) * VEC .., n < NV.
+struct Cols {
+    int dim, lpr, sub;
+};
+// What a lane adds to a row's address for each of its pieces.  Lanes past the row's end take its last piece: every load is
+// unconditional, and what they hold is never used (Row::clear_tail, Row::store).
+template <int DT, int VEC, int NV>
+struct Pieces {
+    int at[NV];  // elements
+    __device__ __forceinline__ explicit Pieces(const Cols& c) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) at[n] = min((n * c.lpr + c.sub) * VEC, c.dim - VEC);
+    }
+};
+template <int DT, int VEC, int NV>
+struct RawRow {
+    Raw<DT, VEC> r[NV];
+    __device__ __forceinline__ void load(const void* base, long long row, int dim, const Pieces<DT, VEC, NV>& p) {
+        const char* q = (const char*)base + row * (long long)dim * (DT == CRAG_F32 ? 4 : 2);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) r[n].load(q, p.at[n]);
+    }
+};
 template <int VEC, int NV>
 struct Row {
     float x[NV][VEC];
@@ -108,23 +126,20 @@ struct Row {
             for (int k = 0; k < VEC; ++k) x[n][k] = 0.f;
     }
     template <int DT>
-    __device__ __forceinline__ void load(const void* base, long long row, int dim, int lpr, int sub, bool on) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int e = (n * lpr + sub) * VEC;
-            if (on && e < dim) {
-                load_vec<DT, VEC>(base, row * dim + e, x[n]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) x[n][k] = 0.f;
-            }
-        }
-    }
-    __device__ __forceinline__ void fma(const Row& o, float w) {
+    __device__ __forceinline__ void load(const void* base, long long row, int dim, const Pieces<DT, VEC, NV>& p) {
+        RawRow<DT, VEC, NV> o;
+        o.load(base, row, dim, p);
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[n][k] = fmaf(o.x[n][k], w, x[n][k]);
+            for (int k = 0; k < VEC; ++k) x[n][k] = o.r[n].get(k);
+    }
+    template <int DT>
+    __device__ __forceinline__ void fma(const RawRow<DT, VEC, NV>& o, float w) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[n][k] = fmaf(o.r[n].get(k), w, x[n][k]);
     }
     __device__ __forceinline__ void add(const Row& o) {
 #pragma unroll
@@ -132,14 +147,28 @@ struct Row {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) x[n][k] += o.x[n][k];
     }
-    __device__ __forceinline__ void store(void* base, int dt, long long row, int dim, int lpr, int sub) const {
+    __device__ __forceinline__ void clear_tail(const Cols& c) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+            if ((n * c.lpr + c.sub) * VEC >= c.dim) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) x[n][k] = 0.f;
+            }
+    }
+    template <bool STREAM = false>
+    __device__ __forceinline__ void store(void* base, int dt, long long row, const Cols& c) const {
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int e = (n * lpr + sub) * VEC;
-            if (e < dim) store_vec<VEC>(base, dt, row * dim + e, x[n]);
+            const int e = (n * c.lpr + c.sub) * VEC;
+            if (e < c.dim) store_vec<VEC, STREAM>(base, dt, row * c.dim + e, x[n]);
         }
     }
 };
+// rows in flight per group of lanes
+template <int DT, int VEC, int NV>
+constexpr int rows_ahead() {
+    return Raw<DT, VEC>::WORDS * NV <= 4 ? 8 : (Raw<DT, VEC>::WORDS * NV <= 24 ? 4 : 2);
+}
 
 // Last entry of off[0 .. n] that is <= p, as its index (-1: none)
 __device__ __forceinline__ int last_le(const long long* __restrict__ off, int n, long long p) {
@@ -151,46 +180,83 @@ __device__ __forceinline__ int last_le(const long long* __restrict__ off, int n,
     return lo;
 }
 
-// A finished segment's epilogue: forward scale, pool factor, norm and coefficient; backward nothing.  All lanes of the row.
-template <bool BWD, int VEC, int NV>
-__device__ __forceinline__ void finish(const CragSegArgs& a, long long seg, Row<VEC, NV>& r, int count, int sub) {
-    if constexpr (!BWD) {
-        float f = a.scale;
-        if (a.mode == CRAG_POOL_MEAN) f = (float)((double)a.scale / (count > 0 ? count : 1));
-        if (a.mode == CRAG_POOL_SQRT) f = (float)((double)a.scale / sqrt((double)(count > 0 ? count : 1)));
-        float coef = f;
-        if (a.normalize) {
-            // |p| in float64: squares of float32 neither overflow nor vanish there
-            double ss = 0.0;
+// A bag's epilogue: scale, pool factor, norm, coefficient; the row is held whole by lpr lanes.
+template <int VEC, int NV>
+__device__ __forceinline__ void finish_bag(const CragSegArgs& a, long long bag, Row<VEC, NV>& r, int count, const Cols& c) {
+    float f = a.scale;
+    if (a.mode == CRAG_POOL_MEAN) f = (float)((double)a.scale / (count > 0 ? count : 1));
+    if (a.mode == CRAG_POOL_SQRT) f = (float)((double)a.scale / sqrt((double)(count > 0 ? count : 1)));
+    float coef = f;
+    if (a.normalize) {
+        // |p| in float64: squares of float32 neither overflow nor vanish there
+        r.clear_tail(c);
+        double ss = 0.0;
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
+        for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) ss += (double)r.x[n][k] * (double)r.x[n][k];
-            for (int o = a.lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-            const double s = sqrt(ss);  // of the unscaled sum: y = sign(f) * sum / |sum|
-            const double inv = s > 0.0 && f != 0.f ? (f < 0.f ? -1.0 : 1.0) / s : 0.0 * s;
+            for (int k = 0; k < VEC; ++k) ss += (double)r.x[n][k] * (double)r.x[n][k];
+        for (int o = c.lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+        const double s = sqrt(ss);  // of the unscaled sum: y = sign(f) * sum / |sum|
+        const double inv = s > 0.0 && f != 0.f ? (f < 0.f ? -1.0 : 1.0) / s : 0.0 * s;
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
+        for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) r.x[n][k] = (float)((double)r.x[n][k] * inv);
-            coef = (float)inv;  // s c_b / |s c_b sum|
-        } else {
+            for (int k = 0; k < VEC; ++k) r.x[n][k] = (float)((double)r.x[n][k] * inv);
+        coef = (float)inv;  // s c_b / |s c_b sum|
+    } else {
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
+        for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) r.x[n][k] *= f;
-        }
-        if (a.coef && sub == 0) a.coef[seg] = coef;
+            for (int k = 0; k < VEC; ++k) r.x[n][k] *= f;
     }
-    r.store(a.out, a.out_dtype, seg, a.dim, a.lpr, sub);
+    if (a.coef && c.sub == 0) a.coef[bag] = coef;
+    r.store(a.out, a.out_dtype, bag, c);
 }
 
-// One group of lpr lanes walks the positions [g * share, (g + 1) * share).
+// Backward, the blocks behind those of the sums: rows of tokens that do not occur are zero.  A thread looks its token up
+// among the sorted keys, a wave writes the rows of its 64 tokens -- past the caches, which hold the table's rows.
+__device__ __forceinline__ void zero_absent(const CragSegArgs& a, long long block) {
+    const int lane = threadIdx.x & 63;
+    const long long first = block * 256 + (threadIdx.x & ~63), v = first + lane;
+    bool absent = false;
+    if (v < a.vocab) {
+        long long lo = 0, hi = a.n;  // the first position whose key is not below v
+        while (lo < hi) {
+            const long long mid = (lo + hi) >> 1;
+            if ((long long)a.keys[mid] < v) lo = mid + 1; else hi = mid;
+        }
+        absent = lo == a.n || (long long)a.keys[lo] != v;
+    }
+    const long long bytes = (long long)a.dim * (a.out_dtype == CRAG_F32 ? 4 : 2);
+    for (unsigned long long m = __ballot(absent); m; m &= m - 1) {
+        char* row = (char*)a.out + (first + __builtin_ctzll(m)) * bytes;
+        if (bytes % 16 == 0) {
+            for (int i = lane * 16; i < bytes; i += 1024) __builtin_nontemporal_store((u32x4_t){0, 0, 0, 0}, (u32x4_t*)(row + i));
+        } else {
+            for (int i = lane * 2; i < bytes; i += 128) *(uint16_t*)(row + i) = 0;
+        }
+    }
+}
+
+// One group of lpr lanes walks the positions [g * share, (g + 1) * share).  A segment that lies whole in a share is stored:
+// backward that is the token's gradient, forward a plain sum for k_embed_finish (scale, norm and count would cost this
+// kernel's registers half of its waves).
 template <int DT, bool BWD, int VEC, int NV>
 __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
-    constexpr int U = NV * VEC <= 8 ? 8 : 4;  // rows in flight
+    constexpr int U = rows_ahead<DT, VEC, NV>();
+    if constexpr (BWD) {
+        if ((long long)blockIdx.x >= a.sum_blocks) {
+            zero_absent(a, (long long)blockIdx.x - a.sum_blocks);
+            return;
+        }
+    }
     const int lane = threadIdx.x & 63;
-    const int lpr = a.lpr, sub = lane & (lpr - 1), first = lane & ~(lpr - 1);
+    const int lpr = a.lpr, first = lane & ~(lpr - 1);
+    Cols c;
+    c.dim = a.dim;
+    c.lpr = lpr;
+    c.sub = lane & (lpr - 1);
+    const int sub = c.sub;
     const long long g = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / lpr) + lane / lpr;
     const long long T = a.n;
     long long p0 = g * a.share;
@@ -201,46 +267,76 @@ __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
     long long seg = -1;       // segment the running sum belongs to
     bool before = false;      // ... and it has positions in front of this share
     int count = 0;
-    long long head = -1, tail = -1;
+    int head = -1, tail = -1;
     if constexpr (!BWD) {
         lo = a.offsets[0];
         hi = a.offsets[a.n_seg];
         lo = lo < 0 ? 0 : lo;
         hi = hi > T ? T : hi;
     }
+    const Pieces<DT, VEC, NV> pieces(c);
     Row<VEC, NV> acc;
     acc.zero();
-    auto partial = [&](int which) {
-        acc.store(a.partial, CRAG_F32, 2 * g + which, a.dim, lpr, sub);
-        if (sub == 0) a.partial_count[2 * g + which] = count;
-        (which == 0 ? head : tail) = seg;
-    };
-    for (long long base = p0; base < p0 + a.share; base += lpr) {  // the same number of rounds in every group
-        // what each position of the round reads: lane `sub` looks up position base + sub
-        const long long pm = base + sub;
-        int row = -1, key = -1;
-        float w = 0.f;
-        if (pm < p1) {
-            if constexpr (BWD) {
-                key = (int)a.keys[pm];
-                if (key < a.vocab) {
-                    const uint32_t t = a.perm[pm];
-                    row = a.bag[t];
-                    w = a.weights ? a.weights[t] : 1.f;
-                } else {
-                    key = -1;
-                }
-            } else if (pm >= lo && pm < hi) {
-                const int id = a.ids[pm];
-                if (id >= 0 && id < a.vocab) {
-                    row = id;
-                    w = a.weights ? a.weights[pm] : 1.f;
-                }
-            }
+    auto done = [&](bool after) {
+        if (before || after) {
+            const int which = before ? 0 : 1;
+            acc.store(a.partial, CRAG_F32, 2 * g + which, c);
+            if (!BWD && sub == 0) a.partial_count[2 * g + which] = count;
+            if (before) head = (int)seg; else tail = (int)seg;
+        } else if constexpr (BWD) {
+            acc.template store<true>(a.out, a.out_dtype, seg, c);
+        } else {
+            acc.store(a.sums, CRAG_F32, seg, c);
+            if (sub == 0) a.sums_count[seg] = count;
         }
-        const int rounds = a.share < lpr ? a.share : lpr;
+    };
+    // What each position of a round reads: lane `sub` looks up position base + sub.  Forward that is its token and weight;
+    // backward its key and where it was before the sort, and with that its bag and weight.  All of it is asked for a round
+    // ahead (backward the first half two rounds): waited for in turn, a round's lookups would cost as much as its rows.
+    auto look_up = [&](long long pm, int& i, float& f) {
+        i = -1;
+        f = 0.f;
+        if (pm >= p1) return;
+        if constexpr (BWD) {
+            const uint32_t k = a.keys[pm];
+            i = k < (uint32_t)a.vocab ? (int)k : -1;
+            f = __builtin_bit_cast(float, a.perm[pm]);
+        } else {
+            const int id = a.ids[pm];
+            f = a.weights ? a.weights[pm] : 1.f;
+            i = pm >= lo && pm < hi && id >= 0 && id < a.vocab ? id : -1;
+        }
+    };
+    auto of_bag = [&](int k, float was, int& r, float& f) {
+        r = -1;
+        f = 0.f;
+        if (k < 0) return;
+        const uint32_t t = __builtin_bit_cast(uint32_t, was);
+        r = a.bag[t];
+        f = a.weights ? a.weights[t] : 1.f;
+    };
+    int row, key = -1, row_n, key_n = -1;
+    float w, w_n, was_n = 0.f;
+    if constexpr (BWD) {
+        float was;
+        look_up(p0 + sub, key, was);
+        look_up(p0 + lpr + sub, key_n, was_n);
+        of_bag(key, was, row, w);
+    } else {
+        look_up(p0 + sub, row, w);
+    }
+    for (long long base = p0; base < p0 + a.share; base += lpr) {  // the same number of rounds in every group
+        int key_nn = -1;
+        float was_nn = 0.f;
+        if constexpr (BWD) {
+            of_bag(key_n, was_n, row_n, w_n);
+            look_up(base + 2 * lpr + sub, key_nn, was_nn);
+        } else {
+            look_up(base + lpr + sub, row_n, w_n);
+        }
+        const int rounds = p0 + a.share - base < lpr ? (int)(p0 + a.share - base) : lpr;
         for (int j = 0; j < rounds; j += U) {
-            Row<VEC, NV> x[U];
+            RawRow<DT, VEC, NV> x[U];
             float wu[U];
             int ru[U], ku[U];
 #pragma unroll
@@ -248,207 +344,378 @@ __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
                 ru[u] = __shfl(row, first + j + u);
                 wu[u] = __shfl(w, first + j + u);
                 if constexpr (BWD) ku[u] = __shfl(key, first + j + u);
-                x[u].template load<DT>(a.src, ru[u], a.dim, lpr, sub, ru[u] >= 0);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const long long p = base + j + u;
-                if (p >= p1) continue;
-                if constexpr (BWD) {
+            for (int u = 0; u < U; ++u) x[u].load(a.src, max(ru[u], 0), a.dim, pieces);
+            if constexpr (BWD) {
+                // tokens change at every few positions, and the end of a run is short: one stands at each position
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const long long p = base + j + u;
+                    if (p >= p1) continue;
                     const int k = ku[u];
                     if (k != (int)seg || p == p0) {
-                        if (p != p0 && seg >= 0) {
-                            if (before) partial(0); else finish<BWD>(a, seg, acc, count, sub);
-                        }
+                        if (p != p0 && seg >= 0) done(false);
                         before = p == p0 && p > 0 && k >= 0 && (int)a.keys[p - 1] == k;
                         seg = k;
                         acc.zero();
                     }
                     if (k >= 0) acc.fma(x[u], wu[u]);
-                } else {
-                    if (p < lo || p >= hi) continue;
+                }
+            } else {
+                // the common case, for all groups of the wave at once: U rows of the bag that the sum belongs to
+                bool plain = seg >= 0 && base + j + U <= p1 && base + j + U <= end && base + j + U <= hi;
+#pragma unroll
+                for (int u = 0; u < U; ++u) plain = plain && ru[u] >= 0;
+                if (__all(plain)) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) acc.fma(x[u], wu[u]);
+                    count += U;
+                    continue;
+                }
+                // a border of bags or shares, or padding: one position after the other, out of the cache that the loads above
+                // filled (with the rows of both ways in registers half as many waves would fit)
+#pragma unroll 1
+                for (int u = 0; u < U; ++u) {
+                    const long long p = base + j + u;
+                    if (p >= p1) break;
+                    const int r = __shfl(row, first + j + u);
+                    const float wp = __shfl(w, first + j + u);
+                    if (p < lo) continue;
+                    if (p >= hi) break;
                     if (seg < 0 || p >= end) {
-                        if (seg >= 0) {
-                            if (before) partial(0); else finish<BWD>(a, seg, acc, count, sub);
-                        }
+                        if (seg >= 0) done(false);
                         seg = last_le(a.offsets, a.n_seg, p);
-                        if (seg >= a.n_seg) { seg = -1; hi = p; continue; }
+                        if (seg >= a.n_seg) {
+                            seg = -1;
+                            hi = p;
+                            break;
+                        }
                         end = a.offsets[seg + 1];
-                        before = a.offsets[seg] < p0 && p == p0;
+                        before = a.offsets[seg] < p0 && p == p0 && p0 > lo;
                         count = 0;
                         acc.zero();
                     }
-                    if (ru[u] >= 0) {
-                        acc.fma(x[u], wu[u]);
+                    if (r >= 0) {
+                        RawRow<DT, VEC, NV> one;
+                        one.load(a.src, r, a.dim, pieces);
+                        acc.fma(one, wp);
                         ++count;
                     }
                 }
             }
         }
+        row = row_n;
+        w = w_n;
+        if constexpr (BWD) {
+            key = key_n;
+            key_n = key_nn;
+            was_n = was_nn;
+        }
     }
     if (seg >= 0) {
-        bool after;
-        if constexpr (BWD) after = p1 < T && (int)a.keys[p1] == (int)seg;
-        else after = p1 < hi && end > p1;
-        if (before) partial(0);
-        else if (after) partial(1);
-        else finish<BWD>(a, seg, acc, count, sub);
+        if constexpr (BWD) done(p1 < T && (int)a.keys[p1] == (int)seg);
+        else done(p1 < hi && end > p1);
     }
-    if (sub == 0 && g < a.n_share) {
-        a.partial_seg[2 * g] = (int)head;
-        a.partial_seg[2 * g + 1] = (int)tail;
+    if (BWD && sub == 0 && g < a.n_share) {
+        a.partial_seg[2 * g] = head;
+        a.partial_seg[2 * g + 1] = tail;
     }
 }
 
-// Blocks [0, n_share): the segment whose first partial sum is share g's tail -- it goes on through the heads of the shares
-// behind it.  Blocks behind that: forward, the bags without positions.
-template <bool BWD, int VEC, int NV>
+// Sums of `n` partial rows -- slot(0), slot(1), ... in this order -- by `gp` groups of lanes of a block, group `grp` of them
+// a run each; the result is in group 0.  All threads of the block come here (barriers).
+template <int VEC, int NV, typename Slot>
+__device__ __forceinline__ int join_rows(const CragSegArgs& a, int n, int grp, int gp, int slot_of_block, Slot slot, const Cols& c, float* part,
+                                         int* part_count, Row<VEC, NV>& acc) {
+    const int per = (n + gp - 1) / gp, i0 = grp * per, i1 = i0 + per < n ? i0 + per : n;
+    const Pieces<CRAG_F32, VEC, NV> pieces(c);
+    int count = 0;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) {
+        const long long s = slot(i);
+        Row<VEC, NV> x;
+        x.template load<CRAG_F32>(a.partial, s, a.dim, pieces);
+        acc.add(x);
+        if (a.partial_count) count += a.partial_count[s];
+    }
+    if (gp == 1) return count;
+    const int rowlen = c.lpr * VEC * NV;
+    if (grp > 0) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) part[slot_of_block * rowlen + (v * c.lpr + c.sub) * VEC + k] = acc.x[v][k];
+        if (c.sub == 0) part_count[slot_of_block] = count;
+    }
+    __syncthreads();
+    if (grp == 0)
+        for (int o = 1; o < gp && o * per < n; ++o) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc.x[v][k] += part[(slot_of_block + o) * rowlen + (v * c.lpr + c.sub) * VEC + k];
+            count += part_count[slot_of_block + o];
+        }
+    return count;
+}
+
+// Forward, after k_segsum: every bag, from its sum or, where it crosses borders of shares, from its partial sums.  `gp` groups
+// of lanes per bag.
+template <int VEC, int NV>
+__global__ __launch_bounds__(256) void k_embed_finish(CragSegArgs a, int gp) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ int part_count[64];
+    float* part = (float*)smem;  // [256 / lpr][lpr * VEC * NV]
+    Cols c;
+    c.dim = a.dim;
+    c.lpr = a.lpr;
+    c.sub = threadIdx.x & (a.lpr - 1);
+    const int slot_of_block = threadIdx.x / a.lpr, grp = slot_of_block % gp;
+    const long long b = ((long long)blockIdx.x * (256 / a.lpr) + slot_of_block) / gp;
+    long long x0 = 0, x1 = 0, g0 = 0, g1 = -1;
+    int n = 0;
+    if (b < a.n_seg) {
+        x0 = a.offsets[b];
+        x1 = a.offsets[b + 1];
+        x0 = x0 < 0 ? 0 : x0;
+        x1 = x1 > a.n ? a.n : x1;
+        if (x0 < x1) {
+            g0 = x0 / a.share;
+            g1 = (x1 - 1) / a.share;
+            n = g0 == g1 ? 0 : (int)(g1 - g0 + 1);
+        }
+    }
+    Row<VEC, NV> acc;
+    acc.zero();
+    // the bag is the tail of share g0 unless it begins with that share, and the head of the others; where it begins with
+    // share g0 and goes on, that is the tail as well (nothing of it lies in front)
+    int count = join_rows<VEC, NV>(a, n, grp, gp, slot_of_block, [&](int i) { return i == 0 ? 2 * g0 + 1 : 2 * (g0 + i); }, c, part, part_count, acc);
+    if (b >= a.n_seg || grp != 0) return;
+    if (n == 0 && x0 < x1) {
+        acc.template load<CRAG_F32>(a.sums, b, a.dim, Pieces<CRAG_F32, VEC, NV>(c));
+        count = a.sums_count[b];
+    }
+    finish_bag(a, b, acc, count, c);
+}
+
+// Backward, after k_segsum: block g joins the token whose first partial sum is share g's tail -- it goes on through the heads
+// of the shares behind it.
+template <int VEC, int NV>
 __global__ __launch_bounds__(256) void k_segjoin(CragSegArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    float* part = (float*)smem;  // [256 / lpr][dim of a row as held: lpr * VEC * NV]
-    __shared__ int s_end, s_count;
-    const int tid = threadIdx.x, lpr = a.lpr, sub = tid & (lpr - 1), grp = tid / lpr, groups = 256 / lpr;
-    if ((long long)blockIdx.x >= a.n_share) {
-        if constexpr (!BWD) {
-            const long long stride = (long long)(gridDim.x - a.n_share) * groups;
-            for (long long b = ((long long)blockIdx.x - a.n_share) * groups + grp; b < a.n_seg; b += stride) {
-                long long x0 = a.offsets[b], x1 = a.offsets[b + 1];
-                x0 = x0 < 0 ? 0 : x0;
-                x1 = x1 > a.n ? a.n : x1;
-                if (x0 < x1) continue;
-                Row<VEC, NV> r;
-                r.zero();
-                finish<BWD>(a, b, r, 0, sub);
-            }
-        }
-        return;
-    }
+    __shared__ int part_count[64];
+    __shared__ int s_end;
+    const int tid = threadIdx.x;
     const long long g = blockIdx.x;
     const int seg = a.partial_seg[2 * g + 1];
     if (seg < 0) return;
-    if (tid == 0) {
-        s_end = 0x7fffffff;
-        s_count = 0;
-    }
+    Cols c;
+    c.dim = a.dim;
+    c.lpr = a.lpr;
+    c.sub = tid & (a.lpr - 1);
+    if (tid == 0) s_end = 0x7fffffff;
     __syncthreads();
-    // the last share that holds a head of this segment
-    for (long long j0 = g + 1;; j0 += 256) {
+    for (long long j0 = g + 1;; j0 += 256) {  // the last share that holds a head of this token
         const long long j = j0 + tid;
         if (j >= a.n_share || a.partial_seg[2 * j] != seg) atomicMin(&s_end, (int)(j < a.n_share ? j : a.n_share));
         __syncthreads();
         if (s_end != 0x7fffffff) break;
         __syncthreads();
     }
-    const int n = s_end - (int)g;  // partial sums: tail of g, heads of g + 1 .. s_end - 1
+    const int n = s_end - (int)g, gp = 256 / a.lpr, grp = tid / a.lpr;  // partial sums: tail of g, heads of g + 1 .. s_end - 1
     Row<VEC, NV> acc;
     acc.zero();
-    int count = 0;
-    const int per = (n + groups - 1) / groups;
-    const int i0 = grp * per, i1 = i0 + per < n ? i0 + per : n;
-#pragma unroll 4
-    for (int i = i0; i < i1; ++i) {
-        const long long slot = i == 0 ? 2 * g + 1 : 2 * (g + i);
-        Row<VEC, NV> x;
-        x.template load<CRAG_F32>(a.partial, slot, a.dim, lpr, sub, true);
-        acc.add(x);
-        count += a.partial_count[slot];
-    }
-    if (!BWD && sub == 0 && count) atomicAdd(&s_count, count);
-    const int rowlen = lpr * VEC * NV;
-    if (grp > 0) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) part[grp * rowlen + (v * lpr + sub) * VEC + k] = acc.x[v][k];
-    }
-    __syncthreads();
-    if (grp == 0) {
-        for (int o = 1; o < groups && o * per < n; ++o)
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) acc.x[v][k] += part[o * rowlen + (v * lpr + sub) * VEC + k];
-        finish<BWD>(a, seg, acc, s_count, sub);
-    }
+    join_rows<VEC, NV>(a, n, grp, gp, grp, [&](int i) { return i == 0 ? 2 * g + 1 : 2 * (g + i); }, c, (float*)smem, part_count, acc);
+    if (grp == 0) acc.store(a.out, a.out_dtype, seg, c);
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
+struct BwdArgs {
+    const float *grad, *y, *coef;
+    float* dp;
+    int n_bags, dim, normalize;
+    const int* ids;
+    long long n;
+    const long long* offsets;
+    int vocab;
+    int* bag;
+    uint32_t *keys, *perm;
+    uint32_t* hist;
+    int tiles, mask;  // of the first digit
+};
+
 // dp_b = coef_b (g_b - y_b <g_b, y_b>), or coef_b g_b.  One wave per bag.
-__global__ __launch_bounds__(256) void k_embed_dpool(const float* __restrict__ grad, const float* __restrict__ y,
-                                                     const float* __restrict__ coef, int n_bags, int dim, int normalize,
-                                                     float* __restrict__ dp) {
+__device__ __forceinline__ void dpool(const BwdArgs& a, long long b) {
     const int lane = threadIdx.x & 63;
-    const long long b = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (b >= n_bags) return;
-    const float* g = grad + b * dim;
-    const float* yb = y + b * dim;
+    if (b >= a.n_bags) return;
+    const float* g = a.grad + b * a.dim;
+    const float* yb = a.y + b * a.dim;
     double dot = 0.0;
-    if (normalize) {
-        for (int d = lane; d < dim; d += 64) dot += (double)g[d] * (double)yb[d];
+    if (a.normalize) {
+        for (int d = lane; d < a.dim; d += 64) dot += (double)g[d] * (double)yb[d];
         for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
     }
-    const float c = coef[b];
-    for (int d = lane; d < dim; d += 64) {
-        const double v = normalize ? (double)g[d] - (double)yb[d] * dot : (double)g[d];
-        dp[b * dim + d] = (float)(v * (double)c);
+    const double k = (double)a.coef[b];
+    for (int d = lane; d < a.dim; d += 64) {
+        const double v = a.normalize ? (double)g[d] - (double)yb[d] * dot : (double)g[d];
+        a.dp[b * a.dim + d] = (float)(v * k);
     }
 }
-
-// bag[t] of every position (-1 outside every bag); the sort's first keys and payload
-__global__ __launch_bounds__(256) void k_embed_bag_of(const int* __restrict__ ids, long long n, const long long* __restrict__ offsets,
-                                                      int n_bags, int vocab, int* __restrict__ bag, uint32_t* __restrict__ keys,
-                                                      uint32_t* __restrict__ perm) {
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (t >= n) return;
-    int b = last_le(offsets, n_bags, t);
-    if (b >= n_bags) b = -1;
-    bag[t] = b;
-    const int id = ids[t];
-    keys[t] = b >= 0 && id >= 0 && id < vocab ? (uint32_t)id : (uint32_t)vocab;
-    perm[t] = (uint32_t)t;
+// the sort's key of a position: its token, or vocab (behind all tokens) where it has none
+__device__ __forceinline__ uint32_t key_of(const BwdArgs& a, long long t, int bag) {
+    const int id = a.ids[t];
+    return bag >= 0 && id >= 0 && id < a.vocab ? (uint32_t)id : (uint32_t)a.vocab;
+}
+__device__ __forceinline__ int bag_at(const BwdArgs& a, long long t) {
+    const int b = last_le(a.offsets, a.n_bags, t);
+    return b >= a.n_bags ? -1 : b;
 }
 
-// up to SORT_SMALL positions: one workgroup sorts (key, position) in LDS
+// Lanes of a wave whose digit equals this lane's, among `on` lanes
+__device__ __forceinline__ unsigned long long same_digit(uint32_t d, int bits, bool on) {
+    unsigned long long same = __ballot(on);
+    for (int bit = 0; bit < bits; ++bit) {
+        const unsigned long long m = __ballot((d >> bit) & 1u);
+        same &= (d >> bit) & 1u ? m : ~m;
+    }
+    return same;
+}
+
+// Up to SORT_SMALL positions: block 0 makes the keys and sorts (key, position) in LDS, stable, 8 bits a pass; the other blocks
+// do dp.  One launch for all that comes in front of the sums.
 constexpr int SORT_SMALL = 8192;
-__global__ __launch_bounds__(1024) void k_sort_small(uint32_t* __restrict__ keys, uint32_t* __restrict__ perm, int n, int P) {
+__global__ __launch_bounds__(1024) void k_bwd_start_small(BwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    unsigned long long* s = (unsigned long long*)smem;
-    for (int i = threadIdx.x; i < P; i += 1024) s[i] = i < n ? ((unsigned long long)keys[i] << 32) | (uint32_t)i : ~0ull;
-    __syncthreads();
-    for (int k = 2; k <= P; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = threadIdx.x; i < (P >> 1); i += 1024) {
-                const int x = ((i & ~(j - 1)) << 1) | (i & (j - 1)), y = x | j;
-                const bool up = (x & k) == 0;
-                const unsigned long long u = s[x], v = s[y];
-                if ((u > v) == up) {
-                    s[x] = v;
-                    s[y] = u;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    if (blockIdx.x > 0) {
+        dpool(a, (long long)(blockIdx.x - 1) * 16 + wv);
+        return;
+    }
+    const int n = (int)a.n, run = (n + 1023) / 1024 * 64;  // keys per wave
+    uint32_t* cnt = (uint32_t*)smem;  // [16][256]
+    uint32_t* ws = cnt + 16 * 256;    // [4]
+    uint32_t* key[2] = {ws + 4, ws + 4 + 16 * run};
+    uint16_t* pos[2] = {(uint16_t*)(key[1] + 16 * run), (uint16_t*)(key[1] + 16 * run) + 16 * run};
+    if (a.keys) {
+        for (int t = tid; t < n; t += 1024) {
+            const int b = bag_at(a, t);
+            a.bag[t] = b;
+            key[0][t] = key_of(a, t, b);
+            pos[0][t] = (uint16_t)t;
+        }
+        int cur = 0;
+        for (int shift = 0; shift < 32 && (a.vocab >> shift) > 0; shift += 8) {
+            for (int i = tid; i < 16 * 256; i += 1024) cnt[i] = 0;
+            __syncthreads();
+            for (int i = lane; i < run; i += 64) {
+                const int t = wv * run + i;
+                if (t < n) atomicAdd(&cnt[wv * 256 + ((key[cur][t] >> shift) & 255u)], 1u);
+            }
+            __syncthreads();
+            uint32_t tot = 0, inc = 0;
+            if (tid < 256) {
+                for (int w = 0; w < 16; ++w) tot += cnt[w * 256 + tid];
+                inc = tot;
+                for (int o = 1; o < 64; o <<= 1) {
+                    const uint32_t x = __shfl_up(inc, o);
+                    if (lane >= o) inc += x;
+                }
+                if (lane == 63) ws[wv] = inc;
+            }
+            __syncthreads();
+            if (tid < 256) {
+                uint32_t at = inc - tot;
+                for (int w = 0; w < wv; ++w) at += ws[w];
+                for (int w = 0; w < 16; ++w) {
+                    const uint32_t x = cnt[w * 256 + tid];
+                    cnt[w * 256 + tid] = at;
+                    at += x;
                 }
             }
             __syncthreads();
+            volatile uint32_t* next = cnt + wv * 256;
+            for (int i = 0; i < run; i += 64) {
+                const int t = wv * run + i + lane;
+                const bool on = t < n;
+                const uint32_t k = on ? key[cur][t] : 0u;
+                const uint16_t p = on ? pos[cur][t] : (uint16_t)0;
+                const uint32_t d = (k >> shift) & 255u;
+                const unsigned long long same = same_digit(d, 8, on);
+                const uint32_t rank = __popcll(same & ((1ull << lane) - 1ull));
+                uint32_t where = 0;
+                if (on) where = next[d];
+                __builtin_amdgcn_wave_barrier();
+                if (on && rank == 0) next[d] = where + (uint32_t)__popcll(same);
+                __builtin_amdgcn_wave_barrier();
+                if (on) {
+                    key[cur ^ 1][where + rank] = k;
+                    pos[cur ^ 1][where + rank] = p;
+                }
+            }
+            __syncthreads();
+            cur ^= 1;
         }
-    for (int i = threadIdx.x; i < n; i += 1024) {
-        keys[i] = (uint32_t)(s[i] >> 32);
-        perm[i] = (uint32_t)s[i];
+        for (int t = tid; t < n; t += 1024) {
+            a.keys[t] = key[cur][t];
+            a.perm[t] = pos[cur][t];
+        }
+    } else {
+        for (int t = tid; t < n; t += 1024) a.bag[t] = bag_at(a, t);
     }
 }
 
-// Stable least-significant-digit radix sort, 8 bits a pass: counts per tile, prefix per digit, ordered scatter.
-constexpr int SORT_TILE = 4096, SORT_PER = SORT_TILE / 256;
-__global__ __launch_bounds__(256) void k_sort_count(const uint32_t* __restrict__ keys, long long n, int shift, int tiles,
+// More: stable least-significant-digit radix sort with digits of up to SORT_BITS bits -- counts per tile, prefix per digit,
+// ordered scatter.  The first launch makes the keys and counts their first digit; its other blocks do dp.
+constexpr int SORT_BITS = 10, SORT_TILE = 2048, SORT_PER = SORT_TILE / 256;
+__global__ __launch_bounds__(256) void k_bwd_start(BwdArgs a) {
+    __shared__ uint32_t h[1 << SORT_BITS];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x >= a.tiles) {
+        dpool(a, (long long)(blockIdx.x - a.tiles) * 4 + (tid >> 6));
+        return;
+    }
+    for (int d = tid; d <= a.mask; d += 256) h[d] = 0;
+    __syncthreads();
+    const long long t0 = (long long)blockIdx.x * SORT_TILE + tid * SORT_PER;
+    if (t0 < a.n) {
+        int b = last_le(a.offsets, a.n_bags, t0);
+        long long end = b < a.n_bags ? a.offsets[b + 1] : 0;
+#pragma unroll
+        for (int i = 0; i < SORT_PER; ++i) {
+            const long long t = t0 + i;
+            if (t < a.n) {
+                if (b < a.n_bags && t >= end) {
+                    b = last_le(a.offsets, a.n_bags, t);
+                    end = b < a.n_bags ? a.offsets[b + 1] : 0;
+                }
+                const int bag = b < a.n_bags ? b : -1;
+                a.bag[t] = bag;
+                if (a.keys) {
+                    const uint32_t k = key_of(a, t, bag);
+                    a.keys[t] = k;
+                    atomicAdd(&h[k & a.mask], 1u);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (a.keys)
+        for (int d = tid; d <= a.mask; d += 256) a.hist[(long long)d * a.tiles + blockIdx.x] = h[d];
+}
+__global__ __launch_bounds__(256) void k_sort_count(const uint32_t* __restrict__ keys, long long n, int shift, int mask, int tiles,
                                                     uint32_t* __restrict__ hist) {
-    __shared__ uint32_t h[256];
-    h[threadIdx.x] = 0;
+    __shared__ uint32_t h[1 << SORT_BITS];
+    for (int d = threadIdx.x; d <= mask; d += 256) h[d] = 0;
     __syncthreads();
     const long long base = (long long)blockIdx.x * SORT_TILE;
 #pragma unroll
     for (int i = 0; i < SORT_PER; ++i) {
         const long long p = base + i * 256 + threadIdx.x;
-        if (p < n) atomicAdd(&h[(keys[p] >> shift) & 255u], 1u);
+        if (p < n) atomicAdd(&h[(keys[p] >> shift) & mask], 1u);
     }
     __syncthreads();
-    hist[(long long)threadIdx.x * tiles + blockIdx.x] = h[threadIdx.x];
+    for (int d = threadIdx.x; d <= mask; d += 256) hist[(long long)d * tiles + blockIdx.x] = h[d];
 }
 // block d: exclusive prefix of digit d's counts over the tiles, its total behind them
 __global__ __launch_bounds__(256) void k_sort_prefix(uint32_t* __restrict__ hist, int tiles, uint32_t* __restrict__ total) {
@@ -474,14 +741,16 @@ __global__ __launch_bounds__(256) void k_sort_prefix(uint32_t* __restrict__ hist
     }
     if (threadIdx.x == 0) total[blockIdx.x] = run;
 }
+// perm == null: position p holds p
 __global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ perm, long long n,
-                                                      int shift, int tiles, const uint32_t* __restrict__ hist,
+                                                      int shift, int bits, int tiles, const uint32_t* __restrict__ hist,
                                                       const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
                                                       uint32_t* __restrict__ perm_out) {
-    __shared__ uint32_t cnt[4][256];  // per wave: counts of its quarter of the tile, then where its next key of a digit goes
+    __shared__ uint32_t cnt[4][1 << SORT_BITS];  // per wave: counts of its quarter of the tile, then where its next key of a digit goes
     __shared__ uint32_t ws[4];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
+    const int bins = 1 << bits, mask = bins - 1, per = (bins + 255) / 256;
+    for (int d = tid; d < 4 * bins; d += 256) cnt[d >> bits][d & mask] = 0;
     __syncthreads();
     const long long base = (long long)blockIdx.x * SORT_TILE + wv * (SORT_TILE / 4);
     uint32_t k[SORT_PER], v[SORT_PER];
@@ -489,38 +758,41 @@ __global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict
     for (int i = 0; i < SORT_PER; ++i) {
         const long long p = base + i * 64 + lane;
         k[i] = p < n ? keys[p] : 0u;
-        v[i] = p < n ? perm[p] : 0u;
-        if (p < n) atomicAdd(&cnt[wv][(k[i] >> shift) & 255u], 1u);
+        v[i] = p >= n ? 0u : (perm ? perm[p] : (uint32_t)p);
+        if (p < n) atomicAdd(&cnt[wv][(k[i] >> shift) & mask], 1u);
     }
-    // where digit tid starts: all smaller digits, then this digit in the tiles in front
-    const uint32_t tot = total[tid];
-    uint32_t inc = tot;
+    // where each digit starts: all smaller digits, then this digit in the tiles in front; thread tid has digits tid * per ..
+    uint32_t mine = 0;
+    for (int j = 0; j < per; ++j)
+        if (tid * per + j < bins) mine += total[tid * per + j];
+    uint32_t inc = mine;
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t x = __shfl_up(inc, o);
         if (lane >= o) inc += x;
     }
     if (lane == 63) ws[wv] = inc;
     __syncthreads();
-    uint32_t at = inc - tot + hist[(long long)tid * tiles + blockIdx.x];
-    for (int w = 0; w < wv; ++w) at += ws[w];
-    for (int w = 0; w < 4; ++w) {
-        const uint32_t c = cnt[w][tid];
-        cnt[w][tid] = at;
-        at += c;
+    uint32_t start = inc - mine;
+    for (int w = 0; w < wv; ++w) start += ws[w];
+    for (int j = 0; j < per; ++j) {
+        const int d = tid * per + j;
+        if (d < bins) {
+            uint32_t at = start + hist[(long long)d * tiles + blockIdx.x];
+            start += total[d];
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t c = cnt[w][d];
+                cnt[w][d] = at;
+                at += c;
+            }
+        }
     }
     __syncthreads();
     volatile uint32_t* next = cnt[wv];
 #pragma unroll
     for (int i = 0; i < SORT_PER; ++i) {
-        const long long p = base + i * 64 + lane;
-        const bool on = p < n;
-        const uint32_t d = (k[i] >> shift) & 255u;
-        unsigned long long same = __ballot(on);
-#pragma unroll
-        for (int bit = 0; bit < 8; ++bit) {
-            const unsigned long long m = __ballot((d >> bit) & 1u);
-            same &= (d >> bit) & 1u ? m : ~m;
-        }
+        const bool on = base + i * 64 + lane < n;
+        const uint32_t d = (k[i] >> shift) & mask;
+        const unsigned long long same = same_digit(d, bits, on);
         const uint32_t rank = __popcll(same & ((1ull << lane) - 1ull));
         uint32_t where = 0;
         if (on) where = next[d];
@@ -534,63 +806,84 @@ __global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict
     }
 }
 
-// dw_t = <dp_b, E[id_t]>; groups of lpr lanes over shares of the positions, as k_segsum
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over aligned groups of lpr lanes, in all of them: quads, halves of eight and sixteen by moves inside a row of lanes
+__device__ __forceinline__ float add_lanes(float v, int lpr) {
+    v = dpp_add<0xB1>(v);   // xor 1
+    v = dpp_add<0x4E>(v);   // xor 2
+    v = dpp_add<0x141>(v);  // the other four of eight
+    if (lpr >= 16) v = dpp_add<0x140>(v);  // the other eight of sixteen
+    if (lpr >= 32) v += __shfl_xor(v, 16);
+    if (lpr >= 64) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// dw_t = <dp_b, E[id_t]>; groups of lanes over shares of the positions, as in k_segsum
 template <int DT, int VEC, int NV>
 __global__ __launch_bounds__(256) void k_embed_dweights(CragSegArgs a, const void* __restrict__ table, const int* __restrict__ ids,
                                                         float* __restrict__ dw) {
-    constexpr int U = NV * VEC <= 8 ? 8 : 4;
+    constexpr int U = rows_ahead<DT, VEC, NV>();
     const int lane = threadIdx.x & 63;
-    const int lpr = a.lpr, sub = lane & (lpr - 1), first = lane & ~(lpr - 1);
+    const int lpr = a.lpr, first = lane & ~(lpr - 1);
+    Cols c;
+    c.dim = a.dim;
+    c.lpr = lpr;
+    c.sub = lane & (lpr - 1);
+    const int sub = c.sub;
     const long long g = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / lpr) + lane / lpr;
     const long long p0 = g * a.share, p1 = p0 + a.share < a.n ? p0 + a.share : a.n;
+    const Pieces<DT, VEC, NV> pieces(c);
+    const Pieces<CRAG_F32, VEC, NV> dp_pieces(c);
     int cur = -1;
     Row<VEC, NV> d;
     d.zero();
-    for (long long base = p0; base < p0 + a.share; base += lpr) {
+    auto look_up = [&](long long pm, int& id, int& bag) {
+        id = bag = -1;
+        if (pm >= p1) return;
+        const int b = a.bag[pm];
+        id = ids[pm];
+        bag = id >= 0 && id < a.vocab ? b : -1;
+    };
+    int id, bag, id_n, bag_n;
+    look_up(p0 + sub, id, bag);
+    for (long long base = p0; base < p0 + a.share; base += lpr, id = id_n, bag = bag_n) {
         const long long pm = base + sub;
-        int id = -1, bag = -1;
-        if (pm < p1) {
-            bag = a.bag[pm];
-            id = ids[pm];
-            if (bag < 0 || id < 0 || id >= a.vocab) id = -1;
-        }
+        look_up(pm + lpr, id_n, bag_n);  // a round ahead
         float mine = 0.f;
-        const int rounds = a.share < lpr ? a.share : lpr;
+        const int rounds = p0 + a.share - base < lpr ? (int)(p0 + a.share - base) : lpr;
         for (int j = 0; j < rounds; j += U) {
-            Row<VEC, NV> x[U];
+            RawRow<DT, VEC, NV> x[U];
             int bu[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) bu[u] = __shfl(bag, first + j + u);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int id_u = __shfl(id, first + j + u);
-                bu[u] = __shfl(bag, first + j + u);
-                if (id_u < 0) bu[u] = -1;
-                x[u].template load<DT>(table, id_u, a.dim, lpr, sub, id_u >= 0);
+                x[u].load(table, bu[u] >= 0 ? id_u : 0, a.dim, pieces);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (bu[u] >= 0 && bu[u] != cur) {
                     cur = bu[u];
-                    d.template load<CRAG_F32>(a.src, cur, a.dim, lpr, sub, true);
+                    d.template load<CRAG_F32>(a.src, cur, a.dim, dp_pieces);
                 }
                 float s = 0.f;
-                if (bu[u] >= 0) {
 #pragma unroll
-                    for (int n = 0; n < NV; ++n)
+                for (int n = 0; n < NV; ++n) {
+                    float t = 0.f;
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) s = fmaf(x[u].x[n][k], d.x[n][k], s);
+                    for (int k = 0; k < VEC; ++k) t = fmaf(x[u].r[n].get(k), d.x[n][k], t);
+                    s += (n * lpr + sub) * VEC < a.dim ? t : 0.f;  // (behind the row's end: a copy that may hold an infinity)
                 }
-                for (int o = lpr >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
-                if (sub == j + u) mine = s;
+                s = add_lanes(s, lpr);
+                if (sub == j + u) mine = bu[u] >= 0 ? s : 0.f;
             }
         }
         if (pm < p1) dw[pm] = mine;
     }
-}
-
-__global__ __launch_bounds__(256) void k_fill_rows(u32x4_t* __restrict__ out, long long n16, unsigned char* __restrict__ rest, int n_rest) {
-    const long long stride = (long long)gridDim.x * 256;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n16; i += stride) out[i] = (u32x4_t){0, 0, 0, 0};
-    if (blockIdx.x == 0 && (int)threadIdx.x < n_rest) rest[threadIdx.x] = 0;
 }
 
 __global__ __launch_bounds__(256) void k_zero_f32(float* __restrict__ out, long long n) {
@@ -603,14 +896,14 @@ struct Shape {
     int vec, nv, lpr;
 };
 // lanes per row and pieces per lane: the fewest idle lanes, then the most lanes
-Shape row_shape(int dim, int vec) {
-    const int pieces = (dim + vec - 1) / vec;
-    static const int kNv[] = {1, 2, 3, 4, 8, 16, 32};
+Shape row_shape(int width, int vec) {
+    const int pieces = (width + vec - 1) / vec;
+    static const int kNv[] = {1, 2, 3, 4, 5, 6, 8, 16, 32};
     Shape best = {vec, 0, 0};
     int best_held = 0x7fffffff;
-    for (int lpr = 64; lpr >= 8; lpr >>= 1)
+    for (int lpr = 64; lpr >= 8; lpr >>= 1)  // (no fewer: a group looks up eight positions at a time)
         for (int nv : kNv) {
-            if (nv * vec > 32) continue;
+            if (nv * vec > 32 || ((nv == 5 || nv == 6) && vec != 4)) continue;
             if (lpr * nv < pieces) continue;
             if (lpr * nv < best_held) {
                 best_held = lpr * nv;
@@ -621,56 +914,106 @@ Shape row_shape(int dim, int vec) {
         }
     return best;
 }
-int vec_of(int dim, int esz, std::initializer_list<const void*> ptrs) {
-    for (int vec : {esz == 2 ? 8 : 4, 2}) {
-        bool ok = dim % vec == 0;
-        for (const void* p : ptrs) ok = ok && ((uintptr_t)p % (size_t)(vec * esz > 16 ? 16 : vec * esz)) == 0;
-        if (ok) return vec;
-    }
+// the most elements that one load may take: what the row length and the pointer allow, 16 bytes at most
+int vec_of(int dim, int esz, const void* p) {
+    for (int vec = 16 / esz; vec > 1; vec >>= 1)
+        if (dim % vec == 0 && (uintptr_t)p % (size_t)(vec * esz) == 0) return vec;
     return 1;
 }
-// positions a group of lanes walks: shares enough to fill the chip several times over, but not so many that joining the
-// segments that cross their borders weighs against the sums themselves
+// Positions a group of lanes walks: as many groups as the chip holds at once (about twelve waves a CU), at least eight
+// positions each: a segment that crosses a border costs a row written and read again, and a second round of waves that is
+// not full costs half a round (1M tokens of 384 float32: 168 positions a group 120 us, 128 141 us).
 int share_of(long long n, int lpr) {
-    const long long groups = 256ll * 16 * (64 / lpr);
-    int c = 8;
-    while (c < 256 && n / c > groups) c <<= 1;
-    return c;
+    const long long groups = 256ll * 12 * (64 / lpr);
+    return (int)std::max<long long>(8, ((n + groups - 1) / groups + 7) / 8 * 8);
+}
+
+struct Walk {  // how a gather of n rows is cut up
+    Shape sh;
+    int share;
+    long long n_share, blocks;
+};
+Walk plan_walk(long long n, int dim, int dtype, const void* src) {
+    Walk w;
+    w.sh = row_shape(dim, vec_of(dim, dtype == CRAG_F32 ? 4 : 2, src));
+    w.share = share_of(n, w.sh.lpr);
+    w.n_share = (n + w.share - 1) / w.share;
+    const int per_block = 4 * (64 / w.sh.lpr);
+    w.blocks = (w.n_share + per_block - 1) / per_block;
+    return w;
+}
+void apply(CragSegArgs& a, const Walk& w) {
+    a.lpr = w.sh.lpr;
+    a.share = w.share;
+    a.n_share = w.n_share;
 }
 
 #define CRAG_SEG_CASES(X) \
-    X(8, 1) X(8, 2) X(8, 3) X(8, 4) X(4, 1) X(4, 2) X(4, 3) X(4, 4) X(4, 8) X(2, 1) X(2, 2) X(2, 3) X(2, 4) X(2, 8) X(2, 16) \
-    X(1, 1) X(1, 2) X(1, 3) X(1, 4) X(1, 8) X(1, 16) X(1, 32)
+    X(8, 1) X(8, 2) X(8, 3) X(8, 4) X(4, 1) X(4, 2) X(4, 3) X(4, 4) X(4, 5) X(4, 6) X(4, 8) X(2, 1) X(2, 2) X(2, 3) X(2, 4) X(2, 8) \
+    X(2, 16) X(1, 1) X(1, 2) X(1, 3) X(1, 4) X(1, 8) X(1, 16) X(1, 32)
 
 template <int DT, bool BWD>
-int launch_segsum(const CragSegArgs& a, const Shape& sh, hipStream_t s) {
-    const long long blocks = (a.n_share + 4 * (64 / sh.lpr) - 1) / (4 * (64 / sh.lpr));
-    long long empties = 0;
-    if (!BWD) empties = std::min<long long>(512, (a.n_seg + 255) / 256);
-    const size_t lds = sizeof(float) * 256 * sh.vec * sh.nv;
-#define X(V, N)                                                                                                                \
-    if (sh.vec == V && sh.nv == N) {                                                                                           \
-        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                           \
-            if (blocks) hipLaunchKernelGGL((k_segsum<DT, BWD, V, N>), dim3((unsigned)blocks), dim3(256), 0, s, a);              \
-            if (a.n_share + empties)                                                                                           \
-                hipLaunchKernelGGL((k_segjoin<BWD, V, N>), dim3((unsigned)(a.n_share + empties)), dim3(256), lds, s, a);         \
-            return (int)hipGetLastError();                                                                                     \
-        }                                                                                                                      \
+int launch_segsum(CragSegArgs a, const Walk& w, hipStream_t s) {
+    a.sum_blocks = w.blocks;
+    const long long blocks = w.blocks + (BWD ? ((long long)a.vocab + 255) / 256 : 0);
+    if (!blocks) return 0;
+#define X(V, N)                                                                                                     \
+    if (w.sh.vec == V && w.sh.nv == N) {                                                                            \
+        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                \
+            hipLaunchKernelGGL((k_segsum<DT, BWD, V, N>), dim3((unsigned)blocks), dim3(256), 0, s, a);               \
+            return (int)hipGetLastError();                                                                          \
+        }                                                                                                           \
+    }
+    CRAG_SEG_CASES(X)
+#undef X
+    return -1;
+}
+// joins: whole rows of float32, so shapes of their own
+int launch_finish(CragSegArgs a, hipStream_t s) {
+    const Shape sh = row_shape(a.dim, std::min(vec_of(a.dim, 4, nullptr), vec_of(a.dim, a.out_dtype == CRAG_F32 ? 4 : 2, a.out)));
+    a.lpr = sh.lpr;
+    // groups of lanes per bag: one for each dozen partial rows of a bag of average length; for three while CUs are idle
+    const long long rows = a.n_seg > 0 ? a.n / a.share / a.n_seg : 0;
+    int gp = 1;
+    while (gp < 256 / sh.lpr && rows > 3 * gp && (rows > 12 * gp || (long long)a.n_seg * gp < 256 * (256 / sh.lpr))) gp <<= 1;
+    const long long per = 256 / sh.lpr / gp, blocks = (a.n_seg + per - 1) / per;
+    const size_t lds = gp > 1 ? sizeof(float) * 256 * sh.vec * sh.nv : 0;
+#define X(V, N)                                                                                                  \
+    if (sh.vec == V && sh.nv == N) {                                                                             \
+        if constexpr (V != 8) {                                                                                  \
+            hipLaunchKernelGGL((k_embed_finish<V, N>), dim3((unsigned)blocks), dim3(256), lds, s, a, gp);         \
+            return (int)hipGetLastError();                                                                       \
+        }                                                                                                        \
+    }
+    CRAG_SEG_CASES(X)
+#undef X
+    return -1;
+}
+int launch_join(CragSegArgs a, hipStream_t s) {
+    const Shape sh = row_shape(a.dim, std::min(vec_of(a.dim, 4, nullptr), vec_of(a.dim, a.out_dtype == CRAG_F32 ? 4 : 2, a.out)));
+    a.lpr = sh.lpr;
+    a.partial_count = nullptr;
+    if (!a.n_share) return 0;
+#define X(V, N)                                                                                                                          \
+    if (sh.vec == V && sh.nv == N) {                                                                                                     \
+        if constexpr (V != 8) {                                                                                                          \
+            hipLaunchKernelGGL((k_segjoin<V, N>), dim3((unsigned)a.n_share), dim3(256), sizeof(float) * 256 * sh.vec * sh.nv, s, a);      \
+            return (int)hipGetLastError();                                                                                               \
+        }                                                                                                                                \
     }
     CRAG_SEG_CASES(X)
 #undef X
     return -1;
 }
 template <int DT>
-int launch_dweights(const CragSegArgs& a, const Shape& sh, const void* table, const int* ids, float* dw, hipStream_t s) {
-    const long long blocks = (a.n_share + 4 * (64 / sh.lpr) - 1) / (4 * (64 / sh.lpr));
-    if (!blocks) return 0;
-#define X(V, N)                                                                                                            \
-    if (sh.vec == V && sh.nv == N) {                                                                                       \
-        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                       \
-            hipLaunchKernelGGL((k_embed_dweights<DT, V, N>), dim3((unsigned)blocks), dim3(256), 0, s, a, table, ids, dw);   \
-            return (int)hipGetLastError();                                                                                 \
-        }                                                                                                                  \
+int launch_dweights(const CragSegArgs& a, const Walk& w, const void* table, const int* ids, float* dw, hipStream_t s) {
+    if (!w.blocks) return 0;
+#define X(V, N)                                                                                                                 \
+    if (w.sh.vec == V && w.sh.nv == N) {                                                                                        \
+        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                            \
+            hipLaunchKernelGGL((k_embed_dweights<DT, V, N>), dim3((unsigned)w.blocks), dim3(256), 0, s, a, table, ids, dw); \
+            return (int)hipGetLastError();                                                                                      \
+        }                                                                                                                       \
     }
     CRAG_SEG_CASES(X)
 #undef X
@@ -690,42 +1033,43 @@ struct Carve {
 long long most_shares(long long n, int dim) {
     long long most = 1;
     for (int vec : {1, 2, 4, 8}) {
-        const Shape sh = row_shape(dim, vec);
-        const int share = share_of(n, sh.lpr);
+        const int share = share_of(n, row_shape(dim, vec).lpr);
         most = std::max(most, (n + share - 1) / share);
     }
     return most;
 }
 
-struct SegWs {
-    float* partial;
-    int *partial_seg, *partial_count;
+struct FwdWs {
+    float *partial, *sums;
+    int *partial_count, *sums_count;
 };
-SegWs carve_seg(Carve& c, long long n, int dim) {
+FwdWs carve_fwd(Carve& c, long long n, int n_bags, int dim) {
     const size_t slots = 2 * (size_t)most_shares(n, dim);
-    SegWs w;
+    FwdWs w;
     w.partial = (float*)c.take(sizeof(float) * slots * (size_t)dim);
-    w.partial_seg = (int*)c.take(sizeof(int) * slots);
     w.partial_count = (int*)c.take(sizeof(int) * slots);
+    w.sums = (float*)c.take(sizeof(float) * (size_t)n_bags * (size_t)dim);  // (a float32 output holds them itself)
+    w.sums_count = (int*)c.take(sizeof(int) * (size_t)n_bags);
     return w;
 }
 struct BwdWs {
-    SegWs seg;
-    float* dp;
-    int* bag;
+    float *partial, *dp;
+    int *partial_seg, *bag;
     uint32_t *keys[2], *perm[2], *hist, *total;
 };
 BwdWs carve_bwd(Carve& c, long long n, int n_bags, int dim) {
+    const size_t slots = 2 * (size_t)most_shares(n, dim);
     BwdWs w;
-    w.seg = carve_seg(c, n, dim);
+    w.partial = (float*)c.take(sizeof(float) * slots * (size_t)dim);
+    w.partial_seg = (int*)c.take(sizeof(int) * slots);
     w.dp = (float*)c.take(sizeof(float) * (size_t)n_bags * (size_t)dim);
     w.bag = (int*)c.take(sizeof(int) * (size_t)n);
     for (int i = 0; i < 2; ++i) {
         w.keys[i] = (uint32_t*)c.take(sizeof(uint32_t) * (size_t)n);
         w.perm[i] = (uint32_t*)c.take(sizeof(uint32_t) * (size_t)n);
     }
-    w.hist = (uint32_t*)c.take(sizeof(uint32_t) * 256 * (size_t)((n + SORT_TILE - 1) / SORT_TILE));
-    w.total = (uint32_t*)c.take(sizeof(uint32_t) * 256);
+    w.hist = (uint32_t*)c.take(n > SORT_SMALL ? sizeof(uint32_t) * ((size_t)1 << SORT_BITS) * (size_t)((n + SORT_TILE - 1) / SORT_TILE) : 0);
+    w.total = (uint32_t*)c.take(sizeof(uint32_t) << SORT_BITS);
     return w;
 }
 
@@ -734,40 +1078,36 @@ BwdWs carve_bwd(Carve& c, long long n, int n_bags, int dim) {
 size_t crag_embed_ws_bytes(long long n, int n_bags, int dim, bool backward) {
     Carve c{nullptr};
     if (backward) carve_bwd(c, n, n_bags, dim);
-    else carve_seg(c, n, dim);
+    else carve_fwd(c, n, n_bags, dim);
     return c.used;
 }
 
 int crag_launch_embed_forward(const CragEmbedArgs& e, hipStream_t s) {
     Carve c{(char*)e.workspace};
-    const SegWs w = carve_seg(c, e.n, e.dim);
-    const int esz = e.dtype == CRAG_F32 ? 4 : 2;
-    int vec = vec_of(e.dim, esz, {e.table});
-    const int osz = e.out_dtype == CRAG_F32 ? 4 : 2;
-    while (vec > 1 && ((uintptr_t)e.out % (size_t)std::min(16, vec * osz))) vec = vec > 2 ? 2 : 1;
-    const Shape sh = row_shape(e.dim, vec);
+    const FwdWs ws = carve_fwd(c, e.n, e.n_bags, e.dim);
+    const Walk w = plan_walk(e.n, e.dim, e.dtype, e.table);
     CragSegArgs a = {};
+    apply(a, w);
     a.src = e.table;
     a.n = e.n;
     a.n_seg = e.n_bags;
     a.dim = e.dim;
     a.vocab = (int)e.vocab;
-    a.lpr = sh.lpr;
-    a.share = share_of(e.n, sh.lpr);
-    a.n_share = (e.n + a.share - 1) / a.share;
     a.ids = e.ids;
     a.weights = e.weights;
     a.offsets = e.offsets;
-    a.partial = w.partial;
-    a.partial_seg = w.partial_seg;
-    a.partial_count = w.partial_count;
+    a.partial = ws.partial;
+    a.partial_count = ws.partial_count;
+    a.sums = e.out_dtype == CRAG_F32 ? (float*)e.out : ws.sums;
+    a.sums_count = ws.sums_count;
     a.out = e.out;
     a.out_dtype = e.out_dtype;
     a.mode = e.mode;
     a.normalize = e.normalize;
     a.scale = e.scale;
     a.coef = e.coef;
-    return e.dtype == CRAG_F32 ? launch_segsum<CRAG_F32, false>(a, sh, s) : launch_segsum<CRAG_BF16, false>(a, sh, s);
+    const int rc = e.dtype == CRAG_F32 ? launch_segsum<CRAG_F32, false>(a, w, s) : launch_segsum<CRAG_BF16, false>(a, w, s);
+    return rc ? rc : launch_finish(a, s);
 }
 
 int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
@@ -779,14 +1119,26 @@ int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
     if (e.n_bags == 0) {  // every position is outside every bag
         if (e.d_weights && e.n > 0) hipLaunchKernelGGL(k_zero_f32, dim3((unsigned)((e.n + 255) / 256)), dim3(256), 0, s, e.d_weights, e.n);
         e.n = 0;
+        e.d_weights = nullptr;
     }
-    if (e.n_bags > 0)
-        hipLaunchKernelGGL(k_embed_dpool, dim3((unsigned)((e.n_bags + 3) / 4)), dim3(256), 0, s, e.grad, e.y, e.coef, e.n_bags, e.dim,
-                           e.normalize, w.dp);
-    if (e.n > 0)
-        hipLaunchKernelGGL(k_embed_bag_of, dim3((unsigned)((e.n + 255) / 256)), dim3(256), 0, s, e.ids, e.n, e.offsets, e.n_bags,
-                           (int)e.vocab, w.bag, w.keys[0], w.perm[0]);
-    if ((rc = (int)hipGetLastError())) return rc;
+    BwdArgs b = {};
+    b.grad = e.grad;
+    b.y = e.y;
+    b.coef = e.coef;
+    b.dp = w.dp;
+    b.n_bags = e.n_bags;
+    b.dim = e.dim;
+    b.normalize = e.normalize;
+    b.ids = e.ids;
+    b.n = e.n;
+    b.offsets = e.offsets;
+    b.vocab = (int)e.vocab;
+    b.bag = w.bag;
+    b.hist = w.hist;
+    if (e.d_table) {
+        b.keys = w.keys[0];
+        b.perm = w.perm[0];
+    }
     CragSegArgs a = {};
     a.src = w.dp;
     a.n = e.n;
@@ -794,51 +1146,49 @@ int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
     a.vocab = (int)e.vocab;
     a.bag = w.bag;
     a.weights = e.weights;
-    if (e.d_weights && e.n > 0) {
-        const Shape sh = row_shape(e.dim, vec_of(e.dim, esz, {e.table}));
-        a.lpr = sh.lpr;
-        a.share = share_of(e.n, sh.lpr);
-        a.n_share = (e.n + a.share - 1) / a.share;
-        rc = e.dtype == CRAG_F32 ? launch_dweights<CRAG_F32>(a, sh, e.table, e.ids, e.d_weights, s)
-                                 : launch_dweights<CRAG_BF16>(a, sh, e.table, e.ids, e.d_weights, s);
-        if (rc) return rc;
-    }
-    if (!e.d_table) return 0;
-    // rows of tokens that do not occur are zero
-    const size_t bytes = (size_t)e.vocab * (size_t)e.dim * (size_t)esz;
-    const size_t n16 = ((uintptr_t)e.d_table % 16) == 0 ? bytes / 16 : 0;
-    if (n16 == 0 && bytes >= 16) return -3;  // refused by the caller
-    const long long fill_blocks = std::max<long long>(1, std::min<long long>(8192, ((long long)n16 + 255) / 256));
-    hipLaunchKernelGGL(k_fill_rows, dim3((unsigned)fill_blocks), dim3(256), 0, s, (u32x4_t*)e.d_table, (long long)n16,
-                       (unsigned char*)e.d_table + n16 * 16, (int)(bytes - n16 * 16));
-    if ((rc = (int)hipGetLastError())) return rc;
-    if (e.n == 0) return 0;
+    // as soon as dp is there: the caches may still hold the forward pass's rows of the table, which the gradient's rows drive
+    // out (109 us against 150 behind a pass that wrote 400 MB, 1M tokens of 384 elements)
+    auto weights = [&]() -> int {
+        if (!e.d_weights || e.n == 0) return (int)hipGetLastError();
+        const Walk k = plan_walk(e.n, e.dim, e.dtype, e.table);
+        apply(a, k);
+        return e.dtype == CRAG_F32 ? launch_dweights<CRAG_F32>(a, k, e.table, e.ids, e.d_weights, s)
+                                   : launch_dweights<CRAG_BF16>(a, k, e.table, e.ids, e.d_weights, s);
+    };
     int cur = 0;
     if (e.n <= SORT_SMALL) {
-        int P = 2;
-        while (P < e.n) P <<= 1;
-        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(1024), sizeof(unsigned long long) * (size_t)P, s, w.keys[0], w.perm[0], (int)e.n, P);
+        const int run = (int)((e.n + 1023) / 1024 * 64);
+        const size_t lds = sizeof(uint32_t) * (16 * 256 + 4 + 2 * 16 * (size_t)run) + sizeof(uint16_t) * 2 * 16 * (size_t)run;
+        static std::atomic<uint64_t> lds_ok;
+        crag_allow_dynamic_lds((const void*)k_bwd_start_small, sizeof(uint32_t) * (16 * 256 + 4) + 12 * SORT_SMALL, lds_ok);
+        if (e.n > 0) hipLaunchKernelGGL(k_bwd_start_small, dim3(1 + (e.n_bags + 15) / 16), dim3(1024), lds, s, b);
+        if ((rc = weights())) return rc;
     } else {
         const int tiles = (int)((e.n + SORT_TILE - 1) / SORT_TILE);
-        for (int shift = 0; shift < 32 && (e.vocab >> shift) > 0; shift += 8) {
-            hipLaunchKernelGGL(k_sort_count, dim3(tiles), dim3(256), 0, s, w.keys[cur], e.n, shift, tiles, w.hist);
-            hipLaunchKernelGGL(k_sort_prefix, dim3(256), dim3(256), 0, s, w.hist, tiles, w.total);
-            hipLaunchKernelGGL(k_sort_scatter, dim3(tiles), dim3(256), 0, s, w.keys[cur], w.perm[cur], e.n, shift, tiles, w.hist, w.total,
-                               w.keys[cur ^ 1], w.perm[cur ^ 1]);
+        int bits = 1;
+        while (e.vocab >> bits) ++bits;  // of the largest key, vocab itself
+        const int passes = (bits + SORT_BITS - 1) / SORT_BITS, digit = (bits + passes - 1) / passes;
+        b.tiles = tiles;
+        b.mask = (1 << digit) - 1;
+        hipLaunchKernelGGL(k_bwd_start, dim3(tiles + (e.n_bags + 3) / 4), dim3(256), 0, s, b);
+        if ((rc = weights())) return rc;
+        for (int p = 0; e.d_table && p < passes; ++p) {
+            if (p > 0) hipLaunchKernelGGL(k_sort_count, dim3(tiles), dim3(256), 0, s, w.keys[cur], e.n, p * digit, b.mask, tiles, w.hist);
+            hipLaunchKernelGGL(k_sort_prefix, dim3(1 << digit), dim3(256), 0, s, w.hist, tiles, w.total);
+            hipLaunchKernelGGL(k_sort_scatter, dim3(tiles), dim3(256), 0, s, w.keys[cur], p ? w.perm[cur] : (const uint32_t*)nullptr, e.n,
+                               p * digit, digit, tiles, w.hist, w.total, w.keys[cur ^ 1], w.perm[cur ^ 1]);
             cur ^= 1;
         }
     }
-    if ((rc = (int)hipGetLastError())) return rc;
-    const Shape sh = row_shape(e.dim, e.dim % 4 == 0 ? 4 : (e.dim % 2 == 0 ? 2 : 1));  // dp and partials: 256-byte aligned
-    a.lpr = sh.lpr;
-    a.share = share_of(e.n, sh.lpr);
-    a.n_share = (e.n + a.share - 1) / a.share;
+    if ((rc = (int)hipGetLastError()) || !e.d_table) return rc;
+    const Walk k = plan_walk(e.n, e.dim, CRAG_F32, w.dp);
+    apply(a, k);
     a.keys = w.keys[cur];
     a.perm = w.perm[cur];
-    a.partial = w.seg.partial;
-    a.partial_seg = w.seg.partial_seg;
-    a.partial_count = w.seg.partial_count;
+    a.partial = w.partial;
+    a.partial_seg = w.partial_seg;
     a.out = e.d_table;
     a.out_dtype = e.dtype;
-    return launch_segsum<CRAG_F32, true>(a, sh, s);
+    if ((rc = launch_segsum<CRAG_F32, true>(a, k, s))) return rc;
+    return launch_join(a, s);
 }

@@ -235,7 +235,7 @@ int crag_merge_rerank_device(int device, const void* entries_dev, int G, int B, 
  * front of the first or behind the last belong to no bag.  An empty bag gives zeros.
  *   table_dev     [vocab][dim] float32 or bf16, row-major; dim <= 2048
  *   weights_dev   [n_tokens], NULL = ones
- *   out_dev       [n_bags][dim], out_dtype float32 or bf16.  Sums are float32 (norms float64); one rounding at the end
+ *   out_dev       [n_bags][dim], out_dtype float32 or bf16, 16-byte aligned.  Sums are float32 (norms float64); one rounding at the end
  *   coef_dev      [n_bags], may be NULL: what the backward call needs of this one
  * n_tokens < 2^31.  Both calls are asynchronous on `stream`, allocate nothing and may be captured into a graph; everything
  * they need beside the buffers is in the caller's workspace (crag_embed_workspace bytes, 256-byte aligned), which belongs to
