@@ -657,7 +657,11 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     char* desc_dev = merged ? (char*)ws->stage.p : (char*)ws->desc.p;
     const QueryDesc* qd_dev = (const QueryDesc*)desc_dev;
     const GroupDesc* gd_dev = (const GroupDesc*)(desc_dev + sizeof(QueryDesc) * (size_t)B);
-    if (noalloc) {
+    // 4-bit rows, one collection: the launch that splits the queries writes the descriptors (unless they go up with the
+    // host's queries anyway)
+    const bool fp4_desc = fp4 && P.mfma && !merged;
+    if (fp4_desc) {
+    } else if (noalloc) {
         // one collection, so one QueryDesc for all queries and at most B / 8 groups: they travel as kernel arguments
         if ((rc = put_descriptors(qd[0], gd.data(), (int)gd.size(), B, (QueryDesc*)ws->desc.p, (GroupDesc*)gd_dev, st))) return rc;
     } else {
@@ -712,7 +716,8 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         const size_t piece_bytes = (size_t)crag_fp4_query_bytes(n_blocks, h0->dim_pad, narrow);
         if ((rc = ws->qscan.ensure(piece_bytes + sizeof(float) * (size_t)B))) return rc;
         float* res = (float*)((char*)ws->qscan.p + piece_bytes);
-        if (crag_launch_fp4_split(q_dev, P.mfma ? nullptr : gd_dev, n_blocks, B, h0->dim_pad, h0->metric, narrow, ws->qscan.p, res, st))
+        if (crag_launch_fp4_split(q_dev, P.mfma ? nullptr : gd_dev, n_blocks, B, h0->dim_pad, h0->metric, narrow, ws->qscan.p, res,
+                                  fp4_desc ? &qd[0] : nullptr, fp4_desc ? (QueryDesc*)desc_dev : nullptr, st))
             return fail(CRAG_E_HIP, "query split launch failed");
         qres = res;
         fa.queries = ws->qscan.p;
@@ -904,7 +909,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         if (prof) HIPCHK(hipEventRecord(ws->ev[3], st));
         for (const auto& g : gd) prof_rows += (double)(g.n_rows - g.from[2]);
     }
-    FinalizeArgs f;
+    FinalizeArgs f = {};
     f.qd = qd_dev;
     f.queries = q_dev;
     f.B = B;
@@ -939,14 +944,20 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     f.seg_cap = seg_cap;
     f.cand_stride = cand_stride;
     f.qres = qres;
+    f.out_ids = mo ? mo->ids : nullptr;
+    f.out_scores = mo ? mo->scores : nullptr;
+    f.out_dist = mo ? mo->dist : nullptr;
+    f.out_counts = mo ? mo->counts : nullptr;
+    f.top_k = top_k;
+    f.symbol_boost = mo ? mo->symbol_boost : 0.0;
     f.qmap = nullptr;
     if ((rc = crag_launch_finalize(f, st))) return fail(CRAG_E_HIP, "finalize launch failed");
+    f.out_ids = nullptr;  // the fallback tiers patch entries; the rerank then runs once more, over all of them
     auto merge = [&]() -> int {
         if (!mo) return 0;
         return crag_launch_merge_rerank(entries_dev, 1, B, P.kc, top_k, mo->symbol_boost, mo->ids, mo->scores, mo->dist,
                                         mo->counts, st);
     };
-    if (merge()) return fail(CRAG_E_HIP, "merge_rerank launch failed");
     bool patched = false;
 
     // ---- verify: every query must carry an exactness certificate ----
@@ -1744,7 +1755,8 @@ int crag_debug_dense_scores(crag_index* h, const void* queries_dev, int B, int p
         const int n_blocks = crag_fp4_query_blocks(B, h->dim_pad);
         const size_t piece_bytes = (size_t)crag_fp4_query_bytes(n_blocks, h->dim_pad, narrow);
         if ((rc = ws->qscan.ensure(piece_bytes + sizeof(float) * (size_t)B))) return rc;
-        if (crag_launch_fp4_split(q, nullptr, n_blocks, B, h->dim_pad, h->metric, narrow, ws->qscan.p, (float*)((char*)ws->qscan.p + piece_bytes), st))
+        if (crag_launch_fp4_split(q, nullptr, n_blocks, B, h->dim_pad, h->metric, narrow, ws->qscan.p, (float*)((char*)ws->qscan.p + piece_bytes),
+                                  nullptr, nullptr, st))
             return fail(CRAG_E_HIP, "query split launch failed");
         Fp4Args a = {};
         a.queries = ws->qscan.p;

@@ -201,6 +201,13 @@ struct FinalizeArgs {
     int n_seg, seg_cap;
     long long cand_stride;            // slots per query in cand (CRAG_CAND_CAP when flat)
     const float* qres;                // 4-bit rows: norm of what the scan's pieces leave of each query; null elsewhere
+    // one shard only, may be null: the rerank of k_merge_rerank in the same launch, results at these places
+    long long* out_ids;
+    double* out_scores;
+    float* out_dist;
+    int* out_counts;
+    int top_k;
+    double symbol_boost;
     const int* qmap;                  // null: block b serves query b; else block b serves query qmap[b] (fallback passes)
 };
 int crag_launch_finalize(const FinalizeArgs& a, hipStream_t s);
@@ -261,9 +268,9 @@ struct Fp4Args {
 int crag_fp4_dim_pad(int dim);  // 0: too long
 int crag_fp4_query_blocks(int B, int dim_pad);
 long long crag_fp4_query_bytes(int n_blocks, int dim_pad, bool narrow);
-// residual[q]: norm of what the pieces of query q leave over
+// residual[q]: norm of what the pieces of query q leave over; desc: written to desc_out[0 .. B) as well (both may be null)
 int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_blocks, int B, int dim_pad, int metric, bool narrow, void* out,
-                          float* residual, hipStream_t s);
+                          float* residual, const QueryDesc* desc, QueryDesc* desc_out, hipStream_t s);
 int crag_fp4_segments(int B, int dim_pad, int n_cus);
 int crag_launch_scan_fp4(const Fp4Args& a, int dim_pad, bool filter, int n_cus, hipStream_t s);
 int crag_launch_scan_fp4_groups(const Fp4Args& a, int dim_pad, int blocks, hipStream_t s);

@@ -393,70 +393,83 @@ __device__ __forceinline__ float e2m3(float t, uint32_t* code) {
     return t < 0.f ? -r : r;
 }
 
-// One wave per query slot; lane l splits group l (dim_pad / 32 <= 64 groups).  Wide: slot = query, 32 to a block.  Narrow:
-// 16 slots to a block; with `groups`, block g holds the queries of group g.
-__global__ __launch_bounds__(64) void k_fp4_split(const float* __restrict__ queries, const GroupDesc* __restrict__ groups, int n_queries,
-                                                  int dim_pad, int metric, int narrow, unsigned char* __restrict__ out, float* __restrict__ residual) {
+// One block per query slot, eight lanes per group of 32 elements, four elements each.  Wide: slot = query, 32 to a block of the
+// operand.  Narrow: 16 slots to a block; with `groups`, block g holds the queries of group g.
+// `desc_out` (may be null): the batch's descriptors, all equal, written by this launch -- the first one that a search makes --
+// rather than by a copy of its own.
+__global__ __launch_bounds__(512) void k_fp4_split(const float* __restrict__ queries, const GroupDesc* __restrict__ groups, int n_queries,
+                                                   int dim_pad, int metric, int narrow, unsigned char* __restrict__ out, float* __restrict__ residual,
+                                                   QueryDesc desc, QueryDesc* __restrict__ desc_out) {
+    __shared__ double wsum[8];
     const int per = narrow ? 16 : 32, pieces = narrow ? 1 : 2;
-    const int blk = blockIdx.x / per, col = blockIdx.x % per, lane = threadIdx.x;
+    const int blk = blockIdx.x / per, col = blockIdx.x % per, tid = threadIdx.x, lane = tid & 63;
     int q;
     if (groups) q = col < groups[blk].nq ? groups[blk].q_first + col : -1;
     else q = (int)blockIdx.x < n_queries ? (int)blockIdx.x : -1;
-    const int ks = dim_pad >> 6, n_grp = dim_pad >> 5;
+    if (desc_out && q >= 0 && tid == 0) desc_out[q] = desc;
+    const int ks = dim_pad >> 6;
     unsigned char* base = out + blk * crag_fp4_qblock_bytes(ks, pieces);
     double left = 0.0;
-    if (lane < n_grp) {
-        float v[32];
-        bool finite = true;
+    if (tid * 4 < dim_pad) {  // whole groups of eight lanes
+        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+        if (q >= 0) v = -*(const f32x4_t*)(queries + (long long)q * dim_pad + tid * 4);
+        const int grp = tid >> 3, part = tid & 7, k = grp >> 1, half = (grp & 1) * 32;
         float big = 0.f;
+        int huge = 0;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-            if (q >= 0) x = *(const f32x4_t*)(queries + (long long)q * dim_pad + lane * 32 + j);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[j + k] = -x[k];
-                finite = finite && fabsf(x[k]) <= 1.329227995784916e36f;  // 2^120: beyond it nothing is split, and everything left over
-                big = fmaxf(big, fabsf(x[k]));
-            }
+        for (int j = 0; j < 4; ++j) {
+            huge |= fabsf(v[j]) <= 1.329227995784916e36f ? 0 : 1;  // 2^120: beyond it nothing is split, and everything left over
+            big = fmaxf(big, fabsf(v[j]));
         }
-        const int k = lane >> 1, half = (lane & 1) * 32;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) {
+                big = fmaxf(big, __shfl_xor(big, o));
+                huge |= __shfl_xor(huge, o);
+            }
             int ex;
             const float m = frexpf(big, &ex);
             int e = ex - (m > 0.9375f ? 2 : 3);  // the smallest with big <= 7.5 * 2^e
-            e = e < -120 || !finite ? -120 : e;
+            e = e < -120 || huge ? -120 : e;
             const float down = ldexpf(1.f, -e), up = ldexpf(1.f, e);
-            uint32_t w[6] = {0, 0, 0, 0, 0, 0};
+            uint32_t w = 0;  // 24 bits: this lane's four codes
             float rest = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 uint32_t c = 0;
-                if (finite) {
+                if (!huge) {
                     const float r = e2m3(v[j] * down, &c);
                     v[j] -= r * up;
                     rest = fmaxf(rest, fabsf(v[j]));
                 }
-                const int bit = 6 * j;
-                w[bit >> 5] |= c << (bit & 31);
-                if ((bit & 31) > 26) w[(bit >> 5) + 1] |= c >> (32 - (bit & 31));
+                w |= c << (6 * j);
             }
             big = rest;
+            // four lanes' 24 bits are three words
+            const uint32_t w1 = __shfl_down(w, 1, 8), w2 = __shfl_down(w, 2, 8), w3 = __shfl_down(w, 3, 8);
             const int i = narrow ? k : 2 * k + p, at = half + (narrow ? 16 * p + col : col);
-            u32x2_t* o = (u32x2_t*)(base + ((long long)i * 64 + at) * 24);
-            o[0] = (u32x2_t){w[0], w[1]};
-            o[1] = (u32x2_t){w[2], w[3]};
-            o[2] = (u32x2_t){w[4], w[5]};
+            if ((part & 3) == 0) {
+                uint32_t* o = (uint32_t*)(base + ((long long)i * 64 + at) * 24 + (part >> 2) * 12);
+                o[0] = w | (w1 << 24);
+                o[1] = (w1 >> 8) | (w2 << 16);
+                o[2] = (w2 >> 16) | (w3 << 8);
+            }
             // -2q is -q with a scale twice as large
-            base[64ll * 24 * ks * pieces + (long long)at * 4 * crag_fp4_qsw(ks, pieces) + i] = (unsigned char)(e + 127 + (metric == CRAG_L2 ? 1 : 0));
+            if (part == 0)
+                base[64ll * 24 * ks * pieces + (long long)at * 4 * crag_fp4_qsw(ks, pieces) + i] = (unsigned char)(e + 127 + (metric == CRAG_L2 ? 1 : 0));
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) left += (double)v[j] * (double)v[j];
+        for (int j = 0; j < 4; ++j) left += (double)v[j] * (double)v[j];
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) left += __shfl_xor(left, o);
-    if (lane == 0 && q >= 0) residual[q] = nextafterf((float)sqrt(left), __builtin_inff());
+    if (lane == 0) wsum[tid >> 6] = left;
+    __syncthreads();
+    if (tid == 0 && q >= 0) {
+        for (int w = 1; w < (int)(blockDim.x >> 6); ++w) left += wsum[w];
+        residual[q] = nextafterf((float)sqrt(left), __builtin_inff());
+    }
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------------
@@ -631,9 +644,10 @@ int crag_fp4_query_blocks(int B, int dim_pad) {
 long long crag_fp4_query_bytes(int n_blocks, int dim_pad, bool narrow) { return n_blocks * crag_fp4_qblock_bytes(dim_pad >> 6, narrow ? 1 : 2); }
 
 int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_blocks, int B, int dim_pad, int metric, bool narrow, void* out,
-                          float* residual, hipStream_t s) {
-    hipLaunchKernelGGL(k_fp4_split, dim3((unsigned)n_blocks * (narrow ? 16u : 32u)), dim3(64), 0, s, (const float*)queries, groups, B, dim_pad, metric,
-                       narrow ? 1 : 0, (unsigned char*)out, residual);
+                          float* residual, const QueryDesc* desc, QueryDesc* desc_out, hipStream_t s) {
+    const unsigned threads = (unsigned)((dim_pad / 4 + 63) / 64 * 64);
+    hipLaunchKernelGGL(k_fp4_split, dim3((unsigned)n_blocks * (narrow ? 16u : 32u)), dim3(threads), 0, s, (const float*)queries, groups, B, dim_pad,
+                       metric, narrow ? 1 : 0, (unsigned char*)out, residual, desc ? *desc : QueryDesc{}, desc_out);
     return (int)hipGetLastError();
 }
 

@@ -265,9 +265,17 @@ __global__ __launch_bounds__(1024) void k_kth(KthArgs a) {
         }
         return;                                                    // from_cand: keep the looser tau
     }
-    for (int i = tid; i < (int)n; i += 1024) {
-        const int e = seg ? seg_slot(scratch, a.n_seg, a.seg_cap, i) : i;
-        keys[i] = src_at(e);
+    // four loads in flight per thread: one after the other they would cost a trip to memory each
+    for (int i0 = tid; i0 < (int)n; i0 += 4 * 1024) {
+        uint32_t k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * 1024;
+            if (i < (int)n) k[u] = src_at(seg ? seg_slot(scratch, a.n_seg, a.seg_cap, i) : i);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + u * 1024 < (int)n) keys[i0 + u * 1024] = k[u];
     }
     __syncthreads();
     const uint32_t t = block_select([&](int i) { return keys[i]; }, (int)n, (uint32_t)a.M - 1u, scratch);
@@ -394,6 +402,15 @@ __device__ __forceinline__ double combine8(double acc) {
     return acc;
 }
 
+// hybrid_search.py:82,99-121: base score of a distance, times the path's and the symbol's factor
+__device__ __forceinline__ double rerank_score(float dist, uint32_t f, double symbol_boost) {
+    const double base = __ddiv_rn(1.0, __dadd_rn(1.0, (double)dist));
+    const uint32_t cls = f & CRAG_FLAG_CLASS_MASK;
+    double boost = cls == 1u ? 0.1 : (cls == 2u ? 1.2 : 1.0);
+    if (f & CRAG_FLAG_SYMBOL) boost = __dmul_rn(boost, symbol_boost);
+    return __dmul_rn(base, boost);
+}
+
 constexpr int FIN_GATHER = 2048;  // candidates that survive the selection cut (m + 1 plus score ties), else sort all
 __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -509,6 +526,14 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             o[i] = e;
         }
         if (tid == 0) a.status[q] = CRAG_ST_OK;
+        if (a.out_ids) {
+            for (int j = tid; j < a.top_k; j += blockDim.x) {
+                a.out_ids[(long long)q * a.top_k + j] = -1;
+                a.out_scores[(long long)q * a.top_k + j] = 0.0;
+                a.out_dist[(long long)q * a.top_k + j] = __builtin_inff();
+            }
+            if (tid == 0) a.out_counts[q] = 0;
+        }
         return;
     }
 
@@ -569,7 +594,12 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     // rank the m exact keys by counting (keys are unique: the row id is part of the key)
     const int kc_valid = m < a.kc ? m : a.kc;
     CragEntry* out = a.entries + (long long)q * a.kc;
-    __shared__ unsigned int kth_bits;
+    __shared__ unsigned int kth_bits, n_keep;
+    // the rerank's arrays (a.out_ids != null), behind the keys that stay live: row, score and distance by rank
+    uint32_t* rr_row = (uint32_t*)(skeys + 1024);      // [CRAG_MAX_KC]
+    float* rr_dist = (float*)(rr_row + CRAG_MAX_KC);   // [CRAG_MAX_KC]
+    double* rr_score = (double*)(rr_dist + CRAG_MAX_KC);  // [CRAG_MAX_KC], negative: not kept
+    if (tid == 0) n_keep = 0;
     for (int i = tid; i < m; i += blockDim.x) {
         const unsigned long long k = ekeys[i];
         int rank = 0;
@@ -599,6 +629,12 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             e.id = D.id_base + (long long)row;
             out[rank] = e;
             if (rank == kc_valid - 1) kth_bits = (uint32_t)(k >> 32);
+            if (a.out_ids) {
+                const double s = rerank_score(e.dist, flags, a.symbol_boost);
+                rr_row[rank] = row;
+                rr_dist[rank] = e.dist;
+                rr_score[rank] = s > 0.01 ? s : -1.0;
+            }
         }
     }
     for (int i = kc_valid + tid; i < a.kc; i += blockDim.x) {
@@ -644,6 +680,29 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         }
         a.status[q] = status;
     }
+    if (!a.out_ids) return;
+    // R5 (hybrid_search.py:120-125) of a single shard, whose entries are in order already: strict > 0.01 filter, stable
+    // descending sort by counting, top_k
+    for (int j = tid; j < kc_valid; j += blockDim.x) {
+        const double s = rr_score[j];
+        if (s < 0.0) continue;
+        int rank = 0;
+        for (int t = 0; t < kc_valid; ++t) rank += rr_score[t] > s || (rr_score[t] == s && t < j);
+        atomicAdd(&n_keep, 1u);
+        if (rank < a.top_k) {
+            a.out_ids[(long long)q * a.top_k + rank] = D.id_base + (long long)rr_row[j];
+            a.out_scores[(long long)q * a.top_k + rank] = s;
+            a.out_dist[(long long)q * a.top_k + rank] = rr_dist[j];
+        }
+    }
+    __syncthreads();
+    const int nk = (int)n_keep < a.top_k ? (int)n_keep : a.top_k;
+    for (int j = nk + tid; j < a.top_k; j += blockDim.x) {
+        a.out_ids[(long long)q * a.top_k + j] = -1;
+        a.out_scores[(long long)q * a.top_k + j] = 0.0;
+        a.out_dist[(long long)q * a.top_k + j] = __builtin_inff();
+    }
+    if (tid == 0) a.out_counts[q] = nk;
 }
 
 // ----------------------------------------------------------------------------------------
@@ -697,13 +756,7 @@ __global__ __launch_bounds__(256) void k_merge_rerank(const CragEntry* __restric
     // R1..R4: hybrid_search.py:82,99-121
     for (int j = tid; j < nv; j += blockDim.x) {
         const int i = sel[j];
-        const double dist = (double)crag_fkey_inv(fk[i]);
-        const double base = __ddiv_rn(1.0, __dadd_rn(1.0, dist));
-        const uint32_t f = fl[i];
-        const uint32_t cls = f & CRAG_FLAG_CLASS_MASK;
-        double boost = cls == 1u ? 0.1 : (cls == 2u ? 1.2 : 1.0);
-        if (f & CRAG_FLAG_SYMBOL) boost = __dmul_rn(boost, symbol_boost);
-        const double s = __dmul_rn(base, boost);
+        const double s = rerank_score(crag_fkey_inv(fk[i]), fl[i], symbol_boost);
         score[j] = s;
         keep[j] = s > 0.01;
     }
