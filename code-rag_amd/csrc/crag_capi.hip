@@ -395,14 +395,16 @@ long long level1_rows(long long N, long long n0, int M, double direct_max) {
 // longer last level and its looser threshold); at top-100 (M = 225) r ~ 3 is 1.5-2 % ahead of r ~ 6 and of r ~ 2.
 constexpr int CRAG_MAX_LEVELS = 8;
 typedef SmallVec<long long, CRAG_MAX_LEVELS> LevelBounds;
-LevelBounds cascade_bounds(long long N, long long n0, int M) {
+LevelBounds cascade_bounds(long long N, long long n0, int M, bool fp4 = false) {
     LevelBounds nb;
     if (N <= n0) return nb;
     const double R = (double)N / (double)n0;
     constexpr int L_MAX = CRAG_MAX_LEVELS;
     static const double r_small = [] { const char* e = getenv("CRAG_CASCADE_R10"); return e && atof(e) > 1.1 ? atof(e) : 6.0; }();
     static const double r_large = [] { const char* e = getenv("CRAG_CASCADE_R100"); return e && atof(e) > 1.1 ? atof(e) : 3.0; }();
-    int L = (int)std::ceil(std::log(R) / std::log(M > 64 ? r_large : r_small));  // (the two variables: same-box sweeps only)
+    // 4-bit rows are read four times as fast, so a level weighs more against its survivors (same box: 256 queries x 1M x 768,
+    // top 10: r = 4 / 6 / 12 318 / 300 / 289 us; 1024 x 300k x 1024, top 100: r = 2.5 / 3.7 808 / 775 us)
+    int L = (int)std::ceil(std::log(R) / std::log(fp4 ? (M > 128 ? 3.7 : 12.0) : M > 64 ? r_large : r_small));  // (the two variables: same-box sweeps only)
     L = std::max(1, std::min(L, L_MAX));
     auto est = [&](int l) { return (double)l * (double)M * std::pow(R, 1.0 / l); };
     while (L < L_MAX && est(L) > 0.75 * CRAG_CAND_CAP && est(L + 1) < est(L)) ++L;
@@ -595,8 +597,9 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         d.name_hash = (const unsigned long long*)h->name_hash;
         d.path_class = h->path_class;
         d.n_rows = h->n_rows;
-        d.n_sample = level0_rows(h->n_rows, P.M);
-        d.n_mid = level1_rows(h->n_rows, d.n_sample, P.M, P.mfma ? CRAG_CAND_CAP / 8 : std::max(32.0, 2048.0 / B));
+        d.n_sample = level0_rows(h->n_rows, fp4 ? 0 : P.M);
+        // (4-bit rows: a level costs more than the survivors it saves; 64 collections x 20k rows 146 -> 130 us without level 1)
+        d.n_mid = level1_rows(h->n_rows, d.n_sample, P.M, P.mfma || fp4 ? CRAG_CAND_CAP / 8 : std::max(32.0, 2048.0 / B));
         d.id_base = h->id_base;
         d.max_xnorm = h->max_xnorm;
         // keep the level-1 candidates and let the full scan start at n_mid when both levels fit the buffer
@@ -826,7 +829,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         k.seed_stride = cand_stride;
         if (crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         // filter levels [n0, n1), [n1, n2), ..., [.., N): each tightens tau from everything found so far
-        const LevelBounds nb = cascade_bounds(N, n0, P.M);
+        const LevelBounds nb = cascade_bounds(N, n0, P.M, fp4);
         long long from = n0;
         if (nb.empty() && prof) {
             HIPCHK(hipEventRecord(ws->ev[1], st));

@@ -40,9 +40,14 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 template <int CK>
 struct Codes {
     u32x4_t c[CK];
+    template <bool STREAM>
     __device__ __forceinline__ void load(const GLOBAL_AS unsigned char* tile, int step, int lane) {
 #pragma unroll
-        for (int k = 0; k < CK; ++k) c[k] = *(const GLOBAL_AS u32x4_t*)(tile + ((step + k) * 64 + lane) * 16);
+        for (int k = 0; k < CK; ++k) {
+            const GLOBAL_AS u32x4_t* p = (const GLOBAL_AS u32x4_t*)(tile + ((step + k) * 64 + lane) * 16);
+            if constexpr (STREAM) c[k] = __builtin_nontemporal_load(p);
+            else c[k] = *p;
+        }
     }
 };
 template <int KS>
@@ -163,7 +168,7 @@ __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, lon
             if (start) xn[r] = *(const GLOBAL_AS f32x4_t*)(xnorm + t * 32 + 8 * r + (lane >> 5) * 4);
         }
     };
-    cur.load(tile, 0, lane);
+    cur.template load<P == 1>(tile, 0, lane);  // one reader: past the caches
     rs.load(tile, lane);
     load_norms(first);
     for (long long t = first; t < last; t += step) {
@@ -180,8 +185,8 @@ __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, lon
         static_for<NCH>([&](auto cc) {
             constexpr int c = cc;
             Codes<CK> next;
-            if constexpr (c + 1 < NCH) next.load(tile, (c + 1) * CK, lane);
-            else next.load(tile_n, 0, lane);
+            if constexpr (c + 1 < NCH) next.template load<P == 1>(tile, (c + 1) * CK, lane);
+            else next.template load<P == 1>(tile_n, 0, lane);
             products<KS, P, QB, c * CK, CK>(cur, rs, q, acc);
             cur = next;
         });
@@ -668,6 +673,7 @@ int crag_launch_scan_fp4(const Fp4Args& args, int dim_pad, bool filter, int n_cu
     const int ks = dim_pad >> 6, B = a.n_queries;
     const long long tiles = ((a.row_end + 31) >> 5) - (a.row_begin >> 5);
     if (B <= CRAG_FP4_GROUP_Q) {
+        // (two workgroups a CU: one leaves a quarter of the bandwidth, three and more are 5-10 % behind, 4M x 384)
         const int blocks = (int)std::min<long long>((tiles + 3) / 4, 2ll * n_cus);
 #define X(K) \
     case K: return launch_narrow<K>(a, blocks, filter, s);

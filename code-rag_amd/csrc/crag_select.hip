@@ -349,47 +349,58 @@ __device__ __forceinline__ double canon_lane(const void* row, const void* q, int
                              : canon_lane_t<CRAG_BF16>(row, q, dim, j, metric, row_off);
 }
 
-// The same partial sum of a 4-bit row in the tiles of crag_fp4.h, q in LDS or in global memory: of a group's four words of
-// eight codes, lane j takes code j of each.  The eight lanes of a row read the same 16 bytes (one request), eight groups
-// ahead of their use; nothing of the row is staged, because every element is used once.
-template <typename QPtr>
-__device__ __forceinline__ double canon_lane_fp4(const void* rows_, QPtr q, int dim, int dim_pad, long long row, int j, int metric) {
+// The same partial sum of a 4-bit row in the tiles of crag_fp4.h (q: float32 or float64, in LDS or in global memory): of a
+// group's four words of eight codes, lane j takes code j of each.  The eight lanes of a row read the same 16 bytes (one
+// request), eight groups at a time, the next eight on their way while these are added; nothing of the row is staged, because
+// every element is used once.
+struct Fp4Batch {
     typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
-    typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-    const __attribute__((address_space(1))) unsigned char* rows = (const __attribute__((address_space(1))) unsigned char*)rows_;
-    double acc = 0.0;
-    for (int g0 = 0; g0 * 32 < dim; g0 += 8) {
-        u32x4_t c[8];
-        uint32_t s[8];
+    u32x4_t c[8];   // groups 8 b .. 8 b + 7
+    uint32_t s[2];  // scale bytes of the even ones and of the odd ones
+    __device__ __forceinline__ void load(const __attribute__((address_space(1))) unsigned char* tile, int ks, int row, int b) {
+        const __attribute__((address_space(1))) unsigned char* sc = tile + 1024 * ks + (long long)row * 4 * crag_fp4_sw(ks) + b * 4;
+        s[0] = *(const __attribute__((address_space(1))) uint32_t*)sc;
+        s[1] = *(const __attribute__((address_space(1))) uint32_t*)(sc + 128 * crag_fp4_sw(ks));
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            if ((g0 + u) * 32 < dim) {
-                long long at, sc;
-                crag_fp4_place(dim_pad, row, g0 + u, &at, &sc);
-                c[u] = *(const __attribute__((address_space(1))) u32x4_t*)(rows + at);
-                s[u] = rows[sc];
-            }
+            const int k = b * 4 + (u >> 1);  // rows of two or six steps end inside a batch: their last step again, never used
+            c[u] = *(const __attribute__((address_space(1))) u32x4_t*)(tile + ((k < ks ? k : ks - 1) * 64 + (u & 1) * 32 + row) * 16);
         }
+    }
+};
+template <typename Q>
+__device__ __forceinline__ double canon_lane_fp4(const void* rows, const Q* q, int dim, int dim_pad, long long row, int j, int metric) {
+    typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+    const int ks = dim_pad >> 6, r = (int)(row & 31), n = (dim + 255) / 256;
+    const __attribute__((address_space(1))) unsigned char* tile =
+        (const __attribute__((address_space(1))) unsigned char*)rows + (row >> 5) * crag_fp4_tile_bytes(ks);
+    double acc = 0.0;
+    Fp4Batch cur;
+    cur.load(tile, ks, r, 0);
+    for (int b = 0; b < n; ++b) {
+        Fp4Batch next;
+        next.load(tile, ks, r, b + 1 < n ? b + 1 : b);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float scale = crag_fp4_scale(s[u]);
+            const float scale = crag_fp4_scale((cur.s[u & 1] >> (8 * (u >> 1))) & 255u);
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const int d = (g0 + u) * 32 + 8 * v + j;
+                const int d = b * 256 + u * 32 + 8 * v + j;
                 if (d < dim) {
-                    const f32x2_t two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u][v] >> (4 * j), scale, 0);  // exact
-                    const double a = (double)q[d], b = (double)two.x;
+                    const f32x2_t two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cur.c[u][v] >> (4 * j), scale, 0);  // exact
+                    const double a = (double)q[d], x = (double)two.x;
                     double p;
                     if (metric == CRAG_L2) {
-                        const double t = __dsub_rn(a, b);
+                        const double t = __dsub_rn(a, x);
                         p = __dmul_rn(t, t);
                     } else {
-                        p = __dmul_rn(a, b);
+                        p = __dmul_rn(a, x);
                     }
                     acc = __dadd_rn(acc, p);
                 }
             }
         }
+        cur = next;
     }
     return acc;
 }
@@ -401,6 +412,22 @@ __device__ __forceinline__ double combine8(double acc) {
     acc = __dadd_rn(acc, __shfl_xor(acc, 4));
     return acc;
 }
+
+// How many of n items come before one, counted by the lanes that share it (`lanes` of them, a power of two, neighbours; `part`
+// is this lane's number among them): eight LDS reads in flight per lane, and the lanes' counts are added.
+template <typename Before>
+__device__ __forceinline__ int count_before(int n, int part, int lanes, Before before) {
+    int r = 0, t = part;
+    for (; t + 7 * lanes < n; t += 8 * lanes) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) r += before(t + u * lanes) ? 1 : 0;
+    }
+    for (; t < n; t += lanes) r += before(t) ? 1 : 0;
+    for (int o = 1; o < lanes; o <<= 1) r += __shfl_xor(r, o);
+    return r;
+}
+// lanes per item so that a block of 1024 threads has all of them at work on n items
+__device__ __forceinline__ int lanes_per_item(int n) { return n <= 64 ? 16 : (n <= 128 ? 8 : (n <= 256 ? 4 : (n <= 512 ? 2 : 1))); }
 
 // hybrid_search.py:82,99-121: base score of a distance, times the path's and the symbol's factor
 __device__ __forceinline__ double rerank_score(float dist, uint32_t f, double symbol_boost) {
@@ -474,16 +501,17 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     }
     __syncthreads();
     if (c_sorted <= 1024) {
-        // rank by counting (keys are unique: the row id is part of the key): every thread reads the same LDS
-        // word at a time (broadcast), two barriers in all -- a bitonic network of this size costs 21-55
+        // rank by counting (keys are unique: the row id is part of the key): the lanes read the same few LDS
+        // words at a time, two barriers in all -- a bitonic network of this size costs 21-55
+        const int lanes = lanes_per_item(c_sorted), i = tid / lanes, part = tid % lanes;  // c_sorted * lanes <= 1024
         unsigned long long k = ~0ull;
         int rank = 0;
-        if (tid < c_sorted) {
-            k = skeys[tid];
-            for (int j = 0; j < c_sorted; ++j) rank += skeys[j] < k ? 1 : 0;
+        if (i < c_sorted) {
+            k = skeys[i];
+            rank = count_before(c_sorted, part, lanes, [&](int j) { return skeys[j] < k; });
         }
         __syncthreads();
-        if (tid < c_sorted) skeys[rank] = k;
+        if (i < c_sorted && part == 0) skeys[rank] = k;
         __syncthreads();
     } else {
         int P = 2048;
@@ -542,12 +570,16 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     // 128-KiB region is free now), so the order-defining add chains read LDS instead of chasing 2-byte loads
     {
         unsigned char* stage_q = (unsigned char*)(skeys + 1024);  // m + 1 <= CRAG_MAX_M + 1 <= 1024 keys stay live
-        const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;  // (of 4-bit rows only the query is staged)
-        const int q_bytes = row_bytes > 4096 ? row_bytes : 4096;
+        const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;
+        const int q_bytes = a.dtype == CRAG_FP4 ? a.dim_pad * 8 : 4096;  // of 4-bit rows only the query is staged, as float64
         unsigned char* stage_r = stage_q + q_bytes;
         int rpr = (int)((sizeof(unsigned long long) * (CRAG_CAND_CAP - 1024) - q_bytes) / (size_t)row_bytes);
         if (rpr > 128 || a.dtype == CRAG_FP4) rpr = 128;  // 1024 threads / 8 lanes; 4-bit rows are read where they lie
-        for (int c = tid; c < chunks; c += 1024) ((uint4*)stage_q)[c] = ((const uint4*)qv)[c];
+        if (a.dtype == CRAG_FP4) {
+            for (int d = tid; d < a.dim_pad; d += 1024) ((double*)stage_q)[d] = (double)((const float*)qv)[d];
+        } else {
+            for (int c = tid; c < chunks; c += 1024) ((uint4*)stage_q)[c] = ((const uint4*)qv)[c];
+        }
         for (int base = 0; base < m; base += rpr) {
             const int nr = m - base < rpr ? m - base : rpr;
             __syncthreads();  // the previous round's readers are done
@@ -580,7 +612,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             double acc = 0.0;
             if (r < nr)
                 acc = a.dtype == CRAG_FP4
-                          ? canon_lane_fp4(D.rows, (const float*)stage_q, a.dim, a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), j, a.metric)
+                          ? canon_lane_fp4(D.rows, (const double*)stage_q, a.dim, a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), j, a.metric)
                           : canon_lane(stage_r, stage_q, a.dtype, a.dim, j, a.metric, (long long)r * a.dim_pad);
             acc = combine8(acc);
             if (r < nr && j == 0) {
@@ -600,11 +632,11 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     float* rr_dist = (float*)(rr_row + CRAG_MAX_KC);   // [CRAG_MAX_KC]
     double* rr_score = (double*)(rr_dist + CRAG_MAX_KC);  // [CRAG_MAX_KC], negative: not kept
     if (tid == 0) n_keep = 0;
-    for (int i = tid; i < m; i += blockDim.x) {
-        const unsigned long long k = ekeys[i];
-        int rank = 0;
-        for (int t = 0; t < m; ++t) rank += ekeys[t] < k;
-        if (rank < a.kc) {
+    const int m_lanes = lanes_per_item(m);  // m <= CRAG_MAX_M: every item has its lanes at once
+    if (tid / m_lanes < m) {
+        const unsigned long long k = ekeys[tid / m_lanes];
+        const int rank = count_before(m, tid % m_lanes, m_lanes, [&](int t) { return ekeys[t] < k; });
+        if (rank < a.kc && tid % m_lanes == 0) {
             const uint32_t row = (uint32_t)(k & 0xffffffffull);
             uint32_t flags = 0;
             if (D.path_class) flags |= (uint32_t)((const __attribute__((address_space(1))) unsigned char*)D.path_class)[row] & CRAG_FLAG_CLASS_MASK;
@@ -683,13 +715,12 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     if (!a.out_ids) return;
     // R5 (hybrid_search.py:120-125) of a single shard, whose entries are in order already: strict > 0.01 filter, stable
     // descending sort by counting, top_k
-    for (int j = tid; j < kc_valid; j += blockDim.x) {
+    const int r_lanes = lanes_per_item(kc_valid), j = tid / r_lanes;
+    if (j < kc_valid && rr_score[j] >= 0.0) {
         const double s = rr_score[j];
-        if (s < 0.0) continue;
-        int rank = 0;
-        for (int t = 0; t < kc_valid; ++t) rank += rr_score[t] > s || (rr_score[t] == s && t < j);
-        atomicAdd(&n_keep, 1u);
-        if (rank < a.top_k) {
+        const int rank = count_before(kc_valid, tid % r_lanes, r_lanes, [&](int t) { return rr_score[t] > s || (rr_score[t] == s && t < j); });
+        if (tid % r_lanes == 0) atomicAdd(&n_keep, 1u);
+        if (rank < a.top_k && tid % r_lanes == 0) {
             a.out_ids[(long long)q * a.top_k + rank] = D.id_base + (long long)rr_row[j];
             a.out_scores[(long long)q * a.top_k + rank] = s;
             a.out_dist[(long long)q * a.top_k + rank] = rr_dist[j];
