@@ -349,10 +349,10 @@ __device__ __forceinline__ double canon_lane(const void* row, const void* q, int
                              : canon_lane_t<CRAG_BF16>(row, q, dim, j, metric, row_off);
 }
 
-// The same partial sum of a 4-bit row in the tiles of crag_fp4.h (q: float32 or float64, in LDS or in global memory): of a
-// group's four words of eight codes, lane j takes code j of each.  The eight lanes of a row read the same 16 bytes (one
-// request), eight groups at a time, the next eight on their way while these are added; nothing of the row is staged, because
-// every element is used once.
+// The same sum of a 4-bit row in the tiles of crag_fp4.h (q: float32 or float64, in LDS or in global memory), by four lanes
+// that take two of the eight partial sums each: of a group's four words of eight codes, lane j takes the neighbours 2 j and
+// 2 j + 1, which one instruction decodes.  The lanes of a row read the same 16 bytes (one request), eight groups at a time, the
+// next eight on their way while these are added; nothing of the row is staged, because every element is used once.
 struct Fp4Batch {
     typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
     u32x4_t c[8];   // groups 8 b .. 8 b + 7
@@ -369,12 +369,13 @@ struct Fp4Batch {
     }
 };
 template <typename Q>
-__device__ __forceinline__ double canon_lane_fp4(const void* rows, const Q* q, int dim, int dim_pad, long long row, int j, int metric) {
+__device__ __forceinline__ double canon_fp4(const void* rows, const Q* q, int dim, int dim_pad, long long row, int j, int metric) {
     typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+    typedef __attribute__((ext_vector_type(2))) Q q2_t;
     const int ks = dim_pad >> 6, r = (int)(row & 31), n = (dim + 255) / 256;
     const __attribute__((address_space(1))) unsigned char* tile =
         (const __attribute__((address_space(1))) unsigned char*)rows + (row >> 5) * crag_fp4_tile_bytes(ks);
-    double acc = 0.0;
+    double acc[2] = {0.0, 0.0};
     Fp4Batch cur;
     cur.load(tile, ks, r, 0);
     for (int b = 0; b < n; ++b) {
@@ -383,26 +384,31 @@ __device__ __forceinline__ double canon_lane_fp4(const void* rows, const Q* q, i
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const float scale = crag_fp4_scale((cur.s[u & 1] >> (8 * (u >> 1))) & 255u);
+            const int d0 = b * 256 + u * 32 + 2 * j;
+            if (b * 256 + u * 32 < dim) {  // (elements behind the row's end are zero in both: they add +0)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int d = b * 256 + u * 32 + 8 * v + j;
-                if (d < dim) {
-                    const f32x2_t two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cur.c[u][v] >> (4 * j), scale, 0);  // exact
-                    const double a = (double)q[d], x = (double)two.x;
-                    double p;
-                    if (metric == CRAG_L2) {
-                        const double t = __dsub_rn(a, x);
-                        p = __dmul_rn(t, t);
-                    } else {
-                        p = __dmul_rn(a, x);
+                for (int v = 0; v < 4; ++v) {
+                    const f32x2_t two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(cur.c[u][v] >> (8 * j), scale, 0);  // exact
+                    const q2_t a = *(const q2_t*)(q + d0 + 8 * v);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        double p;
+                        if (metric == CRAG_L2) {
+                            const double t = __dsub_rn((double)a[h], (double)two[h]);
+                            p = __dmul_rn(t, t);
+                        } else {
+                            p = __dmul_rn((double)a[h], (double)two[h]);
+                        }
+                        acc[h] = __dadd_rn(acc[h], p);
                     }
-                    acc = __dadd_rn(acc, p);
                 }
             }
         }
         cur = next;
     }
-    return acc;
+    double s = __dadd_rn(acc[0], acc[1]);  // the order of combine8
+    s = __dadd_rn(s, __shfl_xor(s, 1));
+    return __dadd_rn(s, __shfl_xor(s, 2));
 }
 
 __device__ __forceinline__ double combine8(double acc) {
@@ -574,7 +580,8 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         const int q_bytes = a.dtype == CRAG_FP4 ? a.dim_pad * 8 : 4096;  // of 4-bit rows only the query is staged, as float64
         unsigned char* stage_r = stage_q + q_bytes;
         int rpr = (int)((sizeof(unsigned long long) * (CRAG_CAND_CAP - 1024) - q_bytes) / (size_t)row_bytes);
-        if (rpr > 128 || a.dtype == CRAG_FP4) rpr = 128;  // 1024 threads / 8 lanes; 4-bit rows are read where they lie
+        if (rpr > 128) rpr = 128;  // 1024 threads / 8 lanes
+        if (a.dtype == CRAG_FP4) rpr = 256;  // read where they lie, by four lanes
         if (a.dtype == CRAG_FP4) {
             for (int d = tid; d < a.dim_pad; d += 1024) ((double*)stage_q)[d] = (double)((const float*)qv)[d];
         } else {
@@ -608,13 +615,15 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
                 }
             }
             __syncthreads();
-            const int r = tid >> 3, j = tid & 7;
+            const int lanes = a.dtype == CRAG_FP4 ? 4 : 8, r = tid / lanes, j = tid % lanes;
             double acc = 0.0;
-            if (r < nr)
-                acc = a.dtype == CRAG_FP4
-                          ? canon_lane_fp4(D.rows, (const double*)stage_q, a.dim, a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), j, a.metric)
-                          : canon_lane(stage_r, stage_q, a.dtype, a.dim, j, a.metric, (long long)r * a.dim_pad);
-            acc = combine8(acc);
+            if (a.dtype == CRAG_FP4) {
+                if (r < nr)
+                    acc = canon_fp4(D.rows, (const double*)stage_q, a.dim, a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), j, a.metric);
+            } else {
+                if (r < nr) acc = canon_lane(stage_r, stage_q, a.dtype, a.dim, j, a.metric, (long long)r * a.dim_pad);
+                acc = combine8(acc);
+            }
             if (r < nr && j == 0) {
                 const double dist = a.metric == CRAG_L2 ? acc : __dsub_rn(1.0, acc);
                 ekeys[base + r] = ((unsigned long long)crag_fkey((float)dist) << 32) | (uint32_t)(skeys[base + r] & 0xffffffffull);
@@ -838,19 +847,20 @@ __global__ __launch_bounds__(1024) void k_rescore_wide(FinalizeArgs a, unsigned 
     unsigned long long* __restrict__ cq = cand_rw + (long long)q * a.cand_stride;
     const size_t esz = a.dtype == CRAG_BF16 ? 2 : 4;
     const void* qv = (const char*)a.queries + (size_t)q * a.dim_pad * esz;
-    const int j = tid & 7;
-    for (int i0 = 0; i0 < c; i0 += 128) {  // the trip count is block-uniform: combine8 shuffles among all lanes
-        const int i = i0 + (tid >> 3);
+    const bool fp4 = a.dtype == CRAG_FP4;
+    const int lanes = fp4 ? 4 : 8, j = tid % lanes;
+    for (int i0 = 0; i0 < c; i0 += 1024 / lanes) {  // the trip count is block-uniform: combine8 shuffles among all lanes
+        const int i = i0 + tid / lanes;
         int slot = 0;
         uint32_t row = 0;
         double acc = 0.0;
         if (i < c) {
             slot = seg ? seg_slot(seg_off, a.n_seg, a.seg_cap, i) : i;
             row = (uint32_t)(cq[slot] & 0xffffffffull);
-            acc = a.dtype == CRAG_FP4 ? canon_lane_fp4(D.rows, (const float*)qv, a.dim, a.dim_pad, (long long)row, j, a.metric)
-                                      : canon_lane(D.rows, qv, a.dtype, a.dim, j, a.metric, (long long)row * a.dim_pad);
+            acc = fp4 ? canon_fp4(D.rows, (const float*)qv, a.dim, a.dim_pad, (long long)row, j, a.metric)
+                      : canon_lane(D.rows, qv, a.dtype, a.dim, j, a.metric, (long long)row * a.dim_pad);
         }
-        acc = combine8(acc);
+        if (!fp4) acc = combine8(acc);
         if (i < c && j == 0) {
             const double dist = a.metric == CRAG_L2 ? acc : __dsub_rn(1.0, acc);
             cq[slot] = ((unsigned long long)crag_fkey((float)dist) << 32) | row;
