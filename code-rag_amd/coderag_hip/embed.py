@@ -21,6 +21,7 @@ question/chunk pairs).  With the identity as its table it computes HashingEmbedd
 """
 from __future__ import annotations
 
+import functools
 import warnings
 import zlib
 from typing import Callable, List, Optional, Sequence, Tuple
@@ -97,10 +98,19 @@ def _check_bags(table, ids, offsets, weights):
         raise ValueError("one weight per id")
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(n_tokens: int, n_bags: int, dim: int, backward: bool) -> int:
+    return int(check(_lib.load().crag_embed_workspace(n_tokens, n_bags, dim, int(backward)), "crag_embed_workspace"))
+
+
 def _workspace(n_tokens: int, n_bags: int, dim: int, backward: bool, device):
+    """(tensor or None, its address or None, its bytes)"""
     import torch
-    size = check(_lib.load().crag_embed_workspace(n_tokens, n_bags, dim, int(backward)), "crag_embed_workspace")
-    return torch.empty(max(int(size), 256), dtype=torch.uint8, device=device)
+    size = _workspace_bytes(n_tokens, n_bags, dim, backward)
+    if size == 0:
+        return None, None, 0
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), size
 
 
 def _dtype_id(t) -> int:
@@ -117,11 +127,11 @@ def _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, wa
     dev, n_bags, (vocab, dim) = table.device, offsets.numel() - 1, table.shape
     out = torch.empty((n_bags, dim), dtype=out_dtype, device=dev)
     coef = torch.empty((n_bags,), dtype=torch.float32, device=dev) if want_coef else None
-    ws = _workspace(ids.numel(), n_bags, dim, False, dev)
+    n = ids.numel()
+    ws, ws_ptr, ws_bytes = _workspace(n, n_bags, dim, False, dev)
     check(_lib.load().crag_embed_forward_device(
-        dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), ids.numel(), offsets.data_ptr(),
-        n_bags, POOL_MODES[mode], float(scale), int(bool(normalize)), out.data_ptr(), _dtype_id(out), _ptr(coef), ws.data_ptr(),
-        ws.numel(), torch.cuda.current_stream(dev).cuda_stream), "crag_embed_forward_device")
+        dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), n, offsets.data_ptr(), n_bags,
+        POOL_MODES[mode], float(scale), int(bool(normalize)), out.data_ptr(), _dtype_id(out), _ptr(coef), ws_ptr, ws_bytes, torch.cuda.current_stream(dev).cuda_stream), "crag_embed_forward_device")
     return out, coef
 
 
@@ -151,11 +161,11 @@ def _bag_function():
             grad = grad.contiguous()
             d_table = torch.empty_like(table) if ctx.needs_input_grad[0] else None
             d_weights = torch.empty_like(weights) if weights is not None and ctx.needs_input_grad[1] else None
-            ws = _workspace(ids.numel(), n_bags, dim, True, dev)
+            ws, ws_ptr, ws_bytes = _workspace(ids.numel(), n_bags, dim, True, dev)
             check(_lib.load().crag_embed_backward_device(
                 dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), ids.numel(),
                 offsets.data_ptr(), n_bags, int(ctx.normalize), y.data_ptr(), coef.data_ptr(), grad.data_ptr(), _ptr(d_table),
-                _ptr(d_weights), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream),
+                _ptr(d_weights), ws_ptr, ws_bytes, torch.cuda.current_stream(dev).cuda_stream),
                 "crag_embed_backward_device")
             return d_table, d_weights, None, None, None, None, None
 

@@ -499,35 +499,109 @@ __global__ __launch_bounds__(256) void k_embed_finish(CragSegArgs a, int gp) {
     finish_bag(a, b, acc, count, c);
 }
 
-// Backward, after k_segsum: block g joins the token whose first partial sum is share g's tail -- it goes on through the heads
-// of the shares behind it.
+// Forward for few positions (BAG_MOST in all): a block per bag, its groups of lanes a run of positions each, joined in LDS -- one
+// launch, and no workspace.  (1 bag of 120 tokens: 6 us on the GPU and one launch's host time, against 12 us and two.)
+constexpr int BAG_MOST = 4096, BAG_THREADS = 512;
+template <int DT, int VEC, int NV>
+__global__ __launch_bounds__(BAG_THREADS) void k_embed_bag(CragSegArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ int part_count[BAG_THREADS / 8];
+    float* part = (float*)smem;  // [groups][lpr * VEC * NV]
+    Cols c;
+    c.dim = a.dim;
+    c.lpr = a.lpr;
+    c.sub = threadIdx.x & (a.lpr - 1);
+    const Pieces<DT, VEC, NV> pieces(c);
+    const long long b = blockIdx.x;
+    const int groups = BAG_THREADS / a.lpr, grp = threadIdx.x / a.lpr;
+    long long x0 = a.offsets[b], x1 = a.offsets[b + 1];
+    x0 = x0 < 0 ? 0 : x0;
+    x1 = x1 > a.n ? a.n : x1;
+    const int len = x1 > x0 ? (int)(x1 - x0) : 0, per = (len + groups - 1) / groups;
+    const int i0 = grp * per, i1 = i0 + per < len ? i0 + per : len;
+    Row<VEC, NV> acc;
+    acc.zero();
+    int count = 0;
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) {
+        const int id = a.ids[x0 + i];
+        const float w = a.weights ? a.weights[x0 + i] : 1.f;
+        const bool on = id >= 0 && id < a.vocab;
+        RawRow<DT, VEC, NV> x;
+        x.load(a.src, on ? id : 0, a.dim, pieces);
+        if (on) {
+            acc.fma(x, w);
+            ++count;
+        }
+    }
+    const int rowlen = a.lpr * VEC * NV;
+    if (grp > 0 && i0 < len) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) part[grp * rowlen + (v * a.lpr + c.sub) * VEC + k] = acc.x[v][k];
+        if (c.sub == 0) part_count[grp] = count;
+    }
+    __syncthreads();
+    if (grp > 0) return;
+    for (int o = 1; o < groups && o * per < len; ++o) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc.x[v][k] += part[o * rowlen + (v * a.lpr + c.sub) * VEC + k];
+        count += part_count[o];
+    }
+    finish_bag(a, b, acc, count, c);
+}
+
+// Backward, after k_segsum: a token whose first partial sum is share g's tail goes on through the heads of the shares behind
+// it.  A block looks at four shares, one to a wave; a wave joins up to JOIN_ALONE rows by itself, longer ones (frequent tokens)
+// take the whole block.
+constexpr int JOIN_ALONE = 16;
 template <int VEC, int NV>
 __global__ __launch_bounds__(256) void k_segjoin(CragSegArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ int part_count[64];
-    __shared__ int s_end;
-    const int tid = threadIdx.x;
-    const long long g = blockIdx.x;
-    const int seg = a.partial_seg[2 * g + 1];
-    if (seg < 0) return;
+    __shared__ int s_seg[4], s_rows[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const long long g = (long long)blockIdx.x * 4 + wave;
+    const int seg = g < a.n_share ? a.partial_seg[2 * g + 1] : -1;
+    int n = 0;  // partial sums: tail of g, heads of g + 1 .. g + n - 1
+    if (seg >= 0)
+        for (long long j0 = g + 1;; j0 += 64) {
+            const long long j = j0 + lane;
+            const unsigned long long other = __ballot(j >= a.n_share || a.partial_seg[2 * j] != seg);
+            if (other) {
+                n = (int)(j0 - g) + __builtin_ctzll(other);
+                break;
+            }
+        }
     Cols c;
     c.dim = a.dim;
     c.lpr = a.lpr;
     c.sub = tid & (a.lpr - 1);
-    if (tid == 0) s_end = 0x7fffffff;
+    if (lane == 0) {
+        s_seg[wave] = seg;
+        s_rows[wave] = n;
+    }
+    if (n > 0 && n <= JOIN_ALONE && lane < a.lpr) {
+        Row<VEC, NV> acc;
+        acc.zero();
+        join_rows<VEC, NV>(a, n, 0, 1, 0, [&](int i) { return i == 0 ? 2 * g + 1 : 2 * (g + i); }, c, nullptr, nullptr, acc);
+        acc.template store<true>(a.out, a.out_dtype, seg, c);
+    }
     __syncthreads();
-    for (long long j0 = g + 1;; j0 += 256) {  // the last share that holds a head of this token
-        const long long j = j0 + tid;
-        if (j >= a.n_share || a.partial_seg[2 * j] != seg) atomicMin(&s_end, (int)(j < a.n_share ? j : a.n_share));
-        __syncthreads();
-        if (s_end != 0x7fffffff) break;
+    for (int w = 0; w < 4; ++w) {
+        const int rows = s_rows[w];
+        if (rows <= JOIN_ALONE) continue;
+        const long long gw = (long long)blockIdx.x * 4 + w;
+        const int gp = 256 / a.lpr, grp = tid / a.lpr;
+        Row<VEC, NV> acc;
+        acc.zero();
+        join_rows<VEC, NV>(a, rows, grp, gp, grp, [&](int i) { return i == 0 ? 2 * gw + 1 : 2 * (gw + i); }, c, (float*)smem, part_count, acc);
+        if (grp == 0) acc.template store<true>(a.out, a.out_dtype, s_seg[w], c);
         __syncthreads();
     }
-    const int n = s_end - (int)g, gp = 256 / a.lpr, grp = tid / a.lpr;  // partial sums: tail of g, heads of g + 1 .. s_end - 1
-    Row<VEC, NV> acc;
-    acc.zero();
-    join_rows<VEC, NV>(a, n, grp, gp, grp, [&](int i) { return i == 0 ? 2 * g + 1 : 2 * (g + i); }, c, (float*)smem, part_count, acc);
-    if (grp == 0) acc.store(a.out, a.out_dtype, seg, c);
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
@@ -968,6 +1042,20 @@ int launch_segsum(CragSegArgs a, const Walk& w, hipStream_t s) {
 #undef X
     return -1;
 }
+template <int DT>
+int launch_bag(const CragSegArgs& a, const Shape& sh, hipStream_t s) {
+    const size_t lds = sizeof(float) * BAG_THREADS * sh.vec * sh.nv;  // at most 64 KiB
+#define X(V, N)                                                                                                                     \
+    if (sh.vec == V && sh.nv == N) {                                                                                                \
+        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                                \
+            hipLaunchKernelGGL((k_embed_bag<DT, V, N>), dim3((unsigned)a.n_seg), dim3(BAG_THREADS), lds, s, a);                      \
+            return (int)hipGetLastError();                                                                                          \
+        }                                                                                                                           \
+    }
+    CRAG_SEG_CASES(X)
+#undef X
+    return -1;
+}
 // joins: whole rows of float32, so shapes of their own
 int launch_finish(CragSegArgs a, hipStream_t s) {
     const Shape sh = row_shape(a.dim, std::min(vec_of(a.dim, 4, nullptr), vec_of(a.dim, a.out_dtype == CRAG_F32 ? 4 : 2, a.out)));
@@ -997,7 +1085,7 @@ int launch_join(CragSegArgs a, hipStream_t s) {
 #define X(V, N)                                                                                                                          \
     if (sh.vec == V && sh.nv == N) {                                                                                                     \
         if constexpr (V != 8) {                                                                                                          \
-            hipLaunchKernelGGL((k_segjoin<V, N>), dim3((unsigned)a.n_share), dim3(256), sizeof(float) * 256 * sh.vec * sh.nv, s, a);      \
+            hipLaunchKernelGGL((k_segjoin<V, N>), dim3((unsigned)((a.n_share + 3) / 4)), dim3(256), sizeof(float) * 256 * sh.vec * sh.nv, s, a);      \
             return (int)hipGetLastError();                                                                                               \
         }                                                                                                                                \
     }
@@ -1044,6 +1132,7 @@ struct FwdWs {
     int *partial_count, *sums_count;
 };
 FwdWs carve_fwd(Carve& c, long long n, int n_bags, int dim) {
+    if (n <= BAG_MOST) return FwdWs{};
     const size_t slots = 2 * (size_t)most_shares(n, dim);
     FwdWs w;
     w.partial = (float*)c.take(sizeof(float) * slots * (size_t)dim);
@@ -1106,6 +1195,7 @@ int crag_launch_embed_forward(const CragEmbedArgs& e, hipStream_t s) {
     a.normalize = e.normalize;
     a.scale = e.scale;
     a.coef = e.coef;
+    if (e.n <= BAG_MOST) return e.dtype == CRAG_F32 ? launch_bag<CRAG_F32>(a, w.sh, s) : launch_bag<CRAG_BF16>(a, w.sh, s);
     const int rc = e.dtype == CRAG_F32 ? launch_segsum<CRAG_F32, false>(a, w, s) : launch_segsum<CRAG_BF16, false>(a, w, s);
     return rc ? rc : launch_finish(a, s);
 }

@@ -300,10 +300,11 @@ def test_workspace_size_is_checked():
     import torch
     lib = ch.load()
     table = torch.randn((10, 8), device="cuda")
-    ids, off = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 4], device="cuda")
     out, ws = torch.empty((1, 8), device="cuda"), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
-    need = lib.crag_embed_workspace(4, 1, 8, 0)
-    args = [0, table.data_ptr(), 10, 8, 0, ids.data_ptr(), None, 4, off.data_ptr(), 1, 0, 1.0, 0, out.data_ptr(), 0, None, ws.data_ptr(), need, None]
+    ids = torch.zeros(5000, dtype=torch.int32, device="cuda")
+    off = torch.tensor([0, 4], device="cuda")
+    need = lib.crag_embed_workspace(5000, 1, 8, 0)
+    args = [0, table.data_ptr(), 10, 8, 0, ids.data_ptr(), None, 5000, off.data_ptr(), 1, 0, 1.0, 0, out.data_ptr(), 0, None, ws.data_ptr(), need, None]
     assert lib.crag_embed_forward_device(*args) == 0
     torch.cuda.synchronize()
     assert torch.allclose(out[0], 4 * table[0])
