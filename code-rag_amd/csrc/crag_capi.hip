@@ -1384,6 +1384,7 @@ int check_embed(const char* who, const void* table, int64_t vocab, int dim, int 
     const std::string w = who;
     if (!table || vocab <= 0 || vocab > 0x7fffffff || dim <= 0 || n < 0 || n > 0x7fffffff || n_bags < 0) return fail(CRAG_E_INVALID, w + ": bad arguments");
     if (dim > CRAG_MAX_EMBED_DIM) return fail(CRAG_E_LIMIT, w + ": more than 2048 elements per row");
+    if (n_bags > CRAG_MAX_EMBED_BAGS) return fail(CRAG_E_LIMIT, w + ": more than 2^24 bags");
     if (dtype != CRAG_F32 && dtype != CRAG_BF16) return fail(CRAG_E_INVALID, w + ": tables are float32 or bf16");
     if (((uintptr_t)table & (dtype == CRAG_F32 ? 3 : 1)) != 0) return fail(CRAG_E_INVALID, w + ": the table must be aligned to its elements");
     if ((n > 0 && !ids) || (n_bags > 0 && !offsets)) return fail(CRAG_E_INVALID, w + ": null buffer");
@@ -1659,7 +1660,7 @@ int crag_search_device(crag_index* h, const void* queries_dev, int B, int top_k,
     mo.counts = out_counts_dev;
     rc = search_entries(hs.data(), true, q, B, top_k, q_hashes_dev, q_hash_off_dev, (CragEntry*)ws->entries.p, ws, st, &mo);
     if (rc) return rc;
-    HIPCHK(hipStreamSynchronize(st));  // only non-trivial after a fallback re-merge
+    HIPCHK(stream_wait(st));  // only non-trivial after a fallback re-merge
     return 0;
 }
 
@@ -1723,7 +1724,7 @@ int crag_search_multi_device(crag_index* const* hs, const void* queries_dev, int
     mo.counts = out_counts_dev;
     rc = search_entries(hs, same, q, B, top_k, q_hashes_dev, q_hash_off_dev, (CragEntry*)ws->entries.p, ws, st, &mo);
     if (rc) return rc;
-    HIPCHK(hipStreamSynchronize(st));  // only non-trivial after a fallback re-merge
+    HIPCHK(stream_wait(st));  // only non-trivial after a fallback re-merge
     return 0;
 }
 
@@ -1877,6 +1878,7 @@ int crag_set_path(crag_index* h, int path) {
 int64_t crag_embed_workspace(int64_t n_tokens, int n_bags, int dim, int backward) {
     if (n_tokens < 0 || n_tokens > 0x7fffffff || n_bags < 0 || dim <= 0) return fail(CRAG_E_INVALID, "crag_embed_workspace: bad arguments");
     if (dim > CRAG_MAX_EMBED_DIM) return fail(CRAG_E_LIMIT, "crag_embed_workspace: more than 2048 elements per row");
+    if (n_bags > CRAG_MAX_EMBED_BAGS) return fail(CRAG_E_LIMIT, "crag_embed_workspace: more than 2^24 bags");
     return (int64_t)crag_embed_ws_bytes(n_tokens, n_bags, dim, backward != 0);
 }
 

@@ -283,6 +283,7 @@ int crag_launch_fp4_row_norms(const void* rows, int dim_pad, long long n, float*
 #define CRAG_POOL_MEAN 1
 #define CRAG_POOL_SQRT 2
 #define CRAG_MAX_EMBED_DIM 2048
+constexpr int CRAG_MAX_EMBED_BAGS = 1 << 24;  // grids of up to 64 threads a bag stay below 2^32
 struct CragEmbedArgs {
     const void* table;  // [vocab][dim], dtype
     long long vocab;
@@ -313,14 +314,14 @@ struct CragSegArgs {
     const int* ids;            // forward
     const float* weights;
     const long long* offsets;  // forward
-    const uint32_t *keys, *perm;  // backward: sorted tokens and their positions
-    const int* bag;               // backward: bag of a position
+    const uint2* pairs;        // backward: sorted (token, position)
+    const int* bag;            // backward: bag of a position
     float* partial;    // [n_share][2][dim]: sum of a segment that began in front of the share, of one that goes on behind it
     int *partial_seg, *partial_count;  // [n_share][2]: backward, forward
     float* sums;       // forward: [n_seg][dim] plain sums of the bags that lie in one share, and how many tokens each has
     int* sums_count;
     void* out;
-    int out_dtype, mode, normalize;
+    int out_dtype, mode, normalize, joined;  // joined: forward, `sums` holds the bags that cross shares too
     float scale;
     float* coef;
 };

@@ -223,9 +223,9 @@ __device__ __forceinline__ void zero_absent(const CragSegArgs& a, long long bloc
         long long lo = 0, hi = a.n;  // the first position whose key is not below v
         while (lo < hi) {
             const long long mid = (lo + hi) >> 1;
-            if ((long long)a.keys[mid] < v) lo = mid + 1; else hi = mid;
+            if ((long long)a.pairs[mid].x < v) lo = mid + 1; else hi = mid;
         }
-        absent = lo == a.n || (long long)a.keys[lo] != v;
+        absent = lo == a.n || (long long)a.pairs[lo].x != v;
     }
     const long long bytes = (long long)a.dim * (a.out_dtype == CRAG_F32 ? 4 : 2);
     for (unsigned long long m = __ballot(absent); m; m &= m - 1) {
@@ -298,9 +298,9 @@ __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
         f = 0.f;
         if (pm >= p1) return;
         if constexpr (BWD) {
-            const uint32_t k = a.keys[pm];
-            i = k < (uint32_t)a.vocab ? (int)k : -1;
-            f = __builtin_bit_cast(float, a.perm[pm]);
+            const uint2 kv = a.pairs[pm];
+            i = kv.x < (uint32_t)a.vocab ? (int)kv.x : -1;
+            f = __builtin_bit_cast(float, kv.y);
         } else {
             const int id = a.ids[pm];
             f = a.weights ? a.weights[pm] : 1.f;
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
                     const int k = ku[u];
                     if (k != (int)seg || p == p0) {
                         if (p != p0 && seg >= 0) done(false);
-                        before = p == p0 && p > 0 && k >= 0 && (int)a.keys[p - 1] == k;
+                        before = p == p0 && p > 0 && k >= 0 && (int)a.pairs[p - 1].x == k;
                         seg = k;
                         acc.zero();
                     }
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
                     if (seg < 0 || p >= end) {
                         if (seg >= 0) done(false);
                         seg = last_le(a.offsets, a.n_seg, p);
-                        if (seg >= a.n_seg) {
+                        if (seg < 0 || seg >= a.n_seg) {
                             seg = -1;
                             hi = p;
                             break;
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
         }
     }
     if (seg >= 0) {
-        if constexpr (BWD) done(p1 < T && (int)a.keys[p1] == (int)seg);
+        if constexpr (BWD) done(p1 < T && (int)a.pairs[p1].x == (int)seg);
         else done(p1 < hi && end > p1);
     }
     if (BWD && sub == 0 && g < a.n_share) {
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(256) void k_embed_finish(CragSegArgs a, int gp) {
         if (x0 < x1) {
             g0 = x0 / a.share;
             g1 = (x1 - 1) / a.share;
-            n = g0 == g1 ? 0 : (int)(g1 - g0 + 1);
+            n = g0 == g1 || a.joined ? 0 : (int)(g1 - g0 + 1);
         }
     }
     Row<VEC, NV> acc;
@@ -499,9 +499,60 @@ __global__ __launch_bounds__(256) void k_embed_finish(CragSegArgs a, int gp) {
     finish_bag(a, b, acc, count, c);
 }
 
-// Forward for few positions (BAG_MOST in all): a block per bag, its groups of lanes a run of positions each, joined in LDS -- one
-// launch, and no workspace.  (1 bag of 120 tokens: 6 us on the GPU and one launch's host time, against 12 us and two.)
-constexpr int BAG_MOST = 4096, BAG_THREADS = 512;
+// Forward, between the two where bags are long: sums of the bags' partial rows, a block per bag and slab of 16 * VEC columns,
+// JOIN_RUNS runs of rows joined in LDS.  One block of k_embed_finish would read them all by itself (1 bag of 4097 tokens, 1536
+// float32: 63 us of 72, against 7 us for this and the finish).
+constexpr int JOIN_RUNS = 64, JOIN_FROM = 64;  // (more partial rows than that in a bag of average length: 100 bags
+// of 50 rows of 384 are 9 us by k_embed_finish alone, 13 by both)
+template <int VEC>
+__global__ __launch_bounds__(16 * JOIN_RUNS) void k_embed_join(CragSegArgs a, int slabs) {
+    __shared__ float part[JOIN_RUNS][16 * VEC];
+    __shared__ int part_count[JOIN_RUNS];
+    const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4;
+    const long long b = blockIdx.x / slabs;
+    const int slab = blockIdx.x % slabs, col = (slab * 16 + lane) * VEC;
+    long long x0 = a.offsets[b], x1 = a.offsets[b + 1];
+    x0 = x0 < 0 ? 0 : x0;
+    x1 = x1 > a.n ? a.n : x1;
+    if (x0 >= x1) return;
+    const long long g0 = x0 / a.share, g1 = (x1 - 1) / a.share;
+    if (g0 == g1) return;  // k_segsum has stored it
+    const int n = (int)(g1 - g0 + 1), per = (n + JOIN_RUNS - 1) / JOIN_RUNS, i0 = grp * per, i1 = i0 + per < n ? i0 + per : n;
+    const int at = min(col, a.dim - VEC);
+    float acc[VEC] = {};
+    int count = 0;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) {
+        const long long s = i == 0 ? 2 * g0 + 1 : 2 * (g0 + i);
+        Raw<CRAG_F32, VEC> x;
+        x.load(a.partial, s * a.dim + at);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += x.get(k);
+        count += a.partial_count[s];
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) part[grp][lane * VEC + k] = acc[k];
+    if (lane == 0) part_count[grp] = count;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int o = 1; o < JOIN_RUNS && o * per < n; ++o) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += part[o][lane * VEC + k];
+        count += part_count[o];
+    }
+    if (col < a.dim) store_vec<VEC>(a.sums, CRAG_F32, b * a.dim + col, acc);
+    if (slab == 0 && lane == 0) a.sums_count[b] = count;
+}
+
+// Forward for few positions: a block per bag, its groups of lanes a run of positions each, joined in LDS -- one launch, and no
+// workspace.  (1 bag of 120 tokens: 6 us on the GPU and one launch's host time, against 12 us and two.)  A block alone reads
+// about 100 GB/s, and any one bag may hold nearly all of the positions, so the rule bounds what they can be in all: 1 bag of
+// 1536 float32 takes 11 us at 128 tokens, 17 at 256 and 43 at 512, the other way 14 .. 18; 1 bag of 64 bf16 15 at 2048 and 24 at
+// 4096 against 15; 64 bags of 384 float32, 4096 tokens in all, 6 against 11.
+constexpr int BAG_MOST = 2048, BAG_ELEMS = 192 << 10, BAG_THREADS = 512;
+bool one_launch(long long n, int n_bags, int dim) {
+    return n <= BAG_MOST * std::min(std::max(n_bags, 1), 2) && n_bags <= (1 << 20) && n * dim <= (long long)BAG_ELEMS * std::min(std::max(n_bags, 1), 8);
+}
 template <int DT, int VEC, int NV>
 __global__ __launch_bounds__(BAG_THREADS) void k_embed_bag(CragSegArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -614,7 +665,8 @@ struct BwdArgs {
     const long long* offsets;
     int vocab;
     int* bag;
-    uint32_t *keys, *perm;
+    uint32_t* keys;  // null: no sort
+    uint2* pairs;    // k_bwd_start_small: the sorted positions
     uint32_t* hist;
     int tiles, mask;  // of the first digit
 };
@@ -731,8 +783,7 @@ __global__ __launch_bounds__(1024) void k_bwd_start_small(BwdArgs a) {
             cur ^= 1;
         }
         for (int t = tid; t < n; t += 1024) {
-            a.keys[t] = key[cur][t];
-            a.perm[t] = pos[cur][t];
+            a.pairs[t] = make_uint2(key[cur][t], pos[cur][t]);
         }
     } else {
         for (int t = tid; t < n; t += 1024) a.bag[t] = bag_at(a, t);
@@ -751,25 +802,23 @@ __global__ __launch_bounds__(256) void k_bwd_start(BwdArgs a) {
     }
     for (int d = tid; d <= a.mask; d += 256) h[d] = 0;
     __syncthreads();
-    const long long t0 = (long long)blockIdx.x * SORT_TILE + tid * SORT_PER;
-    if (t0 < a.n) {
-        int b = last_le(a.offsets, a.n_bags, t0);
-        long long end = b < a.n_bags ? a.offsets[b + 1] : 0;
+    long long t = (long long)blockIdx.x * SORT_TILE + tid;
+    if (t < a.n) {
+        int b = last_le(a.offsets, a.n_bags, t);
+        long long end = b < a.n_bags ? a.offsets[b + 1] : a.n;
 #pragma unroll
-        for (int i = 0; i < SORT_PER; ++i) {
-            const long long t = t0 + i;
-            if (t < a.n) {
-                if (b < a.n_bags && t >= end) {
-                    b = last_le(a.offsets, a.n_bags, t);
-                    end = b < a.n_bags ? a.offsets[b + 1] : 0;
-                }
-                const int bag = b < a.n_bags ? b : -1;
-                a.bag[t] = bag;
-                if (a.keys) {
-                    const uint32_t k = key_of(a, t, bag);
-                    a.keys[t] = k;
-                    atomicAdd(&h[k & a.mask], 1u);
-                }
+        for (int i = 0; i < SORT_PER; ++i, t += 256) {
+            if (t >= a.n) break;
+            for (int step = 0; step < 5 && t >= end && b < a.n_bags; ++step) {  // the next bag, or behind a run of short ones
+                b = step < 4 ? b + 1 : last_le(a.offsets, a.n_bags, t);
+                end = b < a.n_bags ? a.offsets[b + 1] : a.n;
+            }
+            const int bag = b < a.n_bags ? b : -1;
+            a.bag[t] = bag;
+            if (a.keys) {
+                const uint32_t k = key_of(a, t, bag);
+                a.keys[t] = k;
+                atomicAdd(&h[k & a.mask], 1u);
             }
         }
     }
@@ -777,7 +826,8 @@ __global__ __launch_bounds__(256) void k_bwd_start(BwdArgs a) {
     if (a.keys)
         for (int d = tid; d <= a.mask; d += 256) a.hist[(long long)d * a.tiles + blockIdx.x] = h[d];
 }
-__global__ __launch_bounds__(256) void k_sort_count(const uint32_t* __restrict__ keys, long long n, int shift, int mask, int tiles,
+// (a sorted position is a pair: .x its key, .y the position it had)
+__global__ __launch_bounds__(256) void k_sort_count(const uint2* __restrict__ pairs, long long n, int shift, int mask, int tiles,
                                                     uint32_t* __restrict__ hist) {
     __shared__ uint32_t h[1 << SORT_BITS];
     for (int d = threadIdx.x; d <= mask; d += 256) h[d] = 0;
@@ -786,7 +836,7 @@ __global__ __launch_bounds__(256) void k_sort_count(const uint32_t* __restrict__
 #pragma unroll
     for (int i = 0; i < SORT_PER; ++i) {
         const long long p = base + i * 256 + threadIdx.x;
-        if (p < n) atomicAdd(&h[(keys[p] >> shift) & mask], 1u);
+        if (p < n) atomicAdd(&h[(pairs[p].x >> shift) & mask], 1u);
     }
     __syncthreads();
     for (int d = threadIdx.x; d <= mask; d += 256) hist[(long long)d * tiles + blockIdx.x] = h[d];
@@ -815,11 +865,10 @@ __global__ __launch_bounds__(256) void k_sort_prefix(uint32_t* __restrict__ hist
     }
     if (threadIdx.x == 0) total[blockIdx.x] = run;
 }
-// perm == null: position p holds p
-__global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ perm, long long n,
+// the first pass reads the keys alone (pairs == null): position p holds p
+__global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict__ keys, const uint2* __restrict__ pairs, long long n,
                                                       int shift, int bits, int tiles, const uint32_t* __restrict__ hist,
-                                                      const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
-                                                      uint32_t* __restrict__ perm_out) {
+                                                      const uint32_t* __restrict__ total, uint2* __restrict__ out) {
     __shared__ uint32_t cnt[4][1 << SORT_BITS];  // per wave: counts of its quarter of the tile, then where its next key of a digit goes
     __shared__ uint32_t ws[4];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -831,8 +880,9 @@ __global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict
 #pragma unroll
     for (int i = 0; i < SORT_PER; ++i) {
         const long long p = base + i * 64 + lane;
-        k[i] = p < n ? keys[p] : 0u;
-        v[i] = p >= n ? 0u : (perm ? perm[p] : (uint32_t)p);
+        const uint2 kv = p >= n ? make_uint2(0u, 0u) : (pairs ? pairs[p] : make_uint2(keys[p], (uint32_t)p));
+        k[i] = kv.x;
+        v[i] = kv.y;
         if (p < n) atomicAdd(&cnt[wv][(k[i] >> shift) & mask], 1u);
     }
     // where each digit starts: all smaller digits, then this digit in the tiles in front; thread tid has digits tid * per ..
@@ -874,8 +924,7 @@ __global__ __launch_bounds__(256) void k_sort_scatter(const uint32_t* __restrict
         if (on && rank == 0) next[d] = where + (uint32_t)__popcll(same);
         __builtin_amdgcn_wave_barrier();
         if (on) {
-            keys_out[where + rank] = k[i];
-            perm_out[where + rank] = v[i];
+            out[where + rank] = make_uint2(k[i], v[i]);
         }
     }
 }
@@ -1061,7 +1110,7 @@ int launch_finish(CragSegArgs a, hipStream_t s) {
     const Shape sh = row_shape(a.dim, std::min(vec_of(a.dim, 4, nullptr), vec_of(a.dim, a.out_dtype == CRAG_F32 ? 4 : 2, a.out)));
     a.lpr = sh.lpr;
     // groups of lanes per bag: one for each dozen partial rows of a bag of average length; for three while CUs are idle
-    const long long rows = a.n_seg > 0 ? a.n / a.share / a.n_seg : 0;
+    const long long rows = a.joined ? 0 : a.n / a.share / a.n_seg;
     int gp = 1;
     while (gp < 256 / sh.lpr && rows > 3 * gp && (rows > 12 * gp || (long long)a.n_seg * gp < 256 * (256 / sh.lpr))) gp <<= 1;
     const long long per = 256 / sh.lpr / gp, blocks = (a.n_seg + per - 1) / per;
@@ -1132,7 +1181,7 @@ struct FwdWs {
     int *partial_count, *sums_count;
 };
 FwdWs carve_fwd(Carve& c, long long n, int n_bags, int dim) {
-    if (n <= BAG_MOST) return FwdWs{};
+    if (one_launch(n, n_bags, dim)) return FwdWs{};
     const size_t slots = 2 * (size_t)most_shares(n, dim);
     FwdWs w;
     w.partial = (float*)c.take(sizeof(float) * slots * (size_t)dim);
@@ -1144,7 +1193,8 @@ FwdWs carve_fwd(Carve& c, long long n, int n_bags, int dim) {
 struct BwdWs {
     float *partial, *dp;
     int *partial_seg, *bag;
-    uint32_t *keys[2], *perm[2], *hist, *total;
+    uint2* pairs[2];
+    uint32_t *keys, *hist, *total;
 };
 BwdWs carve_bwd(Carve& c, long long n, int n_bags, int dim) {
     const size_t slots = 2 * (size_t)most_shares(n, dim);
@@ -1153,10 +1203,8 @@ BwdWs carve_bwd(Carve& c, long long n, int n_bags, int dim) {
     w.partial_seg = (int*)c.take(sizeof(int) * slots);
     w.dp = (float*)c.take(sizeof(float) * (size_t)n_bags * (size_t)dim);
     w.bag = (int*)c.take(sizeof(int) * (size_t)n);
-    for (int i = 0; i < 2; ++i) {
-        w.keys[i] = (uint32_t*)c.take(sizeof(uint32_t) * (size_t)n);
-        w.perm[i] = (uint32_t*)c.take(sizeof(uint32_t) * (size_t)n);
-    }
+    w.keys = (uint32_t*)c.take(sizeof(uint32_t) * (size_t)n);
+    for (int i = 0; i < 2; ++i) w.pairs[i] = (uint2*)c.take(sizeof(uint2) * (size_t)n);
     w.hist = (uint32_t*)c.take(n > SORT_SMALL ? sizeof(uint32_t) * ((size_t)1 << SORT_BITS) * (size_t)((n + SORT_TILE - 1) / SORT_TILE) : 0);
     w.total = (uint32_t*)c.take(sizeof(uint32_t) << SORT_BITS);
     return w;
@@ -1195,9 +1243,16 @@ int crag_launch_embed_forward(const CragEmbedArgs& e, hipStream_t s) {
     a.normalize = e.normalize;
     a.scale = e.scale;
     a.coef = e.coef;
-    if (e.n <= BAG_MOST) return e.dtype == CRAG_F32 ? launch_bag<CRAG_F32>(a, w.sh, s) : launch_bag<CRAG_BF16>(a, w.sh, s);
+    if (one_launch(e.n, e.n_bags, e.dim)) return e.dtype == CRAG_F32 ? launch_bag<CRAG_F32>(a, w.sh, s) : launch_bag<CRAG_BF16>(a, w.sh, s);
     const int rc = e.dtype == CRAG_F32 ? launch_segsum<CRAG_F32, false>(a, w, s) : launch_segsum<CRAG_BF16, false>(a, w, s);
-    return rc ? rc : launch_finish(a, s);
+    if (rc) return rc;
+    if (e.n / a.share / e.n_bags > JOIN_FROM) {
+        const int cols = e.dim % 4 == 0 ? 64 : 16, slabs = (e.dim + cols - 1) / cols;
+        a.joined = 1;
+        if (cols == 64) hipLaunchKernelGGL(k_embed_join<4>, dim3((unsigned)e.n_bags * slabs), dim3(16 * JOIN_RUNS), 0, s, a, slabs);
+        else hipLaunchKernelGGL(k_embed_join<1>, dim3((unsigned)e.n_bags * slabs), dim3(16 * JOIN_RUNS), 0, s, a, slabs);
+    }
+    return launch_finish(a, s);
 }
 
 int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
@@ -1226,8 +1281,8 @@ int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
     b.bag = w.bag;
     b.hist = w.hist;
     if (e.d_table) {
-        b.keys = w.keys[0];
-        b.perm = w.perm[0];
+        b.keys = w.keys;
+        b.pairs = w.pairs[0];
     }
     CragSegArgs a = {};
     a.src = w.dp;
@@ -1263,18 +1318,17 @@ int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
         hipLaunchKernelGGL(k_bwd_start, dim3(tiles + (e.n_bags + 3) / 4), dim3(256), 0, s, b);
         if ((rc = weights())) return rc;
         for (int p = 0; e.d_table && p < passes; ++p) {
-            if (p > 0) hipLaunchKernelGGL(k_sort_count, dim3(tiles), dim3(256), 0, s, w.keys[cur], e.n, p * digit, b.mask, tiles, w.hist);
+            if (p > 0) hipLaunchKernelGGL(k_sort_count, dim3(tiles), dim3(256), 0, s, w.pairs[cur], e.n, p * digit, b.mask, tiles, w.hist);
             hipLaunchKernelGGL(k_sort_prefix, dim3(1 << digit), dim3(256), 0, s, w.hist, tiles, w.total);
-            hipLaunchKernelGGL(k_sort_scatter, dim3(tiles), dim3(256), 0, s, w.keys[cur], p ? w.perm[cur] : (const uint32_t*)nullptr, e.n,
-                               p * digit, digit, tiles, w.hist, w.total, w.keys[cur ^ 1], w.perm[cur ^ 1]);
+            hipLaunchKernelGGL(k_sort_scatter, dim3(tiles), dim3(256), 0, s, w.keys, p ? w.pairs[cur] : (const uint2*)nullptr, e.n, p * digit, digit, tiles,
+                               w.hist, w.total, w.pairs[cur ^ 1]);
             cur ^= 1;
         }
     }
     if ((rc = (int)hipGetLastError()) || !e.d_table) return rc;
     const Walk k = plan_walk(e.n, e.dim, CRAG_F32, w.dp);
     apply(a, k);
-    a.keys = w.keys[cur];
-    a.perm = w.perm[cur];
+    a.pairs = w.pairs[cur];
     a.partial = w.partial;
     a.partial_seg = w.partial_seg;
     a.out = e.d_table;

@@ -237,7 +237,7 @@ int crag_merge_rerank_device(int device, const void* entries_dev, int G, int B, 
  *   weights_dev   [n_tokens], NULL = ones
  *   out_dev       [n_bags][dim], out_dtype float32 or bf16, 16-byte aligned.  Sums are float32 (norms float64); one rounding at the end
  *   coef_dev      [n_bags], may be NULL: what the backward call needs of this one
- * n_tokens < 2^31.  Both calls are asynchronous on `stream`, allocate nothing and may be captured into a graph; everything
+ * n_tokens < 2^31, n_bags <= 2^24.  Both calls are asynchronous on `stream`, allocate nothing and may be captured into a graph; everything
  * they need beside the buffers is in the caller's workspace (crag_embed_workspace bytes, 256-byte aligned; NULL if 0), which belongs to
  * the call until the stream has passed it: calls that can run at once need one each.  They use no atomics on sums: the same
  * inputs give the same bits.

@@ -197,6 +197,29 @@ def test_hashing_embedder_is_a_lookup_in_the_identity():
     assert np.abs(got - want).max() <= 3 * U * np.abs(want).max()     # whole-number sums, one norm and one quotient each
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,dim", [([1024], 384), ([1025], 384), ([4096], 96), ([4097], 96), ([5000], 1536), ([0, 9000, 1, 0, 3], 384), ([2500, 2501], 37),
+                                      ([700] * 9 + [1], 2047), ([1, 30000], 5), ([6000, 0, 6000], 2048)])
+def test_long_bags(lens, dim, dtype):
+    """bags that cross many shares, on both sides of every way the lookup takes"""
+    import torch
+    r = np.random.default_rng(dim)
+    offsets = np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
+    t = int(offsets[-1])
+    ids = r.integers(-3, 300, t).astype(np.int32)
+    w = r.standard_normal(t).astype(np.float32)
+    table = torch.from_numpy(r.standard_normal((290, dim)).astype(np.float32))
+    table = table.bfloat16() if dtype == "bf16" else table
+    case = (table, ids, offsets, w)
+    dev = gpu(*case)
+    for mode, scale, normalize in (("sqrt", 1.0, True), ("mean", -2.0, False)):
+        y, bound = plain(*case, mode, scale, normalize)
+        got = ch.embed_bags(*dev, mode=mode, scale=scale, normalize=normalize)
+        within(got, y, bound)
+        assert torch.equal(got, ch.embed_bags(*dev, mode=mode, scale=scale, normalize=normalize))
+        within(ch.embed_bags(*dev, mode=mode, scale=scale, normalize=normalize, out_dtype=torch.bfloat16), y, bound, bf16=True)
+
+
 def test_positions_outside_every_bag_zero_bags_and_zero_rows():
     import torch
     table = torch.randn((10, 20), device="cuda", requires_grad=True)
