@@ -713,6 +713,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     ScanArgs ga;
     Fp4Args fa = {};
     const float* qres = nullptr;
+    const int many = fp4 && B > h0->n_cus && P.sample_stride <= 8192;
     if (fp4) {
         const bool narrow = !P.mfma || B <= CRAG_FP4_GROUP_Q;
         const int n_blocks = P.mfma ? crag_fp4_query_blocks(B, h0->dim_pad) : (int)gd.size();
@@ -822,6 +823,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         k.B = B;
         k.M = P.M;
         k.tau = tau;
+        k.many = many;
         k.seed_cand = cand;
         k.seed_cnt = segmented ? segcnt : cnt;
         k.seed_n_seg = n_seg;
@@ -860,6 +862,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
                 k1.B = B;
                 k1.M = P.M;
                 k1.tau = tau;
+                k1.many = many;
                 if (segmented) {
                     k1.segcnt = segcnt;
                     k1.n_seg = n_seg;
@@ -884,6 +887,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
             k.B = B;
             k.M = P.M;
             k.tau = tau;
+            k.many = many;
             k.seed_cand = cand;  // later passes continue behind the sample rows
             k.seed_cnt = cnt;
             if (crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
@@ -903,6 +907,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
             k.B = B;
             k.M = P.M;
             k.tau = tau;
+            k.many = many;
             if (crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 1) launch failed");
         }
         if (prof) HIPCHK(hipEventRecord(ws->ev[1], st));
@@ -954,7 +959,9 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     f.top_k = top_k;
     f.symbol_boost = mo ? mo->symbol_boost : 0.0;
     f.qmap = nullptr;
+    f.many = many;
     if ((rc = crag_launch_finalize(f, st))) return fail(CRAG_E_HIP, "finalize launch failed");
+    f.many = 0;
     f.out_ids = nullptr;  // the fallback tiers patch entries; the rerank then runs once more, over all of them
     auto merge = [&]() -> int {
         if (!mo) return 0;

@@ -182,6 +182,7 @@ struct KthArgs {
     long long seed_stride;
     // > 0: src is the tile-major sample of crag_launch_scan_q16 with this Bpad (q_stride, e_stride, off0 unused)
     long long tile_bpad;
+    int many;  // 4-bit rows (samples of at most 8192), more queries than CUs: blocks of 256 threads
 };
 int crag_launch_kth(const KthArgs& a, hipStream_t s);
 struct FinalizeArgs {
@@ -209,6 +210,7 @@ struct FinalizeArgs {
     int top_k;
     double symbol_boost;
     const int* qmap;                  // null: block b serves query b; else block b serves query qmap[b] (fallback passes)
+    int many;                         // 4-bit rows, more queries than CUs, trusted == 0: smaller blocks
 };
 int crag_launch_finalize(const FinalizeArgs& a, hipStream_t s);
 int crag_launch_merge_rerank(const CragEntry* entries, int G, int B, int kc, int top_k, double symbol_boost,

@@ -62,33 +62,30 @@ __global__ __launch_bounds__(256) void k_row_norms(const uint4* __restrict__ row
 }
 
 // ----------------------------------------------------------------------------------------
-// Block-wide selection (1024 threads) over n 32-bit keys read through key(i).  Returns, to every thread,
-// a key T with at least want + 1 keys <= T: the exact want-th smallest (0-based, want < n) unless the
-// histogram bin that holds it is crowded (> KTH_LIST keys, e.g. all keys equal), in which case T is that
-// bin's upper edge.  Selection, not sorting: min/max, a 2048-bin histogram of (key - min) >> shift, a
-// block scan to the bin that holds the wanted rank, then the exact rank inside that bin (sparse when the
-// wanted key sits in the tail of the score distribution, as it does here).
+// Block-wide selection by T threads over 32-bit keys: `each(f)` calls f(key) for every key that this thread has.  Returns, to
+// every thread, the want-th smallest (0-based, want below the number of keys).  Selection, not sorting: min/max, a 2048-bin
+// histogram of (key - min) >> shift, a block scan to the bin that holds the wanted rank, and the exact rank among that bin's
+// few keys.  A bin of more than KTH_LIST keys is cut into bins of its own first (1024 queries, 8192 keys each: 96 us with up to
+// 1024 keys ranked against each other, for the sake of a few queries whose keys are uneven).
 // scratch: KTH_SCRATCH 32-bit words of LDS; the caller's LDS writes of the keys must be fenced by the caller.
-// 2048 bins: k_kth then needs 64 KiB of keys + 12.2 KiB of scratch = under half a CU's LDS, so two of its
-// 1024-thread blocks share a CU (a batch of 1024 queries runs its selections in two rounds instead of four)
 constexpr int KTH_BINS = 2048;
 constexpr int KTH_BITS = 11;
-constexpr int KTH_LIST = 1024;
+constexpr int KTH_LIST = 64;
 constexpr int KTH_SCRATCH = KTH_BINS + KTH_LIST + 48 + 4;
-template <typename KeyFn>
-__device__ __forceinline__ uint32_t block_select(KeyFn key, int n, uint32_t want, uint32_t* scratch) {
+template <int T, typename Each>
+__device__ __forceinline__ uint32_t block_select(Each each, uint32_t want, uint32_t* scratch) {
+    constexpr int W = T / 64, OWN = KTH_BINS / T;
     uint32_t* hist = scratch;              // [KTH_BINS]
     uint32_t* list = hist + KTH_BINS;      // [KTH_LIST]
     uint32_t* wsum = list + KTH_LIST;      // [48] wave totals, wave minima, wave maxima
-    uint32_t* ctl = wsum + 48;             // [4]: bin, rank inside the bin, list length, result
+    uint32_t* ctl = wsum + 48;             // [4]: bin, rank inside the bin, list length, keys in the bin; then the result
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     uint32_t mn = 0xffffffffu, mx = 0u;
-    for (int i = tid; i < n; i += 1024) {
-        const uint32_t k = key(i);
+    each([&](uint32_t k) {
         mn = k < mn ? k : mn;
         mx = k > mx ? k : mx;
-    }
-    for (int i = tid; i < KTH_BINS; i += 1024) hist[i] = 0;
+    });
+    for (int i = tid; i < KTH_BINS; i += T) hist[i] = 0;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         const uint32_t o1 = __shfl_xor(mn, off), o2 = __shfl_xor(mx, off);
@@ -104,62 +101,86 @@ __device__ __forceinline__ uint32_t block_select(KeyFn key, int n, uint32_t want
     mn = wsum[16];
     mx = wsum[32];
 #pragma unroll
-    for (int w = 1; w < 16; ++w) {
+    for (int w = 1; w < W; ++w) {
         mn = wsum[16 + w] < mn ? wsum[16 + w] : mn;
         mx = wsum[32 + w] > mx ? wsum[32 + w] : mx;
     }
     const uint32_t range = mx - mn;
     const int bits = range ? 32 - __builtin_clz(range) : 0;
-    const int shift = bits > KTH_BITS ? bits - KTH_BITS : 0;  // (key - mn) >> shift < KTH_BINS
-    for (int i = tid; i < n; i += 1024) atomicAdd(&hist[(key(i) - mn) >> shift], 1u);
-    __syncthreads();
-    // exclusive scan over the bins: thread t owns bins 2t and 2t+1
-    const uint32_t h0 = hist[2 * tid], h1 = hist[2 * tid + 1];
-    const uint32_t mine = h0 + h1;
-    uint32_t inc = mine;
+    int shift = bits > KTH_BITS ? bits - KTH_BITS : 0;  // (key - mn) >> shift < KTH_BINS
+    uint32_t lo = mn;
+    for (;;) {
+        each([&](uint32_t k) {
+            if (k >= lo && ((k - lo) >> shift) < (uint32_t)KTH_BINS) atomicAdd(&hist[(k - lo) >> shift], 1u);
+        });
+        __syncthreads();
+        // exclusive scan over the bins: thread t owns bins OWN t .. OWN t + OWN - 1
+        uint32_t h[OWN], mine = 0;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = __shfl_up(inc, off);
-        if (lane >= off) inc += o;
-    }
-    if (lane == 63) wsum[wv] = inc;
-    __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < wv; ++w) base += wsum[w];
-    const uint32_t exc = base + inc - mine;
-    const uint32_t M = want + 1;
-    if (exc < M && M <= exc + mine) {  // exactly one thread: the wanted key is in one of its bins
-        uint32_t e = exc;
-        int bsel = 2 * tid;
-        if (e + h0 < M) { e += h0; ++bsel; }
-        ctl[0] = (uint32_t)bsel;
-        ctl[1] = M - e - 1;  // rank of the wanted key inside bin bsel
-    }
-    __syncthreads();
-    const uint32_t bsel = ctl[0], rank = ctl[1];
-    for (int i = tid; i < n; i += 1024) {
-        const uint32_t k = key(i);
-        if (((k - mn) >> shift) == bsel) {
-            const uint32_t p = atomicAdd(&ctl[2], 1u);
-            if (p < KTH_LIST) list[p] = k;
+        for (int o = 0; o < OWN; ++o) {
+            h[o] = hist[OWN * tid + o];
+            mine += h[o];
         }
-    }
-    __syncthreads();
-    const uint32_t L = ctl[2];
-    if (L > KTH_LIST) {  // crowded bin: its upper edge is a valid (looser) answer
-        if (tid == 0) {
-            const unsigned long long edge = (unsigned long long)mn + (((unsigned long long)bsel + 1) << shift) - 1;
-            ctl[3] = edge > mx ? mx : (uint32_t)edge;
+        uint32_t inc = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t o = __shfl_up(inc, off);
+            if (lane >= off) inc += o;
         }
-    } else if (tid < (int)L) {
-        const uint32_t k = list[tid];
+        if (lane == 63) wsum[wv] = inc;
+        __syncthreads();
+        uint32_t base = 0;
+#pragma unroll
+        for (int w = 0; w < W - 1; ++w) base += w < wv ? wsum[w] : 0u;
+        const uint32_t exc = base + inc - mine;
+        if (exc <= want && want < exc + mine) {  // exactly one thread: the wanted key is in one of its bins
+            uint32_t e = exc, in = h[0];
+            int o = 0;
+#pragma unroll
+            for (int j = 0; j < OWN - 1; ++j)
+                if (o == j && e + h[j] <= want) {
+                    e += h[j];
+                    in = h[j + 1];
+                    ++o;
+                }
+            ctl[0] = (uint32_t)(OWN * tid + o);
+            ctl[1] = want - e;  // rank of the wanted key inside its bin
+            ctl[3] = in;
+        }
+        __syncthreads();
+        lo += ctl[0] << shift;
+        want = ctl[1];
+        const uint32_t in = ctl[3];
+        if (shift == 0) {  // a bin is one value
+            __syncthreads();  // scratch may be reused at once
+            return lo;
+        }
+        if (in <= (uint32_t)KTH_LIST) break;
+        shift = shift > KTH_BITS ? shift - KTH_BITS : 0;
+        for (int i = tid; i < KTH_BINS; i += T) hist[i] = 0;
+        __syncthreads();
+    }
+    each([&](uint32_t k) {
+        if (k >= lo && ((k - lo) >> shift) == 0u) list[atomicAdd(&ctl[2], 1u)] = k;
+    });
+    __syncthreads();
+    constexpr int LANES = T / KTH_LIST;  // per item of the list
+    const int L = (int)ctl[2], i = tid / LANES;
+    if (i < L) {
+        const uint32_t k = list[i];
         uint32_t lt = 0, eq = 0;
-        for (uint32_t j = 0; j < L; ++j) {
+#pragma unroll
+        for (int u = 0; u < KTH_LIST / LANES; ++u) {
+            const int j = u * LANES + tid % LANES;
             const uint32_t o = list[j];
-            lt += o < k ? 1u : 0u;
-            eq += o == k ? 1u : 0u;
+            lt += j < L && o < k ? 1u : 0u;
+            eq += j < L && o == k ? 1u : 0u;
         }
-        if (lt <= rank && rank < lt + eq) ctl[3] = k;  // duplicates write the same value
+        for (int o = 1; o < LANES; o <<= 1) {
+            lt += __shfl_xor(lt, o);
+            eq += __shfl_xor(eq, o);
+        }
+        if (lt <= want && want < lt + eq) ctl[3] = k;  // duplicates write the same value
     }
     __syncthreads();
     const uint32_t r = ctl[3];
@@ -169,13 +190,24 @@ __device__ __forceinline__ uint32_t block_select(KeyFn key, int n, uint32_t want
 
 // Segmented candidate buffer (MfmaArgs in crag_common.h): exclusive prefix of the per-segment counts of one
 // query into segoff[0 .. n_seg] (LDS), returns the total; *overflow if a segment ran over.  n_seg <= 1024.
+template <int T>
 __device__ __forceinline__ int block_seg_offsets(const uint32_t* __restrict__ segcnt_q, int n_seg, int seg_cap,
                                                  uint32_t* segoff, uint32_t* wsum, bool* overflow) {
+    constexpr int W = T / 64, OWN = 1024 / T;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    uint32_t c = tid < n_seg ? segcnt_q[tid] : 0u;
-    const bool ov = c > (uint32_t)seg_cap;
-    c = ov ? (uint32_t)seg_cap : c;
-    uint32_t inc = c;
+    uint32_t c[OWN], mine = 0;
+    bool ov = false;
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) c[o] = OWN * tid + o < n_seg ? segcnt_q[OWN * tid + o] : 0u;
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+        if (c[o] > (uint32_t)seg_cap) {
+            ov = true;
+            c[o] = (uint32_t)seg_cap;
+        }
+        mine += c[o];
+    }
+    uint32_t inc = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const uint32_t o = __shfl_up(inc, off);
@@ -183,10 +215,16 @@ __device__ __forceinline__ int block_seg_offsets(const uint32_t* __restrict__ se
     }
     if (lane == 63) wsum[wv] = inc;
     const int any_ov = __syncthreads_or(ov ? 1 : 0);
-    uint32_t base = 0;
-    for (int w = 0; w < wv; ++w) base += wsum[w];
-    if (tid < n_seg) segoff[tid] = base + inc - c;
-    if (tid == n_seg - 1) segoff[n_seg] = base + inc;
+    uint32_t at = inc - mine;
+#pragma unroll
+    for (int w = 0; w < W - 1; ++w) at += w < wv ? wsum[w] : 0u;
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+        const int i = OWN * tid + o;
+        if (i < n_seg) segoff[i] = at;
+        at += c[o];
+        if (i == n_seg - 1) segoff[n_seg] = at;
+    }
     __syncthreads();
     *overflow = any_ov != 0;
     return (int)segoff[n_seg];
@@ -211,23 +249,26 @@ __device__ __forceinline__ void kth_seed(const KthArgs& a, int q, uint32_t j, ui
         a.seed_cand[(long long)q * CRAG_CAND_CAP + j] = e;
     }
 }
-// ... and publishes how many there are (all threads of the block call this)
+// ... and publishes how many there are (all T threads of the block call this)
+template <int T>
 __device__ __forceinline__ void kth_seed_counts(const KthArgs& a, int q, uint32_t total) {
     const uint32_t tid = threadIdx.x;
     if (a.seed_n_seg > 0) {
         const uint32_t ns = (uint32_t)a.seed_n_seg;
-        for (uint32_t sg = tid; sg < ns; sg += 1024) a.seed_cnt[(long long)q * ns + sg] = total > sg ? (total - sg + ns - 1) / ns : 0u;
+        for (uint32_t sg = tid; sg < ns; sg += T) a.seed_cnt[(long long)q * ns + sg] = total > sg ? (total - sg + ns - 1) / ns : 0u;
     } else if (tid == 0) {
         a.seed_cnt[CRAG_CNT(q)] = total;
     }
 }
 
 // per query: tau = score of the M-th smallest ordered key of a strided list (KthArgs in crag_common.h);
-// any tau >= the true M-th smallest keeps the cascade exact (see block_select for when it is looser)
-__global__ __launch_bounds__(1024) void k_kth(KthArgs a) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    uint32_t* keys = (uint32_t*)smem;                        // [CRAG_CAND_CAP]
-    uint32_t* scratch = keys + CRAG_CAND_CAP;                // [KTH_SCRATCH]
+// any tau >= the true M-th smallest keeps the cascade exact
+// T threads hold PER keys each.  A list of more than T * PER is cut (its M-th smallest is no smaller than the whole one's); a
+// sample that seeds is never longer.
+template <int T, int PER>
+__global__ __launch_bounds__(T) void k_kth(KthArgs a) {
+    __shared__ uint32_t scratch[KTH_SCRATCH];
+    __shared__ uint32_t seg_off[1024 + 1];
     const int q = blockIdx.x;
     const int tid = threadIdx.x;
     const bool seg = a.n_seg > 0;
@@ -235,9 +276,10 @@ __global__ __launch_bounds__(1024) void k_kth(KthArgs a) {
     long long n;
     if (seg) {
         bool ov;  // an overflowed segment still holds seg_cap rows <= the old tau
-        n = block_seg_offsets(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, scratch, scratch + KTH_BINS + KTH_LIST, &ov);
+        n = block_seg_offsets<T>(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, seg_off, scratch, &ov);
         if (n > CRAG_CAND_CAP) n = CRAG_CAND_CAP;  // the first CAP gathered rows are all <= the old tau
-        if (!a.qd[q].keep_mid && tid < a.n_seg) a.segcnt[(long long)q * a.n_seg + tid] = 0;
+        if (!a.qd[q].keep_mid)
+            for (int i = tid; i < a.n_seg; i += T) a.segcnt[(long long)q * a.n_seg + i] = 0;
     } else if (from_cand) {
         const unsigned int c = a.cnt[CRAG_CNT(q)];
         n = c < CRAG_CAND_CAP ? c : CRAG_CAND_CAP;  // an overflowed buffer still holds CAP rows <= the old tau
@@ -258,38 +300,37 @@ __global__ __launch_bounds__(1024) void k_kth(KthArgs a) {
     if (n < (long long)a.M || (!from_cand && n == (long long)a.M)) {
         if (!from_cand && tid == 0) a.tau[q] = __builtin_inff();  // every row is a candidate
         if (!from_cand && a.seed_cand) {                           // ... and every sample row is seeded
-            for (int i = tid; i < (int)n; i += 1024)
+            for (int i = tid; i < (int)n; i += T)
                 kth_seed(a, q, (uint32_t)i, src_at(i), (uint32_t)i);
             __syncthreads();
-            kth_seed_counts(a, q, (uint32_t)n);
+            kth_seed_counts<T>(a, q, (uint32_t)n);
         }
         return;                                                    // from_cand: keep the looser tau
     }
-    // four loads in flight per thread: one after the other they would cost a trip to memory each
-    for (int i0 = tid; i0 < (int)n; i0 += 4 * 1024) {
-        uint32_t k[4];
+    const int len = n < T * PER ? (int)n : T * PER;
+    uint32_t keys[PER];  // of positions tid + u T; all loads in flight at once
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * 1024;
-            if (i < (int)n) k[u] = src_at(seg ? seg_slot(scratch, a.n_seg, a.seg_cap, i) : i);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i0 + u * 1024 < (int)n) keys[i0 + u * 1024] = k[u];
+    for (int u = 0; u < PER; ++u) {
+        const int i = tid + u * T;
+        keys[u] = 0u;
+        if (i < len) keys[u] = src_at(seg ? seg_slot(seg_off, a.n_seg, a.seg_cap, i) : i);
     }
-    __syncthreads();
-    const uint32_t t = block_select([&](int i) { return keys[i]; }, (int)n, (uint32_t)a.M - 1u, scratch);
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+            if (tid + u * T < len) f(keys[u]);
+    };
+    const uint32_t t = block_select<T>(each, (uint32_t)a.M - 1u, scratch);
     if (tid == 0) a.tau[q] = crag_fkey_inv(t);
     if (!from_cand && a.seed_cand) {  // sample row i IS row i of the collection; n <= 16384 = CRAG_CAND_CAP
         uint32_t* seed_total = scratch;  // block_select is done with its scratch
         if (tid == 0) *seed_total = 0;
         __syncthreads();
-        for (int i = tid; i < (int)n; i += 1024) {
-            const uint32_t k = keys[i];
-            if (k <= t) kth_seed(a, q, atomicAdd(seed_total, 1u), k, (uint32_t)i);
-        }
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+            if (tid + u * T < len && keys[u] <= t) kth_seed(a, q, atomicAdd(seed_total, 1u), keys[u], (uint32_t)(tid + u * T));
         __syncthreads();
-        kth_seed_counts(a, q, *seed_total);
+        kth_seed_counts<T>(a, q, *seed_total);
     }
 }
 
@@ -432,8 +473,9 @@ __device__ __forceinline__ int count_before(int n, int part, int lanes, Before b
     for (int o = 1; o < lanes; o <<= 1) r += __shfl_xor(r, o);
     return r;
 }
-// lanes per item so that a block of 1024 threads has all of them at work on n items
-__device__ __forceinline__ int lanes_per_item(int n) { return n <= 64 ? 16 : (n <= 128 ? 8 : (n <= 256 ? 4 : (n <= 512 ? 2 : 1))); }
+// lanes per item so that a block of T threads has all of them at work on n items
+template <int T>
+__device__ __forceinline__ int lanes_per_item(int n) { return n <= T / 16 ? 16 : (n <= T / 8 ? 8 : (n <= T / 4 ? 4 : (n <= T / 2 ? 2 : 1))); }
 
 // hybrid_search.py:82,99-121: base score of a distance, times the path's and the symbol's factor
 __device__ __forceinline__ double rerank_score(float dist, uint32_t f, double symbol_boost) {
@@ -445,10 +487,15 @@ __device__ __forceinline__ double rerank_score(float dist, uint32_t f, double sy
 }
 
 constexpr int FIN_GATHER = 2048;  // candidates that survive the selection cut (m + 1 plus score ties), else sort all
-__global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
+// T threads, KEYS candidates in LDS.  1024 threads with room for every candidate serve any call; batches of more queries than CUs
+// on 4-bit rows take 512 threads with less room, two blocks a CU: one selects while the other waits for its rows.
+template <int T, int KEYS>
+__global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
+    constexpr bool ALL = KEYS == CRAG_CAND_CAP;
+    const bool fp4 = !ALL || a.dtype == CRAG_FP4;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    unsigned long long* skeys = (unsigned long long*)smem;                            // [CRAG_CAND_CAP]
-    unsigned long long* ekeys = skeys + CRAG_CAND_CAP;                                // [CRAG_MAX_M]
+    unsigned long long* skeys = (unsigned long long*)smem;                            // [KEYS]
+    unsigned long long* ekeys = skeys + KEYS;                                // [CRAG_MAX_M]
     double* red = (double*)(ekeys + CRAG_MAX_M);                                      // [16]
     uint32_t* sel_scratch = (uint32_t*)(red + 16);                                    // [KTH_SCRATCH]
     uint32_t* sel_count = sel_scratch + KTH_SCRATCH;                                  // [4]
@@ -461,7 +508,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     int c;
     if (seg) {
         bool ov;
-        c = block_seg_offsets(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, seg_off, sel_scratch, &ov);
+        c = block_seg_offsets<T>(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, seg_off, sel_scratch, &ov);
         if (ov || c > CRAG_CAND_CAP) status = CRAG_ST_OVERFLOW;
         if (c > CRAG_CAND_CAP) c = CRAG_CAND_CAP;
     } else {
@@ -477,17 +524,29 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     // candidates whose score is <= the (m + 1)-th smallest score (selection), and only those are sorted.
     int c_sorted = c;
     if (c > 256) {
-        for (int i = tid; i < c; i += 1024) skeys[i] = cand_at(i);
+        const bool held = ALL || c <= KEYS - FIN_GATHER;  // (else every pass reads them where they lie)
+        if (held) {
+            for (int i0 = tid; i0 < c; i0 += 4 * T) {  // four loads in flight
+                unsigned long long k[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i0 + u * T < c) k[u] = cand_at(i0 + u * T);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i0 + u * T < c) skeys[i0 + u * T] = k[u];
+            }
+        }
         __syncthreads();
+        auto key_at = [&](int i) { return held ? skeys[i] : cand_at(i); };
         const uint32_t want = (uint32_t)(m < c ? m : c - 1);
-        const uint32_t t = block_select([&](int i) { return (uint32_t)(skeys[i] >> 32); }, c, want, sel_scratch);
+        const uint32_t t = block_select<T>([&](auto f) { for (int i = tid; i < c; i += T) f((uint32_t)(key_at(i) >> 32)); }, want, sel_scratch);
         // compact in place is not possible without a second buffer: gather into the tail region of skeys
-        unsigned long long* gathered = skeys + CRAG_CAND_CAP - FIN_GATHER;
+        unsigned long long* gathered = skeys + KEYS - FIN_GATHER;
         if (tid == 0) *sel_count = 0;
         __syncthreads();
-        if (c <= CRAG_CAND_CAP - FIN_GATHER) {
-            for (int i = tid; i < c; i += 1024) {
-                const unsigned long long k = skeys[i];
+        if (!ALL || c <= KEYS - FIN_GATHER) {
+            for (int i = tid; i < c; i += T) {
+                const unsigned long long k = key_at(i);
                 if ((uint32_t)(k >> 32) <= t) {
                     const uint32_t p = atomicAdd(sel_count, 1u);
                     if (p < FIN_GATHER) gathered[p] = k;
@@ -497,32 +556,44 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         __syncthreads();
         const uint32_t L = *sel_count;
         __syncthreads();
-        if (c <= CRAG_CAND_CAP - FIN_GATHER && L <= FIN_GATHER) {  // L >= want + 1 by construction
-            for (int i = tid; i < (int)L; i += 1024) skeys[i] = gathered[i];  // FIN_GATHER <= CAP / 2: no overlap
-            c_sorted = (int)L;
+        if ((!ALL || c <= KEYS - FIN_GATHER) && (L <= FIN_GATHER || !held)) {  // L >= want + 1 by construction
+            const int kept = L <= FIN_GATHER ? (int)L : FIN_GATHER;
+            for (int i = tid; i < kept; i += T) skeys[i] = gathered[i];  // FIN_GATHER <= KEYS / 2: no overlap
+            c_sorted = kept;
+            if (L > FIN_GATHER) status = CRAG_ST_OVERFLOW;  // more ties than fit: the fallback's business
             __syncthreads();
         }
     } else {
-        for (int i = tid; i < c; i += 1024) skeys[i] = cand_at(i);
+        for (int i = tid; i < c; i += T) skeys[i] = cand_at(i);
     }
     __syncthreads();
     if (c_sorted <= 1024) {
         // rank by counting (keys are unique: the row id is part of the key): the lanes read the same few LDS
         // words at a time, two barriers in all -- a bitonic network of this size costs 21-55
-        const int lanes = lanes_per_item(c_sorted), i = tid / lanes, part = tid % lanes;  // c_sorted * lanes <= 1024
-        unsigned long long k = ~0ull;
-        int rank = 0;
-        if (i < c_sorted) {
-            k = skeys[i];
-            rank = count_before(c_sorted, part, lanes, [&](int j) { return skeys[j] < k; });
+        constexpr int ITEMS = 1024 / T;
+        const int lanes = lanes_per_item<T>(c_sorted), part = tid % lanes;  // c_sorted * lanes <= T, or one lane and ITEMS each
+        unsigned long long k[ITEMS];
+        int rank[ITEMS];
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int i = tid / lanes + it * T;
+            k[it] = ~0ull;
+            rank[it] = 0;
+            if (i < c_sorted) {
+                const unsigned long long mine = skeys[i];
+                k[it] = mine;
+                rank[it] = count_before(c_sorted, part, lanes, [&](int j) { return skeys[j] < mine; });
+            }
         }
         __syncthreads();
-        if (i < c_sorted && part == 0) skeys[rank] = k;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it)
+            if (tid / lanes + it * T < c_sorted && part == 0) skeys[rank[it]] = k[it];
         __syncthreads();
     } else {
         int P = 2048;
         while (P < c_sorted) P <<= 1;
-        for (int i = c_sorted + tid; i < P; i += 1024) skeys[i] = ~0ull;
+        for (int i = c_sorted + tid; i < P; i += T) skeys[i] = ~0ull;
         __syncthreads();
         bitonic_sort_u64(skeys, P);
     }
@@ -532,7 +603,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     // |q|^2 in fp64 (error bound only)
     {
         double part = 0.0;
-        for (int d = tid; d < a.dim; d += blockDim.x) {
+        for (int d = tid; d < a.dim; d += T) {
             const double v = load_elem_f64(qv, a.dtype, d);
             part += v * v;
         }
@@ -542,7 +613,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         __syncthreads();
         if (tid == 0) {
             double s = 0.0;
-            for (int k = 0; k < (int)(blockDim.x >> 6); ++k) s += red[k];
+            for (int k = 0; k < T / 64; ++k) s += red[k];
             red[0] = s;
         }
         __syncthreads();
@@ -552,7 +623,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         // a query with a NaN or an infinite component (or a norm beyond float64) has no nearest neighbours: no results,
         // nothing for the fallback tiers to settle.  (The reference cannot get here: its queries come out of the embedder.)
         CragEntry* o = a.entries + (long long)q * a.kc;
-        for (int i = tid; i < a.kc; i += blockDim.x) {
+        for (int i = tid; i < a.kc; i += T) {
             CragEntry e;
             e.dist = __builtin_inff();
             e.flags = 0;
@@ -561,7 +632,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
         }
         if (tid == 0) a.status[q] = CRAG_ST_OK;
         if (a.out_ids) {
-            for (int j = tid; j < a.top_k; j += blockDim.x) {
+            for (int j = tid; j < a.top_k; j += T) {
                 a.out_ids[(long long)q * a.top_k + j] = -1;
                 a.out_scores[(long long)q * a.top_k + j] = 0.0;
                 a.out_dist[(long long)q * a.top_k + j] = __builtin_inff();
@@ -577,15 +648,15 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     {
         unsigned char* stage_q = (unsigned char*)(skeys + 1024);  // m + 1 <= CRAG_MAX_M + 1 <= 1024 keys stay live
         const int row_bytes = a.dim_pad * (int)esz, chunks = row_bytes >> 4;
-        const int q_bytes = a.dtype == CRAG_FP4 ? a.dim_pad * 8 : 4096;  // of 4-bit rows only the query is staged, as float64
+        const int q_bytes = fp4 ? a.dim_pad * 8 : 4096;  // of 4-bit rows only the query is staged, as float64
         unsigned char* stage_r = stage_q + q_bytes;
-        int rpr = (int)((sizeof(unsigned long long) * (CRAG_CAND_CAP - 1024) - q_bytes) / (size_t)row_bytes);
-        if (rpr > 128) rpr = 128;  // 1024 threads / 8 lanes
-        if (a.dtype == CRAG_FP4) rpr = 256;  // read where they lie, by four lanes
-        if (a.dtype == CRAG_FP4) {
-            for (int d = tid; d < a.dim_pad; d += 1024) ((double*)stage_q)[d] = (double)((const float*)qv)[d];
+        int rpr = (int)((sizeof(unsigned long long) * (KEYS - 1024) - q_bytes) / (size_t)row_bytes);
+        if (rpr > T / 8) rpr = T / 8;  // eight lanes a row
+        if (fp4) rpr = T / 4;          // read where they lie, by four lanes
+        if (fp4) {
+            for (int d = tid; d < a.dim_pad; d += T) ((double*)stage_q)[d] = (double)((const float*)qv)[d];
         } else {
-            for (int c = tid; c < chunks; c += 1024) ((uint4*)stage_q)[c] = ((const uint4*)qv)[c];
+            for (int c = tid; c < chunks; c += T) ((uint4*)stage_q)[c] = ((const uint4*)qv)[c];
         }
         for (int base = 0; base < m; base += rpr) {
             const int nr = m - base < rpr ? m - base : rpr;
@@ -594,13 +665,13 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             // which makes it a generic pointer to the compiler, and FLAT loads are waited for one at a time
             typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
             const __attribute__((address_space(1))) u32x4_t* grows = (const __attribute__((address_space(1))) u32x4_t*)D.rows;
-            if (a.dtype != CRAG_FP4) {
+            if (!fp4) {
                 const int total = nr * chunks;
-                for (int idx0 = tid; idx0 < total; idx0 += 4 * 1024) {
+                for (int idx0 = tid; idx0 < total; idx0 += 4 * T) {
                     u32x4_t v[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int idx = idx0 + u * 1024;
+                        const int idx = idx0 + u * T;
                         if (idx < total) {
                             const int r = idx / chunks, c = idx - r * chunks;
                             const uint32_t row = (uint32_t)(skeys[base + r] & 0xffffffffull);
@@ -609,15 +680,15 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
                     }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const int idx = idx0 + u * 1024;
+                        const int idx = idx0 + u * T;
                         if (idx < total) ((u32x4_t*)stage_r)[idx] = v[u];
                     }
                 }
             }
             __syncthreads();
-            const int lanes = a.dtype == CRAG_FP4 ? 4 : 8, r = tid / lanes, j = tid % lanes;
+            const int lanes = fp4 ? 4 : 8, r = tid / lanes, j = tid % lanes;
             double acc = 0.0;
-            if (a.dtype == CRAG_FP4) {
+            if (fp4) {
                 if (r < nr)
                     acc = canon_fp4(D.rows, (const double*)stage_q, a.dim, a.dim_pad, (long long)(uint32_t)(skeys[base + r] & 0xffffffffull), j, a.metric);
             } else {
@@ -641,7 +712,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     float* rr_dist = (float*)(rr_row + CRAG_MAX_KC);   // [CRAG_MAX_KC]
     double* rr_score = (double*)(rr_dist + CRAG_MAX_KC);  // [CRAG_MAX_KC], negative: not kept
     if (tid == 0) n_keep = 0;
-    const int m_lanes = lanes_per_item(m);  // m <= CRAG_MAX_M: every item has its lanes at once
+    const int m_lanes = lanes_per_item<T>(m);  // m <= CRAG_MAX_M: every item has its lanes at once
     if (tid / m_lanes < m) {
         const unsigned long long k = ekeys[tid / m_lanes];
         const int rank = count_before(m, tid % m_lanes, m_lanes, [&](int t) { return ekeys[t] < k; });
@@ -678,7 +749,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
             }
         }
     }
-    for (int i = kc_valid + tid; i < a.kc; i += blockDim.x) {
+    for (int i = kc_valid + tid; i < a.kc; i += T) {
         CragEntry e;
         e.dist = __builtin_inff();
         e.flags = 0;
@@ -724,7 +795,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     if (!a.out_ids) return;
     // R5 (hybrid_search.py:120-125) of a single shard, whose entries are in order already: strict > 0.01 filter, stable
     // descending sort by counting, top_k
-    const int r_lanes = lanes_per_item(kc_valid), j = tid / r_lanes;
+    const int r_lanes = lanes_per_item<T>(kc_valid), j = tid / r_lanes;
     if (j < kc_valid && rr_score[j] >= 0.0) {
         const double s = rr_score[j];
         const int rank = count_before(kc_valid, tid % r_lanes, r_lanes, [&](int t) { return rr_score[t] > s || (rr_score[t] == s && t < j); });
@@ -737,7 +808,7 @@ __global__ __launch_bounds__(1024) void k_finalize(FinalizeArgs a) {
     }
     __syncthreads();
     const int nk = (int)n_keep < a.top_k ? (int)n_keep : a.top_k;
-    for (int j = nk + tid; j < a.top_k; j += blockDim.x) {
+    for (int j = nk + tid; j < a.top_k; j += T) {
         a.out_ids[(long long)q * a.top_k + j] = -1;
         a.out_scores[(long long)q * a.top_k + j] = 0.0;
         a.out_dist[(long long)q * a.top_k + j] = __builtin_inff();
@@ -839,7 +910,7 @@ __global__ __launch_bounds__(1024) void k_rescore_wide(FinalizeArgs a, unsigned 
     int c;
     if (seg) {
         bool ov;
-        c = block_seg_offsets(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, seg_off, wsum, &ov);
+        c = block_seg_offsets<1024>(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, seg_off, wsum, &ov);
     } else {
         c = (int)a.cnt[CRAG_CNT(q)];
     }
@@ -1093,20 +1164,21 @@ int crag_launch_row_norms(const void* rows, int dtype, int dim_pad, long long n,
 }
 
 int crag_launch_kth(const KthArgs& a, hipStream_t s) {
-    const size_t lds = sizeof(uint32_t) * (CRAG_CAND_CAP + KTH_SCRATCH);
-    static std::atomic<uint64_t> lds_ok;
-    crag_allow_dynamic_lds((const void*)k_kth, lds, lds_ok);
-    hipLaunchKernelGGL(k_kth, dim3(a.B), dim3(1024), lds, s, a);
+    if (a.many) hipLaunchKernelGGL((k_kth<256, 32>), dim3(a.B), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_kth<1024, CRAG_CAND_CAP / 1024>), dim3(a.B), dim3(1024), 0, s, a);
     return (int)hipGetLastError();
 }
 
-int crag_launch_finalize(const FinalizeArgs& a, hipStream_t s) {
-    const size_t lds = sizeof(unsigned long long) * (CRAG_CAND_CAP + CRAG_MAX_M) + sizeof(double) * 16 +
-                       sizeof(uint32_t) * (KTH_SCRATCH + 4 + 1024 + 4);
+template <int T, int KEYS>
+static int launch_finalize(const FinalizeArgs& a, hipStream_t s) {
+    const size_t lds = sizeof(unsigned long long) * (KEYS + CRAG_MAX_M) + sizeof(double) * 16 + sizeof(uint32_t) * (KTH_SCRATCH + 4 + 1024 + 4);
     static std::atomic<uint64_t> lds_ok;
-    crag_allow_dynamic_lds((const void*)k_finalize, lds, lds_ok);
-    hipLaunchKernelGGL(k_finalize, dim3(a.B), dim3(1024), lds, s, a);
+    crag_allow_dynamic_lds((const void*)k_finalize<T, KEYS>, lds, lds_ok);
+    hipLaunchKernelGGL((k_finalize<T, KEYS>), dim3(a.B), dim3(T), lds, s, a);
     return (int)hipGetLastError();
+}
+int crag_launch_finalize(const FinalizeArgs& a, hipStream_t s) {
+    return a.many ? launch_finalize<512, 6144>(a, s) : launch_finalize<1024, CRAG_CAND_CAP>(a, s);
 }
 
 int crag_launch_merge_rerank(const CragEntry* entries, int G, int B, int kc, int top_k, double symbol_boost,
