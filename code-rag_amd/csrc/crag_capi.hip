@@ -404,7 +404,7 @@ LevelBounds cascade_bounds(long long N, long long n0, int M, bool fp4 = false) {
     static const double r_large = [] { const char* e = getenv("CRAG_CASCADE_R100"); return e && atof(e) > 1.1 ? atof(e) : 3.0; }();
     // 4-bit rows are read four times as fast, so a level weighs more against its survivors (same box: 256 queries x 1M x 768,
     // top 10: r = 4 / 6 / 12 318 / 300 / 289 us; 1024 x 300k x 1024, top 100: r = 2.5 / 3.7 808 / 775 us)
-    int L = (int)std::ceil(std::log(R) / std::log(fp4 ? (M > 128 ? 3.7 : 12.0) : M > 64 ? r_large : r_small));  // (the two variables: same-box sweeps only)
+    int L = (int)std::ceil(std::log(R) / std::log(fp4 ? (M > 128 ? 6.5 : 12.0) : M > 64 ? r_large : r_small));  // (the two variables: same-box sweeps only)
     L = std::max(1, std::min(L, L_MAX));
     auto est = [&](int l) { return (double)l * (double)M * std::pow(R, 1.0 / l); };
     while (L < L_MAX && est(L) > 0.75 * CRAG_CAND_CAP && est(L + 1) < est(L)) ++L;
@@ -540,7 +540,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     P.kc = 2 * top_k;  // hybrid_search.py:62
     // slack rows behind the 2*top_k-th: what the certificate may lose to approximate-score misordering before a
     // query has to take the exact fallback (kc / 8 was 1.5 % ahead of kc / 4 at top-100; no fallbacks either way)
-    P.M = P.kc + std::max(16, P.kc / 8);
+    P.M = P.kc + std::max(16, P.kc / (h0->dtype == CRAG_FP4 ? 6 : 8));
     if (P.M > CRAG_MAX_M) P.M = CRAG_MAX_M;
 
     // ---- which scan: GEMV groups of up to 8 queries, or one of the MFMA scans (one collection per call only) ----
