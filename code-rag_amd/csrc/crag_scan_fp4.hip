@@ -36,25 +36,44 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
-// `CK` K steps of a tile of 32 rows as a wave holds them
+// A line's eight groups lie in LDS in another order, so that sixteen rows' reads of one group take all banks: place p of row r
+// holds group p ^ (r / 2 % 8), in half lines p ^ (r / 4 % 4).  Lane l of the load that fills place p of row r:
+template <int KS>
+__device__ __forceinline__ int swizzle(int piece, int lane) {
+    if ((piece | 3) < KS) return (lane >> 3) * 128 + (((lane & 7) ^ ((piece & 1) * 4 + (lane >> 4))) * 16);
+    return (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 4)) * 16);
+}
+// ... and where a lane reads its group of a step
+template <int KS>
+__device__ __forceinline__ int swizzled(int step, int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    if ((step | 3) < KS) return (step >> 2) * 4096 + r * 128 + ((h * 4 + (step & 3)) ^ ((r >> 1) & 7)) * 16;
+    return (step >> 2) * 4096 + r * 64 + ((h * 2 + (step & 3)) ^ ((r >> 2) & 3)) * 16;
+}
+
+// The pieces of `CK` K steps of a tile on their way to LDS: 1 KiB each, in the order in which they lie in memory
 template <int CK>
-struct Codes {
+struct Pieces {
     u32x4_t c[CK];
-    template <bool STREAM>
+    template <int KS, bool STREAM>
     __device__ __forceinline__ void load(const GLOBAL_AS unsigned char* tile, int step, int lane) {
 #pragma unroll
         for (int k = 0; k < CK; ++k) {
-            const GLOBAL_AS u32x4_t* p = (const GLOBAL_AS u32x4_t*)(tile + ((step + k) * 64 + lane) * 16);
+            const GLOBAL_AS u32x4_t* p = (const GLOBAL_AS u32x4_t*)(tile + (step + k) * 1024 + swizzle<KS>(step + k, lane));
             if constexpr (STREAM) c[k] = __builtin_nontemporal_load(p);
             else c[k] = *p;
         }
+    }
+    __device__ __forceinline__ void put(unsigned char* to, int lane) const {
+#pragma unroll
+        for (int k = 0; k < CK; ++k) *(u32x4_t*)(to + k * 1024 + lane * 16) = c[k];
     }
 };
 template <int KS>
 struct RowScales {
     uint32_t w[crag_fp4_sw(KS)];
     __device__ __forceinline__ void load(const GLOBAL_AS unsigned char* tile, int lane) {
-        const GLOBAL_AS uint32_t* s = (const GLOBAL_AS uint32_t*)(tile + 1024 * KS) + lane * crag_fp4_sw(KS);
+        const GLOBAL_AS uint32_t* s = (const GLOBAL_AS uint32_t*)(tile + 1024 * KS) + ((lane & 31) * 2 + (lane >> 5)) * crag_fp4_sw(KS);
 #pragma unroll
         for (int i = 0; i < crag_fp4_sw(KS); ++i) w[i] = s[i];
     }
@@ -78,18 +97,16 @@ struct Query {
     }
 };
 
-template <int KS, int P, int QB, int STEP, int CK>
-__device__ __forceinline__ void products(const Codes<CK>& t, const RowScales<KS>& rs, const Query<KS, P> (&q)[QB], f32x16_t (&acc)[QB]) {
-    static_for<CK>([&](auto kc) {
-        constexpr int j = kc, k = STEP + j;
-        const i32x8_t a = {(int)t.c[j].x, (int)t.c[j].y, (int)t.c[j].z, (int)t.c[j].w, 0, 0, 0, 0};
-        static_for<P>([&](auto pc) {
-            constexpr int i = k * P + pc;
+// one step: `codes` is the lane's group of its row
+template <int KS, int P, int QB, int STEP>
+__device__ __forceinline__ void products(const u32x4_t& codes, const RowScales<KS>& rs, const Query<KS, P> (&q)[QB], f32x16_t (&acc)[QB]) {
+    const i32x8_t a = {(int)codes.x, (int)codes.y, (int)codes.z, (int)codes.w, 0, 0, 0, 0};
+    static_for<P>([&](auto pc) {
+        constexpr int i = STEP * P + pc;
 #pragma unroll
-            for (int b = 0; b < QB; ++b)
-                acc[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[b].piece[i], acc[b], 4 /* A: E2M1 */, 2 /* B: E2M3 */, k % 4,
-                                                                         (int)rs.w[k / 4], i % 4, (int)q[b].scale[i / 4]);
-        });
+        for (int b = 0; b < QB; ++b)
+            acc[b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[b].piece[i], acc[b], 4 /* A: E2M1 */, 2 /* B: E2M3 */, STEP % 4,
+                                                                     (int)rs.w[STEP / 4], i % 4, (int)q[b].scale[i / 4]);
     });
 }
 
@@ -143,14 +160,23 @@ __device__ __forceinline__ void keep_all(const f32x16_t& s_, int q, long long ro
             (u32x4_t){crag_fkey(s[4 * r]), crag_fkey(s[4 * r + 1]), crag_fkey(s[4 * r + 2]), crag_fkey(s[4 * r + 3])};
 }
 
-// K steps a wave loads ahead: a whole tile, or what the registers of long rows leave room for
-constexpr int chunk_steps(int ks) { return ks <= 8 ? ks : (ks == 12 ? 6 : (ks == 32 ? 4 : 8)); }
+// K steps a wave loads ahead: a whole tile, or whole lines of it where the registers of long rows leave no room
+constexpr int chunk_steps(int ks, int qb) { return ks == 32 || (ks == 12 && qb == 2) ? 4 : (ks <= 12 ? ks : 8); }
+
+// one lane's LDS writes are in front of the others' reads: LDS serves a wave in order, the compiler has to as well
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // Tiles first, first + step, ... < last.  P = 2: a column is a query.  P = 1: columns c and 16 + c are the pieces of query c.
+// `stage`: 1 KiB * chunk_steps of LDS that is this wave's alone.  Loaded straight into the lanes that multiply them, rows of
+// whole lines would be read 16 bytes here and there (1 query, 4M x 384: the scan 130 us, so 150 through the caches and 210 past them).
 template <int KS, int P, int QB, bool FILTER>
 __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, long long first, long long step, long long last, long long row_end,
-                                     const Fp4Args& a, const Query<KS, P> (&q)[QB], const float (&tau)[QB], const int (&qid)[QB], int lane) {
-    constexpr int CK = chunk_steps(KS), NCH = KS / CK;
+                                     const Fp4Args& a, const Query<KS, P> (&q)[QB], const float (&tau)[QB], const int (&qid)[QB], int lane,
+                                     unsigned char* stage) {
+    constexpr int CK = chunk_steps(KS, QB), NCH = KS / CK;
     static_assert(KS % CK == 0, "whole chunks");
     const GLOBAL_AS unsigned char* rows = (const GLOBAL_AS unsigned char*)rows_;
     const GLOBAL_AS float* xnorm = (const GLOBAL_AS float*)xnorm_;
@@ -158,7 +184,7 @@ __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, lon
     const bool start = l2 && (P == 2 || (lane & 16) == 0);  // the accumulators that begin at |x|^2
     if (first >= last) return;
     const GLOBAL_AS unsigned char* tile = rows + first * crag_fp4_tile_bytes(KS);
-    Codes<CK> cur;
+    Pieces<CK> next;
     RowScales<KS> rs;
     f32x4_t xn[4];
     auto load_norms = [&](long long t) {
@@ -168,7 +194,7 @@ __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, lon
             if (start) xn[r] = *(const GLOBAL_AS f32x4_t*)(xnorm + t * 32 + 8 * r + (lane >> 5) * 4);
         }
     };
-    cur.template load<P == 1>(tile, 0, lane);  // one reader: past the caches
+    next.template load<KS, P == 1>(tile, 0, lane);  // one reader: past the caches
     rs.load(tile, lane);
     load_norms(first);
     for (long long t = first; t < last; t += step) {
@@ -184,11 +210,15 @@ __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, lon
         load_norms(tn);
         static_for<NCH>([&](auto cc) {
             constexpr int c = cc;
-            Codes<CK> next;
-            if constexpr (c + 1 < NCH) next.template load<P == 1>(tile, (c + 1) * CK, lane);
-            else next.template load<P == 1>(tile_n, 0, lane);
-            products<KS, P, QB, c * CK, CK>(cur, rs, q, acc);
-            cur = next;
+            next.put(stage, lane);
+            if constexpr (c + 1 < NCH) next.template load<KS, P == 1>(tile, (c + 1) * CK, lane);
+            else next.template load<KS, P == 1>(tile_n, 0, lane);
+            wave_sync();
+            static_for<CK>([&](auto kc) {
+                constexpr int k = kc;
+                products<KS, P, QB, c * CK + k>(*(const u32x4_t*)(stage + swizzled<KS>(c * CK + k, lane) - c * CK * 1024), rs, q, acc);
+            });
+            wave_sync();
         });
         rs = rs_n;
         tile = tile_n;
@@ -210,6 +240,7 @@ __device__ __forceinline__ void walk(const void* rows_, const float* xnorm_, lon
 // same XCD and share its L2.
 template <int KS, int QB, bool FILTER>
 __global__ __launch_bounds__(256, 1) void k_scan_fp4(Fp4Args a) {
+    __shared__ __attribute__((aligned(16))) unsigned char stage[4 * 1024 * chunk_steps(KS, QB)];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wq = a.wave_queries, wr = 4 / wq;
     const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
@@ -227,7 +258,8 @@ __global__ __launch_bounds__(256, 1) void k_scan_fp4(Fp4Args a) {
         qid[b] = id < a.n_queries ? id : -1;
         tau[b] = FILTER && id < a.n_queries ? a.tau[id] : __builtin_nanf("");
     }
-    walk<KS, 2, QB, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + stream, streams, (a.row_end + 31) >> 5, a.row_end, a, q, tau, qid, lane);
+    walk<KS, 2, QB, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + stream, streams, (a.row_end + 31) >> 5, a.row_end, a, q, tau, qid, lane,
+                            stage + wave * 1024 * chunk_steps(KS, QB));
 }
 
 // The same for large batches: the rows' tiles come through a ring in LDS, one copy for all waves of the workgroup, brought
@@ -255,9 +287,10 @@ __device__ __forceinline__ void issue(const GLOBAL_AS unsigned char* tile, const
         if (c > R::CHUNKS || (c == R::CHUNKS && !norms)) break;  // piece CHUNKS: the norms
         const int bytes = c == R::CHUNKS ? 128 : (c == R::CHUNKS - 1 ? (int)crag_fp4_tile_bytes(KS) - 1024 * (R::CHUNKS - 1) : 1024);
         const GLOBAL_AS unsigned char* from = c == R::CHUNKS ? (const GLOBAL_AS unsigned char*)xnorm : tile + c * 1024;
+        const int at = c < KS ? swizzle<KS>(c, lane) : lane * 16;
         const uint32_t to = __builtin_amdgcn_readfirstlane(slot + c * 1024);
         if (lane * 16 < bytes)  // m0 is the LDS address of lane 0; an instruction must lie between its write and its use
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from + lane * 16) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from + at) : "memory");
     }
 }
 
@@ -315,7 +348,7 @@ __global__ __launch_bounds__(64 * Ring<KS>::WAVES, Ring<KS>::WAVES / 4) void k_s
         const unsigned char* slot = smem + (i % R::SLOTS) * R::SLOT;
         RowScales<KS> rs;
 #pragma unroll
-        for (int w = 0; w < crag_fp4_sw(KS); ++w) rs.w[w] = ((const uint32_t*)(slot + 1024 * KS))[lane * crag_fp4_sw(KS) + w];
+        for (int w = 0; w < crag_fp4_sw(KS); ++w) rs.w[w] = ((const uint32_t*)(slot + 1024 * KS))[((lane & 31) * 2 + (lane >> 5)) * crag_fp4_sw(KS) + w];
         f32x16_t acc[QB];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -327,9 +360,7 @@ __global__ __launch_bounds__(64 * Ring<KS>::WAVES, Ring<KS>::WAVES / 4) void k_s
         }
         static_for<KS>([&](auto kc) {
             constexpr int k = kc;
-            Codes<1> c;
-            c.c[0] = *(const u32x4_t*)(slot + k * 1024 + lane * 16);
-            products<KS, 2, QB, k, 1>(c, rs, q, acc);
+            products<KS, 2, QB, k>(*(const u32x4_t*)(slot + swizzled<KS>(k, lane)), rs, q, acc);
         });
         const long long row0 = (first + i * streams) * 32 + (lane >> 5) * 4;
 #pragma unroll
@@ -349,6 +380,7 @@ __global__ __launch_bounds__(64 * Ring<KS>::WAVES, Ring<KS>::WAVES / 4) void k_s
 // (GroupDesc, as the float32 and bf16 scans have them).
 template <int KS, bool FILTER>
 __global__ __launch_bounds__(256) void k_scan_fp4_narrow(Fp4Args a) {
+    __shared__ __attribute__((aligned(16))) unsigned char stage[4 * 1024 * chunk_steps(KS, 1)];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int bid = blockIdx.x, c = lane & 31;
     Query<KS, 1> q[1];
@@ -357,7 +389,7 @@ __global__ __launch_bounds__(256) void k_scan_fp4_narrow(Fp4Args a) {
         const int qid[1] = {c < 16 && c < a.n_queries ? c : -1};
         const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[c] : __builtin_nanf("")};
         walk<KS, 1, 1, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + (long long)bid * 4 + wave, (long long)gridDim.x * 4, (a.row_end + 31) >> 5,
-                               a.row_end, a, q, tau, qid, lane);
+                               a.row_end, a, q, tau, qid, lane, stage + wave * 1024 * chunk_steps(KS, 1));
         return;
     }
     int g = 0;
@@ -372,7 +404,7 @@ __global__ __launch_bounds__(256) void k_scan_fp4_narrow(Fp4Args a) {
     const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[G.q_first + c] : __builtin_nanf("")};
     const long long first = (long long)(bid - G.blk_first[a.pass]) * 4 + wave;
     walk<KS, 1, 1, FILTER>(G.rows, G.xnorm, (G.from[a.pass] >> 5) + first, (long long)G.n_blk[a.pass] * 4, (row_end + 31) >> 5, row_end, a, q, tau, qid,
-                           lane);
+                           lane, stage + wave * 1024 * chunk_steps(KS, 1));
 }
 
 // ---- queries: float32 -> two E2M3 pieces ---------------------------------------------------------------------------------
@@ -418,7 +450,10 @@ __global__ __launch_bounds__(512) void k_fp4_split(const float* __restrict__ que
     if (tid * 4 < dim_pad) {  // whole groups of eight lanes
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
         if (q >= 0) v = -*(const f32x4_t*)(queries + (long long)q * dim_pad + tid * 4);
-        const int grp = tid >> 3, part = tid & 7, k = grp >> 1, half = (grp & 1) * 32;
+        const int grp = tid >> 3, part = tid & 7;
+        int k, half;
+        crag_fp4_step(ks, grp, &k, &half);
+        half *= 32;
         float big = 0.f;
         int huge = 0;
 #pragma unroll

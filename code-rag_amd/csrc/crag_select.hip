@@ -263,8 +263,11 @@ __device__ __forceinline__ void kth_seed_counts(const KthArgs& a, int q, uint32_
 
 // per query: tau = score of the M-th smallest ordered key of a strided list (KthArgs in crag_common.h);
 // any tau >= the true M-th smallest keeps the cascade exact
-// T threads hold PER keys each.  A list of more than T * PER is cut (its M-th smallest is no smaller than the whole one's); a
-// sample that seeds is never longer.
+// PER = 0: the keys lie in LDS, two blocks of 1024 threads a CU, little code -- half of this kernel's time on one query is
+// fetching it (level lists of one query: 3 .. 6 us, 5 .. 8 with 16 keys in registers and every loop over them written out).
+// Else T threads hold PER keys each, and all blocks of a large batch are at work at once (1024 queries: samples of 8192 32 us,
+// level lists 17, against 78 and 24).  A list of more than T * PER is cut (its M-th smallest is no smaller than the whole
+// one's); a sample that seeds is never longer.
 template <int T, int PER>
 __global__ __launch_bounds__(T) void k_kth(KthArgs a) {
     __shared__ uint32_t scratch[KTH_SCRATCH];
@@ -307,28 +310,51 @@ __global__ __launch_bounds__(T) void k_kth(KthArgs a) {
         }
         return;                                                    // from_cand: keep the looser tau
     }
-    const int len = n < T * PER ? (int)n : T * PER;
-    uint32_t keys[PER];  // of positions tid + u T; all loads in flight at once
+    constexpr int MOST = PER ? T * PER : CRAG_CAND_CAP;
+    const int len = n < MOST ? (int)n : MOST;
+    auto load = [&](int i) { return src_at(seg ? seg_slot(seg_off, a.n_seg, a.seg_cap, i) : i); };
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    uint32_t* held = (uint32_t*)smem;  // PER = 0: [CRAG_CAND_CAP]
+    uint32_t own[PER ? PER : 1];       // else those of positions tid + u T
+    // all loads in flight at once, or four
+    if constexpr (PER) {
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-        const int i = tid + u * T;
-        keys[u] = 0u;
-        if (i < len) keys[u] = src_at(seg ? seg_slot(seg_off, a.n_seg, a.seg_cap, i) : i);
+        for (int u = 0; u < PER; ++u) {
+            own[u] = 0u;
+            if (tid + u * T < len) own[u] = load(tid + u * T);
+        }
+    } else {
+        for (int i0 = tid; i0 < len; i0 += 4 * T) {
+            uint32_t k[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * T < len) k[u] = load(i0 + u * T);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * T < len) held[i0 + u * T] = k[u];
+        }
+        __syncthreads();
     }
-    auto each = [&](auto f) {
+    auto each_at = [&](auto f) {
+        if constexpr (PER) {
 #pragma unroll
-        for (int u = 0; u < PER; ++u)
-            if (tid + u * T < len) f(keys[u]);
+            for (int u = 0; u < PER; ++u)
+                if (tid + u * T < len) f(own[u], tid + u * T);
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < len; i += T) f(held[i], i);
+        }
     };
+    auto each = [&](auto f) { each_at([&](uint32_t k, int) { f(k); }); };
     const uint32_t t = block_select<T>(each, (uint32_t)a.M - 1u, scratch);
     if (tid == 0) a.tau[q] = crag_fkey_inv(t);
     if (!from_cand && a.seed_cand) {  // sample row i IS row i of the collection; n <= 16384 = CRAG_CAND_CAP
         uint32_t* seed_total = scratch;  // block_select is done with its scratch
         if (tid == 0) *seed_total = 0;
         __syncthreads();
-#pragma unroll
-        for (int u = 0; u < PER; ++u)
-            if (tid + u * T < len && keys[u] <= t) kth_seed(a, q, atomicAdd(seed_total, 1u), keys[u], (uint32_t)(tid + u * T));
+        each_at([&](uint32_t k, int i) {
+            if (k <= t) kth_seed(a, q, atomicAdd(seed_total, 1u), k, (uint32_t)i);
+        });
         __syncthreads();
         kth_seed_counts<T>(a, q, *seed_total);
     }
@@ -397,16 +423,19 @@ __device__ __forceinline__ double canon_lane(const void* row, const void* q, int
 struct Fp4Batch {
     typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
     u32x4_t c[8];   // groups 8 b .. 8 b + 7
-    uint32_t s[2];  // scale bytes of the even ones and of the odd ones
+    uint32_t s[2];  // scale bytes of the two lanes that the scans give them to
     __device__ __forceinline__ void load(const __attribute__((address_space(1))) unsigned char* tile, int ks, int row, int b) {
-        const __attribute__((address_space(1))) unsigned char* sc = tile + 1024 * ks + (long long)row * 4 * crag_fp4_sw(ks) + b * 4;
-        s[0] = *(const __attribute__((address_space(1))) uint32_t*)sc;
-        s[1] = *(const __attribute__((address_space(1))) uint32_t*)(sc + 128 * crag_fp4_sw(ks));
+        const int sw = crag_fp4_sw(ks);
+        const __attribute__((address_space(1))) uint32_t* sc = (const __attribute__((address_space(1))) uint32_t*)(tile + 1024 * ks) + row * 2 * sw + b;
+        s[0] = sc[0];
+        s[1] = sc[sw];
+        const bool whole = b * 4 + 4 <= ks;  // (half a line: its groups twice, the second time never used)
+        const __attribute__((address_space(1))) unsigned char* line = tile + 4096 * b + row * (whole ? 128 : 64);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int k = b * 4 + (u >> 1);  // rows of two or six steps end inside a batch: their last step again, never used
-            c[u] = *(const __attribute__((address_space(1))) u32x4_t*)(tile + ((k < ks ? k : ks - 1) * 64 + (u & 1) * 32 + row) * 16);
-        }
+        for (int u = 0; u < 8; ++u) c[u] = *(const __attribute__((address_space(1))) u32x4_t*)(line + (whole ? u : u & 3) * 16);
+    }
+    __device__ __forceinline__ uint32_t scale_byte(int u, bool whole) const {
+        return (whole ? s[u >> 2] >> (8 * (u & 3)) : s[(u >> 1) & 1] >> (8 * (u & 1))) & 255u;
     }
 };
 template <typename Q>
@@ -422,9 +451,10 @@ __device__ __forceinline__ double canon_fp4(const void* rows, const Q* q, int di
     for (int b = 0; b < n; ++b) {
         Fp4Batch next;
         next.load(tile, ks, r, b + 1 < n ? b + 1 : b);
+        const bool whole = b * 4 + 4 <= ks;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float scale = crag_fp4_scale((cur.s[u & 1] >> (8 * (u >> 1))) & 255u);
+            const float scale = crag_fp4_scale(cur.scale_byte(u, whole));
             const int d0 = b * 256 + u * 32 + 2 * j;
             if (b * 256 + u * 32 < dim) {  // (elements behind the row's end are zero in both: they add +0)
 #pragma unroll
@@ -1165,7 +1195,12 @@ int crag_launch_row_norms(const void* rows, int dtype, int dim_pad, long long n,
 
 int crag_launch_kth(const KthArgs& a, hipStream_t s) {
     if (a.many) hipLaunchKernelGGL((k_kth<256, 32>), dim3(a.B), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_kth<1024, CRAG_CAND_CAP / 1024>), dim3(a.B), dim3(1024), 0, s, a);
+    else {
+        const size_t lds = sizeof(uint32_t) * CRAG_CAND_CAP;
+        static std::atomic<uint64_t> lds_ok;
+        crag_allow_dynamic_lds((const void*)k_kth<1024, 0>, lds, lds_ok);
+        hipLaunchKernelGGL((k_kth<1024, 0>), dim3(a.B), dim3(1024), lds, s, a);
+    }
     return (int)hipGetLastError();
 }
 
