@@ -250,7 +250,7 @@ class GpuCollection:
                    torch.empty((b, top_k), dtype=torch.float64, device=dev),
                    torch.empty((b, top_k), dtype=torch.float32, device=dev),
                    torch.empty((b,), dtype=torch.int32, device=dev))
-        st = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        st = _lib.current_stream(self.device) if stream is None else stream
         check(self._lib.crag_search_device(self._h, queries.data_ptr(), b, int(top_k), float(symbol_boost),
                                            None if q_hashes is None else q_hashes.data_ptr(),
                                            None if q_hash_off is None else q_hash_off.data_ptr(),
@@ -265,7 +265,7 @@ class GpuCollection:
         if not self._finalized:
             self.finalize()
         self._check_tensor(queries)
-        st = torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
+        st = _lib.current_stream(self.device) if stream is None else stream
         check(self._lib.crag_search_local_device(self._h, queries.data_ptr(), queries.shape[0], int(top_k),
                                                  None if q_hashes is None else q_hashes.data_ptr(),
                                                  None if q_hash_off is None else q_hash_off.data_ptr(),
@@ -315,7 +315,7 @@ def merge_rerank_device(device: int, entries, n_shards: int, b: int, top_k: int,
                torch.empty((b, top_k), dtype=torch.float64, device=dev),
                torch.empty((b, top_k), dtype=torch.float32, device=dev),
                torch.empty((b,), dtype=torch.int32, device=dev))
-    st = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+    st = _lib.current_stream(device) if stream is None else stream
     check(lib.crag_merge_rerank_device(int(device), entries.data_ptr(), int(n_shards), int(b), int(top_k),
                                        float(symbol_boost), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
                                        out[3].data_ptr(), st), "crag_merge_rerank_device")
@@ -378,7 +378,7 @@ def search_multi_device(collections: List[GpuCollection], queries, top_k: int = 
                torch.empty((b, top_k), dtype=torch.float64, device=dev),
                torch.empty((b, top_k), dtype=torch.float32, device=dev),
                torch.empty((b,), dtype=torch.int32, device=dev))
-    st = torch.cuda.current_stream(collections[0].device).cuda_stream if stream is None else stream
+    st = _lib.current_stream(collections[0].device) if stream is None else stream
     check(lib.crag_search_multi_device(hs, queries.data_ptr(), b, int(top_k), float(symbol_boost),
                                        None if q_hashes is None else q_hashes.data_ptr(),
                                        None if q_hash_off is None else q_hash_off.data_ptr(),

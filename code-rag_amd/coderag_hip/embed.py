@@ -131,7 +131,7 @@ def _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, wa
     ws, ws_ptr, ws_bytes = _workspace(n, n_bags, dim, False, dev)
     check(_lib.load().crag_embed_forward_device(
         dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), n, offsets.data_ptr(), n_bags,
-        POOL_MODES[mode], float(scale), int(bool(normalize)), out.data_ptr(), _dtype_id(out), _ptr(coef), ws_ptr, ws_bytes, torch.cuda.current_stream(dev).cuda_stream), "crag_embed_forward_device")
+        POOL_MODES[mode], float(scale), int(bool(normalize)), out.data_ptr(), _dtype_id(out), _ptr(coef), ws_ptr, ws_bytes, _lib.current_stream(dev.index)), "crag_embed_forward_device")
     return out, coef
 
 
@@ -165,7 +165,7 @@ def _bag_function():
             check(_lib.load().crag_embed_backward_device(
                 dev.index, table.data_ptr(), vocab, dim, _dtype_id(table), ids.data_ptr(), _ptr(weights), ids.numel(),
                 offsets.data_ptr(), n_bags, int(ctx.normalize), y.data_ptr(), coef.data_ptr(), grad.data_ptr(), _ptr(d_table),
-                _ptr(d_weights), ws_ptr, ws_bytes, torch.cuda.current_stream(dev).cuda_stream),
+                _ptr(d_weights), ws_ptr, ws_bytes, _lib.current_stream(dev.index)),
                 "crag_embed_backward_device")
             return d_table, d_weights, None, None, None, None, None
 
