@@ -301,6 +301,74 @@ def test_captured_lookup_and_gradient():
         del want
 
 
+def test_gradients_of_every_form():
+    import torch
+    case = make(50, 30, 65, 90, 4)
+    table, ids, offsets, w = gpu(*case)
+    table.requires_grad_(True)
+    w.requires_grad_(True)
+    grad = torch.randn((50, 65), device="cuda")
+    want = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), (table, w), grad)
+    # strided gradients: transposed, broadcast
+    t = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), (table, w), grad.t().contiguous().t())
+    assert torch.equal(t[0], want[0]) and torch.equal(t[1], want[1])
+    one = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w).sum(), (table, w))
+    ones = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), (table, w), torch.ones_like(grad))
+    assert torch.equal(one[0], ones[0]) and torch.equal(one[1], ones[1])
+    # one input alone
+    assert torch.equal(torch.autograd.grad(ch.embed_bags(table, ids, offsets, w.detach()), table, grad)[0], want[0])
+    assert torch.equal(torch.autograd.grad(ch.embed_bags(table.detach(), ids, offsets, w), w, grad)[0], want[1])
+    # bf16 vectors: the gradient comes back rounded to bf16, and is otherwise the same
+    y = ch.embed_bags(table, ids, offsets, w, out_dtype=torch.bfloat16)
+    assert y.dtype == torch.bfloat16
+    half = torch.autograd.grad(y, table, grad.bfloat16())[0]
+    exact = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), table, grad.bfloat16().float())[0]
+    assert torch.equal(half, exact)
+    # the same table twice in one graph
+    both = torch.autograd.grad((ch.embed_bags(table, ids, offsets, w) * grad).sum() + (ch.embed_bags(table, ids, offsets, w) * grad).sum(), table)[0]
+    assert torch.equal(both, want[0] + want[0])
+    # a second derivative is refused
+    (g,) = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), table, grad, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    # changed in place in between
+    y = ch.embed_bags(table, ids, offsets, w)
+    with torch.no_grad():
+        table.add_(1.0)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+def test_two_threads_on_streams_of_their_own():
+    import threading
+    import torch
+    cases = [gpu(*make(30 + 20 * i, 200, 96, 400, i)) for i in range(4)]
+    want = []
+    for table, ids, offsets, w in cases:
+        table.requires_grad_(True)
+        y = ch.embed_bags(table, ids, offsets, w)
+        want.append((y.detach().clone(), torch.autograd.grad(y, table, torch.ones_like(y))[0]))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        table, ids, offsets, w = cases[i]
+        st = torch.cuda.Stream()
+        for _ in range(10):
+            with torch.cuda.stream(st):
+                y = ch.embed_bags(table, ids, offsets, w)
+                g = torch.autograd.grad(y, table, torch.ones_like(y))[0]
+            st.synchronize()
+            bad.extend(1 for a, b in zip((y, g), want[i]) if not torch.equal(a, b))
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
+
 def test_training_through_a_search_batch():
     """the lookup inside a loss of a user's own: gradients of question and chunk bags through one table add up"""
     import torch

@@ -157,6 +157,64 @@ def test_duplicates_ties_and_zero_rows_go_through_the_fallback_tiers(coracle, b)
         agree(col.search(q, 20), want)
 
 
+def awkward(kind):
+    """rows whose scores are unkind to a selection by thresholds"""
+    r = np.random.default_rng(len(kind))
+    if kind == "three rows, 8000 times each":
+        return np.repeat(unit(3, 64, 1), 8000, 0)
+    if kind == "400 rows, 60 times each":
+        return np.tile(unit(400, 64, 2), (60, 1))
+    if kind == "every row nearer than those in front":     # no threshold of a sample holds anything back
+        d = np.zeros((15000, 64), np.float32)
+        d[:, 0] = np.linspace(40, 1, 15000, dtype=np.float32)
+        d[:, 1:] = 0.01 * r.standard_normal((15000, 63)).astype(np.float32)
+        return d
+    if kind == "norms of forty powers of two":             # almost all scores in one bin of their range
+        return unit(20000, 64, 3) * np.exp2(r.integers(-20, 21, (20000, 1))).astype(np.float32)
+    raise KeyError(kind)
+
+
+@pytest.mark.parametrize("b,top_k", [(300, 10), (300, 200), (1030, 3), (256, 60), (5, 25)])
+@pytest.mark.parametrize("kind", ["three rows, 8000 times each", "400 rows, 60 times each", "every row nearer than those in front",
+                                  "norms of forty powers of two"])
+def test_awkward_rows_in_batches_of_every_size(kind, b, top_k):
+    """more queries than CUs take smaller blocks for the selection, with less room: both sides of it, against a float32
+    collection of the rows as they are held"""
+    import torch
+    col = collection(awkward(kind))
+    ref = ch.GpuCollection(64, "f32")
+    ref.add(col.rows_host())
+    q = torch.from_numpy(unit(b, 64, 9)).cuda()
+    for got, want in zip(col.search_device(q, top_k), ref.search_device(q, top_k)):
+        assert torch.equal(got, want)
+
+
+def test_rows_added_in_pieces_and_profiled():
+    import torch
+    rows, cls = unit(9000, 100, 4), (np.arange(9000) % 3).astype(np.uint8)
+    whole = collection(rows, classes=cls)
+    q = torch.from_numpy(unit(40, 100, 5)).cuda()
+    want = whole.search_device(q, 10)
+    parts = ch.GpuCollection(100, "fp4")
+    at = 0
+    for n in (1, 30, 31, 2, 64, 5000, 3, 3869):
+        if n % 2:
+            parts.add(rows[at:at + n], path_class=cls[at:at + n])
+        else:
+            parts.add_device(torch.from_numpy(rows[at:at + n]).cuda(), path_class=torch.from_numpy(cls[at:at + n]).cuda())
+        at += n
+        if n == 64:
+            parts.search_device(q, 10)      # and goes on growing
+    assert at == 9000
+    assert np.array_equal(parts.rows_host(), whole.rows_host())
+    assert np.array_equal(parts.rows_host(61, 70), whole.rows_host()[61:131])
+    parts.set_profiling(True)
+    for k in (1, 17, 40):
+        for got, w in zip(parts.search_device(q[:k], 10), want):
+            assert torch.equal(got, w[:k])
+    assert parts.profile()["searches"] == 3
+
+
 def test_empty_collection_and_refusals():
     import torch
     col = collection(np.zeros((0, 96), np.float32))

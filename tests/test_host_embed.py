@@ -21,14 +21,14 @@ def test_workspace_sizes():
     for n, b, d in ((0, 0, 1), (1, 1, 384), (10 ** 6, 1000, 384), (2 ** 31 - 1, 1, 8), (5000, 3, 2048), (5000, 3, 2047)):
         fwd, bwd = lib.crag_embed_workspace(n, b, d, 0), lib.crag_embed_workspace(n, b, d, 1)
         assert 0 <= fwd <= bwd and (fwd > 0) == (n >= 5000)
-    for bad in ((-1, 1, 8), (2 ** 31, 1, 8), (1, -1, 8), (1, 1, 0), (1, 1, 2049)):
+    for bad in ((-1, 1, 8), (2 ** 31, 1, 8), (1, -1, 8), (1, 1, 0), (1, 1, 2049), (1, 2 ** 24 + 1, 8)):
         assert lib.crag_embed_workspace(*bad, 0) < 0
 
 
 def test_forward_and_backward_refuse_before_touching_a_device():
     lib = ch.load()
     good = [0, 256, 10, 8, 0, 256, None, 5000, 256, 1, 0, 1.0, 0, 256, 0, None, 256, 1 << 30, None]
-    for i, bad in ((1, None), (1, 257), (2, 0), (2, 2 ** 31), (3, 0), (3, 2049), (4, 2), (5, None), (7, -1), (8, None), (9, -1), (10, 3), (13, None), (13, 264), (14, 2),
+    for i, bad in ((1, None), (1, 257), (2, 0), (2, 2 ** 31), (3, 0), (3, 2049), (4, 2), (5, None), (7, -1), (8, None), (9, -1), (9, 2 ** 24 + 1), (10, 3), (13, None), (13, 264), (14, 2),
                    (16, None), (16, 128), (17, 16)):
         wrong = list(good)
         wrong[i] = bad
