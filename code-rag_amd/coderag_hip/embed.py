@@ -156,6 +156,13 @@ def _bag_function():
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
+            if torch.cuda.is_current_stream_capturing():
+                # torch hands a leaf's gradient over on the stream on which the leaf's node was made; where an eager graph
+                # keeps one alive that is the default stream, which a capture must not touch: the process would end
+                for node, _ in ctx.next_functions:
+                    if node is not None and node.metadata.get("coderag_stream") == 0:
+                        raise RuntimeError("embed_bags: a backward pass is being captured while an eager graph of the same table or "
+                                           "weights is alive; delete what was computed from them on the default stream first")
             table, weights, ids, offsets, y, coef = ctx.saved_tensors
             dev, n_bags, (vocab, dim) = table.device, offsets.numel() - 1, table.shape
             grad = grad.contiguous()
@@ -180,7 +187,9 @@ def embed_bags(table, ids, offsets, weights=None, mode: str = "mean", scale: flo
     table: CUDA [vocab, dim] float32 or bfloat16; ids: int32 [T]; offsets: int64 [bags + 1], ascending; weights: float32 [T]
     or None.  Ids outside [0, vocab) are padding: they contribute nothing and do not count.  An empty bag gives zeros.
     Returns [bags, dim] in out_dtype (float32).  Runs on the current stream of the table's device, without a
-    synchronisation.  Differentiable (once) in table and weights; the gradient of the table is dense, in its dtype."""
+    synchronisation, and may be captured into a graph; so may its backward pass, while no eager graph of the same table or
+    weights from the default stream is alive (RuntimeError).  Differentiable (once) in table and weights; the gradient of the
+    table is dense, in its dtype."""
     import torch
     _check_bags(table, ids, offsets, weights)
     if mode not in POOL_MODES:
@@ -189,7 +198,13 @@ def embed_bags(table, ids, offsets, weights=None, mode: str = "mean", scale: flo
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("out_dtype must be float32 or bfloat16")
     if torch.is_grad_enabled() and (table.requires_grad or (weights is not None and weights.requires_grad)):
-        return _bag_function().apply(table, weights, ids, offsets, mode, float(scale), bool(normalize)).to(out_dtype)
+        y = _bag_function().apply(table, weights, ids, offsets, mode, float(scale), bool(normalize))
+        if not torch.cuda.is_current_stream_capturing():
+            stream = _lib.current_stream(table.device.index)
+            for node, _ in y.grad_fn.next_functions:
+                if node is not None:
+                    node.metadata.setdefault("coderag_stream", stream)
+        return y.to(out_dtype)
     return _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, False)[0]
 
 

@@ -301,6 +301,33 @@ def test_captured_lookup_and_gradient():
         del want
 
 
+def test_backward_capture_beside_an_eager_graph_is_refused():
+    import torch
+    table, ids, offsets, w = gpu(*make(20, 40, 64, 100, 3))
+    table.requires_grad_(True)
+    grad = torch.randn((20, 64), device="cuda")
+    y = ch.embed_bags(table, ids, offsets, w)       # alive, on the default stream
+    want = torch.autograd.grad(y, table, grad, retain_graph=True)[0]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), table, grad)
+    torch.cuda.synchronize()
+    fwd = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(fwd):                     # the lookup alone may be captured
+        out = ch.embed_bags(table.detach(), ids, offsets, w)
+    fwd.replay()
+    assert torch.equal(out, y)
+    assert torch.equal(torch.autograd.grad(y, table, grad)[0], want)
+    del y
+    both = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(both):
+        d = torch.autograd.grad(ch.embed_bags(table, ids, offsets, w), table, grad)[0]
+    for _ in range(3):
+        both.replay()
+        assert torch.equal(d, want)
+
+
 def test_gradients_of_every_form():
     import torch
     case = make(50, 30, 65, 90, 4)
