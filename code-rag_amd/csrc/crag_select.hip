@@ -62,11 +62,38 @@ __global__ __launch_bounds__(256) void k_row_norms(const uint4* __restrict__ row
 }
 
 // ----------------------------------------------------------------------------------------
-// Block-wide selection by T threads over 32-bit keys: `each(f)` calls f(key) for every key that this thread has.  Returns, to
-// every thread, the want-th smallest (0-based, want below the number of keys).  Selection, not sorting: min/max, a 2048-bin
-// histogram of (key - min) >> shift, a block scan to the bin that holds the wanted rank, and the exact rank among that bin's
-// few keys.  A bin of more than KTH_LIST keys is cut into bins of its own first (1024 queries, 8192 keys each: 96 us with up to
-// 1024 keys ranked against each other, for the sake of a few queries whose keys are uneven).
+// Sums, minima and maxima over a wave by moves between its lanes (an LDS round trip for each of the six steps would be a tenth
+// of a selection).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_move(uint32_t none, uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <typename Op>
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t none, Op op) {  // inclusive
+    v = op(v, lane_move<0x111, 0xf>(none, v));  // the lane 1, 2, 4, 8 in front, within sixteen lanes
+    v = op(v, lane_move<0x112, 0xf>(none, v));
+    v = op(v, lane_move<0x114, 0xf>(none, v));
+    v = op(v, lane_move<0x118, 0xf>(none, v));
+    v = op(v, lane_move<0x142, 0xa>(none, v));  // lane 15 of the sixteen in front, then lane 31
+    return op(v, lane_move<0x143, 0xc>(none, v));
+}
+__device__ __forceinline__ uint32_t wave_sums(uint32_t v) {
+    return wave_scan(v, 0u, [](uint32_t x, uint32_t y) { return x + y; });
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v) {
+    return __builtin_amdgcn_readlane(wave_scan(v, 0xffffffffu, [](uint32_t x, uint32_t y) { return x < y ? x : y; }), 63);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    return __builtin_amdgcn_readlane(wave_scan(v, 0u, [](uint32_t x, uint32_t y) { return x > y ? x : y; }), 63);
+}
+
+// Block-wide selection by T threads over 32-bit keys (crag_fkey): `each(f)` calls f(key) for every key that this thread has.
+// Returns, to every thread, the want-th smallest (0-based, want below the number of keys).  Selection, not sorting: min/max, a
+// 2048-bin histogram, a block scan to the bin that holds the wanted rank, and the exact rank among that bin's few keys.  The
+// first histogram is of equal steps of the SCORE: equal steps of the key give each power of two as many bins, and where scores
+// cross zero almost all keys share a dozen of them (8000 keys, one query: k_kth 11.4 us, so 9.2).  A bin of more than KTH_LIST keys is then
+// cut into bins of equal steps of the key, as often as it takes (1024 queries, 8192 keys each: 96 us with up to 1024 keys ranked
+// against each other, for the sake of a few queries whose keys are uneven).
 // scratch: KTH_SCRATCH 32-bit words of LDS; the caller's LDS writes of the keys must be fenced by the caller.
 constexpr int KTH_BINS = 2048;
 constexpr int KTH_BITS = 11;
@@ -80,38 +107,38 @@ __device__ __forceinline__ uint32_t block_select(Each each, uint32_t want, uint3
     uint32_t* wsum = list + KTH_LIST;      // [48] wave totals, wave minima, wave maxima
     uint32_t* ctl = wsum + 48;             // [4]: bin, rank inside the bin, list length, keys in the bin; then the result
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    uint32_t mn = 0xffffffffu, mx = 0u;
-    each([&](uint32_t k) {
-        mn = k < mn ? k : mn;
-        mx = k > mx ? k : mx;
-    });
-    for (int i = tid; i < KTH_BINS; i += T) hist[i] = 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint32_t o1 = __shfl_xor(mn, off), o2 = __shfl_xor(mx, off);
-        mn = o1 < mn ? o1 : mn;
-        mx = o2 > mx ? o2 : mx;
-    }
-    if (lane == 0) {
-        wsum[16 + wv] = mn;
-        wsum[32 + wv] = mx;
-    }
-    if (tid == 0) ctl[2] = 0;
-    __syncthreads();
-    mn = wsum[16];
-    mx = wsum[32];
-#pragma unroll
-    for (int w = 1; w < W; ++w) {
-        mn = wsum[16 + w] < mn ? wsum[16 + w] : mn;
-        mx = wsum[32 + w] > mx ? wsum[32 + w] : mx;
-    }
-    const uint32_t range = mx - mn;
-    const int bits = range ? 32 - __builtin_clz(range) : 0;
-    int shift = bits > KTH_BITS ? bits - KTH_BITS : 0;  // (key - mn) >> shift < KTH_BINS
-    uint32_t lo = mn;
-    for (;;) {
+    uint32_t mn, mx;
+    auto min_max = [&](auto in) {  // of the keys that `in` lets through; clears the histogram
+        mn = 0xffffffffu;
+        mx = 0u;
         each([&](uint32_t k) {
-            if (k >= lo && ((k - lo) >> shift) < (uint32_t)KTH_BINS) atomicAdd(&hist[(k - lo) >> shift], 1u);
+            if (!in(k)) return;
+            mn = k < mn ? k : mn;
+            mx = k > mx ? k : mx;
+        });
+        for (int i = tid; i < KTH_BINS; i += T) hist[i] = 0;
+        mn = wave_min(mn);
+        mx = wave_max(mx);
+        if (lane == 0) {
+            wsum[16 + wv] = mn;
+            wsum[32 + wv] = mx;
+        }
+        if (tid == 0) ctl[2] = 0;
+        __syncthreads();
+        mn = wsum[16];
+        mx = wsum[32];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            mn = wsum[16 + w] < mn ? wsum[16 + w] : mn;
+            mx = wsum[32 + w] > mx ? wsum[32 + w] : mx;
+        }
+    };
+    // one histogram: bin_of(k) < KTH_BINS, or more for keys that are not looked at.  Its bin of the wanted key and the keys in
+    // it; `want` becomes the rank among them.
+    auto pick = [&](auto bin_of, uint32_t& bin, uint32_t& in_bin) {
+        each([&](uint32_t k) {
+            const uint32_t h = bin_of(k);
+            if (h < (uint32_t)KTH_BINS) atomicAdd(&hist[h], 1u);
         });
         __syncthreads();
         // exclusive scan over the bins: thread t owns bins OWN t .. OWN t + OWN - 1
@@ -121,12 +148,7 @@ __device__ __forceinline__ uint32_t block_select(Each each, uint32_t want, uint3
             h[o] = hist[OWN * tid + o];
             mine += h[o];
         }
-        uint32_t inc = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = __shfl_up(inc, off);
-            if (lane >= off) inc += o;
-        }
+        const uint32_t inc = wave_sums(mine);
         if (lane == 63) wsum[wv] = inc;
         __syncthreads();
         uint32_t base = 0;
@@ -148,44 +170,70 @@ __device__ __forceinline__ uint32_t block_select(Each each, uint32_t want, uint3
             ctl[3] = in;
         }
         __syncthreads();
-        lo += ctl[0] << shift;
+        bin = ctl[0];
         want = ctl[1];
-        const uint32_t in = ctl[3];
+        in_bin = ctl[3];
+    };
+    // the exact rank among the at most KTH_LIST keys that `in` lets through
+    auto settle = [&](auto in) {
+        each([&](uint32_t k) {
+            if (in(k)) list[atomicAdd(&ctl[2], 1u)] = k;
+        });
+        __syncthreads();
+        constexpr int LANES = T / KTH_LIST;  // per item of the list
+        const int L = (int)ctl[2], i = tid / LANES;
+        if (i < L) {
+            const uint32_t k = list[i];
+            uint32_t lt = 0, eq = 0;
+#pragma unroll
+            for (int u = 0; u < KTH_LIST / LANES; ++u) {
+                const int j = u * LANES + tid % LANES;
+                const uint32_t o = list[j];
+                lt += j < L && o < k ? 1u : 0u;
+                eq += j < L && o == k ? 1u : 0u;
+            }
+            for (int o = 1; o < LANES; o <<= 1) {
+                lt += __shfl_xor(lt, o);
+                eq += __shfl_xor(eq, o);
+            }
+            if (lt <= want && want < lt + eq) ctl[3] = k;  // duplicates write the same value
+        }
+        __syncthreads();
+        const uint32_t r = ctl[3];
+        __syncthreads();  // scratch may be reused at once
+        return r;
+    };
+
+    min_max([](uint32_t) { return true; });
+    uint32_t bin, in_bin, score_bin = 0;
+    const float f0 = crag_fkey_inv(mn), step = (float)KTH_BINS / (crag_fkey_inv(mx) - f0);
+    const bool by_score = mn != mx && step > 0.f && step <= 3.4028234663852886e38f;  // (scores of any kind: no NaN, no infinity in it)
+    auto score_of = [&](uint32_t k) {  // rises with k
+        const float x = (crag_fkey_inv(k) - f0) * step;
+        return x < (float)(KTH_BINS - 1) ? (uint32_t)x : (uint32_t)(KTH_BINS - 1);
+    };
+    if (by_score) {
+        pick(score_of, score_bin, in_bin);
+        if (in_bin <= (uint32_t)KTH_LIST) return settle([&](uint32_t k) { return score_of(k) == score_bin; });
+        min_max([&](uint32_t k) { return score_of(k) == score_bin; });
+    }
+    const uint32_t range = mx - mn;
+    const int bits = range ? 32 - __builtin_clz(range) : 0;
+    int shift = bits > KTH_BITS ? bits - KTH_BITS : 0;  // (key - mn) >> shift < KTH_BINS
+    uint32_t lo = mn;
+    for (;;) {
+        auto bin_of = [&](uint32_t k) { return k >= lo && k <= mx ? (k - lo) >> shift : 0xffffffffu; };
+        pick(bin_of, bin, in_bin);
+        lo += bin << shift;
         if (shift == 0) {  // a bin is one value
             __syncthreads();  // scratch may be reused at once
             return lo;
         }
-        if (in <= (uint32_t)KTH_LIST) break;
+        if (in_bin <= (uint32_t)KTH_LIST) return settle([&](uint32_t k) { return k >= lo && k <= mx && ((k - lo) >> shift) == 0u; });
         shift = shift > KTH_BITS ? shift - KTH_BITS : 0;
         for (int i = tid; i < KTH_BINS; i += T) hist[i] = 0;
         __syncthreads();
     }
-    each([&](uint32_t k) {
-        if (k >= lo && ((k - lo) >> shift) == 0u) list[atomicAdd(&ctl[2], 1u)] = k;
-    });
-    __syncthreads();
-    constexpr int LANES = T / KTH_LIST;  // per item of the list
-    const int L = (int)ctl[2], i = tid / LANES;
-    if (i < L) {
-        const uint32_t k = list[i];
-        uint32_t lt = 0, eq = 0;
-#pragma unroll
-        for (int u = 0; u < KTH_LIST / LANES; ++u) {
-            const int j = u * LANES + tid % LANES;
-            const uint32_t o = list[j];
-            lt += j < L && o < k ? 1u : 0u;
-            eq += j < L && o == k ? 1u : 0u;
-        }
-        for (int o = 1; o < LANES; o <<= 1) {
-            lt += __shfl_xor(lt, o);
-            eq += __shfl_xor(eq, o);
-        }
-        if (lt <= want && want < lt + eq) ctl[3] = k;  // duplicates write the same value
-    }
-    __syncthreads();
-    const uint32_t r = ctl[3];
-    __syncthreads();  // scratch may be reused at once
-    return r;
 }
 
 // Segmented candidate buffer (MfmaArgs in crag_common.h): exclusive prefix of the per-segment counts of one
@@ -207,12 +255,7 @@ __device__ __forceinline__ int block_seg_offsets(const uint32_t* __restrict__ se
         }
         mine += c[o];
     }
-    uint32_t inc = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = __shfl_up(inc, off);
-        if (lane >= off) inc += o;
-    }
+    const uint32_t inc = wave_sums(mine);
     if (lane == 63) wsum[wv] = inc;
     const int any_ov = __syncthreads_or(ov ? 1 : 0);
     uint32_t at = inc - mine;
@@ -237,6 +280,27 @@ __device__ __forceinline__ int seg_slot(const uint32_t* segoff, int n_seg, int s
         if (segoff[mid] <= (uint32_t)i) lo = mid; else hi = mid;
     }
     return lo * seg_cap + (i - (int)segoff[lo]);
+}
+
+// f(i, slot) for every gathered candidate i < most by the T threads of the block, a few neighbouring threads to a segment: no
+// search for the segment of each, and four of a thread's at a time (load, then store: `get` and `put`)
+template <int T, typename V, typename Get, typename Put>
+__device__ __forceinline__ void copy_segments(const uint32_t* segoff, int n_seg, int seg_cap, int most, Get get, Put put) {
+    int lanes = 16;
+    while (lanes > 1 && n_seg * lanes > T) lanes >>= 1;
+    const int part = threadIdx.x % lanes;
+    for (int sg = threadIdx.x / lanes; sg < n_seg; sg += T / lanes) {
+        const int o = (int)segoff[sg], end = (int)segoff[sg + 1] < most ? (int)segoff[sg + 1] : most, slot = sg * seg_cap - o;
+        for (int i0 = o + part; i0 < end; i0 += 4 * lanes) {
+            V v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * lanes < end) v[u] = get(slot + i0 + u * lanes);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i0 + u * lanes < end) put(i0 + u * lanes, v[u]);
+        }
+    }
 }
 
 // level 0 seeds the candidate buffer with the sample rows at or below tau (KthArgs::seed_*): seed number j
@@ -266,9 +330,9 @@ __device__ __forceinline__ void kth_seed_counts(const KthArgs& a, int q, uint32_
 // PER = 0: the keys lie in LDS, two blocks of 1024 threads a CU, little code -- half of this kernel's time on one query is
 // fetching it (level lists of one query: 3 .. 6 us, 5 .. 8 with 16 keys in registers and every loop over them written out).
 // Else T threads hold PER keys each, and all blocks of a large batch are at work at once (1024 queries: samples of 8192 32 us,
-// level lists 17, against 78 and 24).  A list of more than T * PER is cut (its M-th smallest is no smaller than the whole
-// one's); a sample that seeds is never longer.
-template <int T, int PER>
+// 29 us against 78).  A list that is longer is cut (its M-th smallest is no smaller than the whole one's); a sample that
+// seeds is never longer.
+template <int T, int PER, int CAP>
 __global__ __launch_bounds__(T) void k_kth(KthArgs a) {
     __shared__ uint32_t scratch[KTH_SCRATCH];
     __shared__ uint32_t seg_off[1024 + 1];
@@ -310,25 +374,27 @@ __global__ __launch_bounds__(T) void k_kth(KthArgs a) {
         }
         return;                                                    // from_cand: keep the looser tau
     }
-    constexpr int MOST = PER ? T * PER : CRAG_CAND_CAP;
+    constexpr int MOST = PER ? T * PER : CAP;
     const int len = n < MOST ? (int)n : MOST;
-    auto load = [&](int i) { return src_at(seg ? seg_slot(seg_off, a.n_seg, a.seg_cap, i) : i); };
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    uint32_t* held = (uint32_t*)smem;  // PER = 0: [CRAG_CAND_CAP]
+    uint32_t* held = (uint32_t*)smem;  // PER = 0: [CAP]
     uint32_t own[PER ? PER : 1];       // else those of positions tid + u T
     // all loads in flight at once, or four
     if constexpr (PER) {
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
             own[u] = 0u;
-            if (tid + u * T < len) own[u] = load(tid + u * T);
+            if (tid + u * T < len) own[u] = src_at(tid + u * T);
         }
+    } else if (seg) {
+        copy_segments<T, uint32_t>(seg_off, a.n_seg, a.seg_cap, len, src_at, [&](int i, uint32_t k) { held[i] = k; });
+        __syncthreads();
     } else {
         for (int i0 = tid; i0 < len; i0 += 4 * T) {
             uint32_t k[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (i0 + u * T < len) k[u] = load(i0 + u * T);
+                if (i0 + u * T < len) k[u] = src_at(i0 + u * T);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (i0 + u * T < len) held[i0 + u * T] = k[u];
@@ -556,14 +622,19 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
     if (c > 256) {
         const bool held = ALL || c <= KEYS - FIN_GATHER;  // (else every pass reads them where they lie)
         if (held) {
-            for (int i0 = tid; i0 < c; i0 += 4 * T) {  // four loads in flight
-                unsigned long long k[4];
+            if (seg) {
+                copy_segments<T, unsigned long long>(seg_off, a.n_seg, a.seg_cap, c, [&](int slot) { return cq[slot]; },
+                                                     [&](int i, unsigned long long k) { skeys[i] = k; });
+            } else {
+                for (int i0 = tid; i0 < c; i0 += 4 * T) {  // four loads in flight
+                    unsigned long long k[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (i0 + u * T < c) k[u] = cand_at(i0 + u * T);
+                    for (int u = 0; u < 4; ++u)
+                        if (i0 + u * T < c) k[u] = cq[i0 + u * T];
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (i0 + u * T < c) skeys[i0 + u * T] = k[u];
+                    for (int u = 0; u < 4; ++u)
+                        if (i0 + u * T < c) skeys[i0 + u * T] = k[u];
+                }
             }
         }
         __syncthreads();
@@ -1193,14 +1264,18 @@ int crag_launch_row_norms(const void* rows, int dtype, int dim_pad, long long n,
     return (int)hipGetLastError();
 }
 
+template <int T, int CAP>
+static int launch_kth_lds(const KthArgs& a, hipStream_t s) {
+    const size_t lds = sizeof(uint32_t) * CAP;
+    static std::atomic<uint64_t> lds_ok;
+    crag_allow_dynamic_lds((const void*)k_kth<T, 0, CAP>, lds, lds_ok);
+    hipLaunchKernelGGL((k_kth<T, 0, CAP>), dim3(a.B), dim3(T), lds, s, a);
+    return (int)hipGetLastError();
+}
 int crag_launch_kth(const KthArgs& a, hipStream_t s) {
-    if (a.many) hipLaunchKernelGGL((k_kth<256, 32>), dim3(a.B), dim3(256), 0, s, a);
-    else {
-        const size_t lds = sizeof(uint32_t) * CRAG_CAND_CAP;
-        static std::atomic<uint64_t> lds_ok;
-        crag_allow_dynamic_lds((const void*)k_kth<1024, 0>, lds, lds_ok);
-        hipLaunchKernelGGL((k_kth<1024, 0>), dim3(a.B), dim3(1024), lds, s, a);
-    }
+    if (!a.many) return launch_kth_lds<1024, CRAG_CAND_CAP>(a, s);
+    if (a.n_seg > 0 || a.cnt) return launch_kth_lds<256, 4096>(a, s);
+    hipLaunchKernelGGL((k_kth<256, 32, 0>), dim3(a.B), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 
