@@ -743,6 +743,39 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
         return;
     }
 
+    // The exactness certificate, while the others wait for rows: every row that was NOT re-scored has approximate score >= s_M:
+    // the buffer is sorted, so the remaining candidates start at skeys[m], and rows outside the buffer have s > tau >= every
+    // buffered score (s_M = tau when the whole buffer was re-scored).  Its exact distance is therefore at least
+    // s_M + offset - eps.  If the kc-th exact float32 distance is strictly below the float32 rounding of that bound, no such
+    // row can enter (or tie into) the kc nearest.
+    // trusted == 1: the keys are exact and the buffer provably holds the kc nearest (tier 2): nothing to certify.
+    // trusted == 2: the keys are exact but the buffer is still only "every row with approximate score <= tau"
+    // (tier 1): the order inside the buffer is exact, what remains to certify is the rows OUTSIDE it.
+    __shared__ float bound;
+    const bool certify = a.trusted != 1 && status == CRAG_ST_OK && (long long)(a.trusted == 2 ? c : m) < D.n_rows && m > 0 && a.kc > 0;
+    if (tid == T - 64 && certify) {
+        // tightest known lower bound on the approximate score of every row not re-scored
+        const double sM = (m < c && a.trusted == 0) ? (double)crag_fkey_inv((uint32_t)(skeys[m] >> 32)) : (double)a.tau[q];
+        const double u = 5.9604644775390625e-08;  // 2^-24
+        const double X = (double)D.max_xnorm;
+        const double qx = sqrt(qn * X);
+        // 4-bit rows: the scan multiplied pieces of the query (crag_scan_fp4.hip); <what they leave over, x> is at most this
+        const double rest = a.qres ? (double)a.qres[q] * sqrt(X) * 1.0000001 + 1e-34 : 0.0;
+        double eps, lb;
+        if (a.metric == CRAG_L2) {
+            // every partial sum of a scan is bounded by |x|^2 + 2 |q||x|: the 16x16x32 scan starts its accumulators
+            // at |x|^2 (crag_scan_q16.hip); the others add |x|^2 last, which this bound covers as well
+            eps = 2.0 * u * ((double)(a.dim_pad + 4) * (2.0 * qx + X) + 3.0 * X + 1e-30);
+            lb = sM + qn - eps - 2.0 * rest - 1e-12 * (qn + X);
+        } else {
+            eps = 2.0 * u * ((double)(a.dim_pad + 4) * qx + 1e-30);
+            lb = 1.0 + sM - eps - rest - 1e-12 * (1.0 + qx);
+        }
+        float lbf = (float)lb;
+        if ((double)lbf > lb) lbf = nextafterf(lbf, -__builtin_inff());
+        bound = lbf;
+    }
+
     // exact re-scoring: 8 lanes per candidate.  The query and the candidates' rows are first staged in LDS with
     // coalesced 16-byte loads, all in flight at once (the sorted keys occupy skeys[0 .. m]; the rest of that
     // 128-KiB region is free now), so the order-defining add chains read LDS instead of chasing 2-byte loads
@@ -859,38 +892,8 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
     }
     __syncthreads();
 
-    // exactness certificate.  Every row that was NOT re-scored has approximate score >= s_M: the
-    // buffer is sorted, so the remaining candidates start at skeys[m], and rows outside the buffer
-    // have s > tau >= every buffered score (s_M = tau when the whole buffer was re-scored).  Its exact distance is therefore at least
-    // s_M + offset - eps.  If the kc-th exact float32 distance is strictly below the float32
-    // rounding of that bound, no such row can enter (or tie into) the kc nearest.
     if (tid == 0) {
-        // trusted == 1: the keys are exact and the buffer provably holds the kc nearest (tier 2): nothing to certify.
-        // trusted == 2: the keys are exact but the buffer is still only "every row with approximate score <= tau"
-        // (tier 1): the order inside the buffer is exact, what remains to certify is the rows OUTSIDE it.
-        if (a.trusted != 1 && status == CRAG_ST_OK && (long long)(a.trusted == 2 ? c : m) < D.n_rows && kc_valid > 0) {
-            // tightest known lower bound on the approximate score of every row not re-scored
-            const double sM = (m < c && a.trusted == 0) ? (double)crag_fkey_inv((uint32_t)(skeys[m] >> 32)) : (double)a.tau[q];
-            const double u = 5.9604644775390625e-08;  // 2^-24
-            const double X = (double)D.max_xnorm;
-            const double qx = sqrt(qn * X);
-            // 4-bit rows: the scan multiplied pieces of the query (crag_scan_fp4.hip); <what they leave over, x> is at most this
-            const double rest = a.qres ? (double)a.qres[q] * sqrt(X) * 1.0000001 + 1e-34 : 0.0;
-            double eps, lb;
-            if (a.metric == CRAG_L2) {
-                // every partial sum of a scan is bounded by |x|^2 + 2 |q||x|: the 16x16x32 scan starts its accumulators
-                // at |x|^2 (crag_scan_q16.hip); the others add |x|^2 last, which this bound covers as well
-                eps = 2.0 * u * ((double)(a.dim_pad + 4) * (2.0 * qx + X) + 3.0 * X + 1e-30);
-                lb = sM + qn - eps - 2.0 * rest - 1e-12 * (qn + X);
-            } else {
-                eps = 2.0 * u * ((double)(a.dim_pad + 4) * qx + 1e-30);
-                lb = 1.0 + sM - eps - rest - 1e-12 * (1.0 + qx);
-            }
-            float lbf = (float)lb;
-            if ((double)lbf > lb) lbf = nextafterf(lbf, -__builtin_inff());
-            const float dk = crag_fkey_inv(kth_bits);
-            if (!(dk < lbf)) status = CRAG_ST_UNCERTIFIED;
-        }
+        if (certify && !(crag_fkey_inv(kth_bits) < bound)) status = CRAG_ST_UNCERTIFIED;
         a.status[q] = status;
     }
     if (!a.out_ids) return;
