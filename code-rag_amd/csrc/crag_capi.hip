@@ -714,6 +714,11 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     Fp4Args fa = {};
     const float* qres = nullptr;
     const int many = fp4 && B > h0->n_cus && P.sample_stride <= 8192;
+    // 4-bit rows: where no collection has more rows than its sample, k_finalize selects from the sample itself, without a pass
+    // for a threshold in between (1 x 8000 x 384: 20.0 us in two launches, 17.3 in one).  The fallback still wants that pass.
+    bool sample_is_all = fp4 && P.sample_stride <= 8192;
+    for (int b = 0; b < B; ++b) sample_is_all = sample_is_all && qd[(size_t)b].n_rows <= qd[(size_t)b].n_sample;
+    KthArgs kth0 = {};
     if (fp4) {
         const bool narrow = !P.mfma || B <= CRAG_FP4_GROUP_Q;
         const int n_blocks = P.mfma ? crag_fp4_query_blocks(B, h0->dim_pad) : (int)gd.size();
@@ -829,7 +834,8 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         k.seed_n_seg = n_seg;
         k.seed_seg_cap = seg_cap;
         k.seed_stride = cand_stride;
-        if (crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
+        kth0 = k;
+        if (!sample_is_all && crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         // filter levels [n0, n1), [n1, n2), ..., [.., N): each tightens tau from everything found so far
         const LevelBounds nb = cascade_bounds(N, n0, P.M, fp4);
         long long from = n0;
@@ -890,7 +896,8 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
             k.many = many;
             k.seed_cand = cand;  // later passes continue behind the sample rows
             k.seed_cnt = cnt;
-            if (crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
+            kth0 = k;
+            if (!sample_is_all && crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         }
         // level 1: filtered scan of rows [n0, n1) -> tau1 (tightens tau0; never loosens it)
         if (P.need_mid) {
@@ -960,8 +967,13 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     f.symbol_boost = mo ? mo->symbol_boost : 0.0;
     f.qmap = nullptr;
     f.many = many;
+    if (sample_is_all) {
+        f.sample = sample;
+        f.sample_stride = P.sample_stride;
+    }
     if ((rc = crag_launch_finalize(f, st))) return fail(CRAG_E_HIP, "finalize launch failed");
     f.many = 0;
+    f.sample = nullptr;
     f.out_ids = nullptr;  // the fallback tiers patch entries; the rerank then runs once more, over all of them
     auto merge = [&]() -> int {
         if (!mo) return 0;
@@ -997,6 +1009,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         if (noalloc)  // the exact scan needs 8 bytes per row of the collection: not in a fixed scratch array
             return fail(CRAG_E_INEXACT, "crag_search_device_noalloc: a query failed its exactness certificate and needs the exact "
                                         "fallback scan (8 bytes of workspace per row); call crag_search_device for this batch");
+        if (sample_is_all && crag_launch_kth(kth0, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         // device list of the failed queries (tier 1 takes the uncertified ones first, tier 2 whatever is left)
         const size_t nf = failed.size();
         if ((rc = ws->ensure_pinned(sizeof(int) * nf))) return rc;
@@ -1134,6 +1147,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         }
     }
     if (patched && merge()) return fail(CRAG_E_HIP, "merge_rerank launch failed");
+    if (patched) HIPCHK(stream_wait(st));
     return 0;
 }
 
@@ -1667,7 +1681,6 @@ int crag_search_device(crag_index* h, const void* queries_dev, int B, int top_k,
     mo.counts = out_counts_dev;
     rc = search_entries(hs.data(), true, q, B, top_k, q_hashes_dev, q_hash_off_dev, (CragEntry*)ws->entries.p, ws, st, &mo);
     if (rc) return rc;
-    HIPCHK(stream_wait(st));  // only non-trivial after a fallback re-merge
     return 0;
 }
 
@@ -1731,7 +1744,6 @@ int crag_search_multi_device(crag_index* const* hs, const void* queries_dev, int
     mo.counts = out_counts_dev;
     rc = search_entries(hs, same, q, B, top_k, q_hashes_dev, q_hash_off_dev, (CragEntry*)ws->entries.p, ws, st, &mo);
     if (rc) return rc;
-    HIPCHK(stream_wait(st));  // only non-trivial after a fallback re-merge
     return 0;
 }
 

@@ -211,6 +211,10 @@ struct FinalizeArgs {
     double symbol_boost;
     const int* qmap;                  // null: block b serves query b; else block b serves query qmap[b] (fallback passes)
     int many;                         // 4-bit rows, more queries than CUs, trusted == 0: smaller blocks
+    // 4-bit rows, trusted == 0, may be null: no collection of the batch has more rows than its sample (at most 8192).  The
+    // candidates are then all rows, and their ordered scores are here, [B][sample_stride]; cand, cnt and tau are not read
+    const uint32_t* sample;
+    long long sample_stride;
 };
 int crag_launch_finalize(const FinalizeArgs& a, hipStream_t s);
 int crag_launch_merge_rerank(const CragEntry* entries, int G, int B, int kc, int top_k, double symbol_boost,

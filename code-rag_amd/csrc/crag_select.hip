@@ -602,7 +602,9 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
     unsigned int status = CRAG_ST_OK;
     const bool seg = a.n_seg > 0;
     int c;
-    if (seg) {
+    if (a.sample) {
+        c = (int)D.n_rows;
+    } else if (seg) {
         bool ov;
         c = block_seg_offsets<T>(a.segcnt + (long long)q * a.n_seg, a.n_seg, a.seg_cap, seg_off, sel_scratch, &ov);
         if (ov || c > CRAG_CAND_CAP) status = CRAG_ST_OVERFLOW;
@@ -619,7 +621,50 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
     // re-scored, bounds the certificate).  Small buffers are sorted whole; big ones are first cut down to the
     // candidates whose score is <= the (m + 1)-th smallest score (selection), and only those are sorted.
     int c_sorted = c;
-    if (c > 256) {
+    if (a.sample) {
+        // every row: its score into LDS, the m + 1 smallest scores and their ties from there, behind them
+        uint32_t* scores = (uint32_t*)skeys;  // [8192]
+        unsigned long long* gathered = skeys + KEYS - FIN_GATHER;
+        const uint32_t* __restrict__ src = a.sample + (long long)q * a.sample_stride;
+        for (int i0 = tid; i0 < c; i0 += 8 * T) {
+            uint32_t k[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i0 + u * T < c) k[u] = src[i0 + u * T];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i0 + u * T < c) scores[i0 + u * T] = k[u];
+        }
+        if (tid == 0) *sel_count = 0;
+        __syncthreads();
+        if (c > 0) {
+            const uint32_t t = block_select<T>(
+                [&](auto f) {
+#pragma unroll 4
+                    for (int i = tid; i < c; i += T) f(scores[i]);
+                },
+                (uint32_t)(m < c ? m : c - 1), sel_scratch);
+            for (int i = tid; i < c; i += T) {
+                const uint32_t k = scores[i];
+                if (k <= t) {
+                    const uint32_t p = atomicAdd(sel_count, 1u);
+                    if (p < FIN_GATHER) gathered[p] = ((unsigned long long)k << 32) | (uint32_t)i;
+                }
+            }
+            __syncthreads();
+            const uint32_t L = *sel_count;
+            if (ALL && L > FIN_GATHER) {  // ties: all rows are sorted
+                __syncthreads();
+                for (int i = tid; i < c; i += T) skeys[KEYS / 2 + i] = ((unsigned long long)scores[i] << 32) | (uint32_t)i;
+                __syncthreads();
+                for (int i = tid; i < c; i += T) skeys[i] = skeys[KEYS / 2 + i];
+            } else {
+                if (L > FIN_GATHER) status = CRAG_ST_OVERFLOW;
+                c_sorted = L < FIN_GATHER ? (int)L : FIN_GATHER;
+                for (int i = tid; i < c_sorted; i += T) skeys[i] = gathered[i];
+            }
+        }
+    } else if (c > 256) {
         const bool held = ALL || c <= KEYS - FIN_GATHER;  // (else every pass reads them where they lie)
         if (held) {
             if (seg) {
