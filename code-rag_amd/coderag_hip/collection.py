@@ -244,12 +244,11 @@ class GpuCollection:
             self.finalize()
         self._check_tensor(queries)
         b = queries.shape[0]
-        dev = queries.device
         if out is None:
-            out = (torch.empty((b, top_k), dtype=torch.int64, device=dev),
-                   torch.empty((b, top_k), dtype=torch.float64, device=dev),
-                   torch.empty((b, top_k), dtype=torch.float32, device=dev),
-                   torch.empty((b,), dtype=torch.int32, device=dev))
+            out = (queries.new_empty((b, top_k), dtype=torch.int64),
+                   queries.new_empty((b, top_k), dtype=torch.float64),
+                   queries.new_empty((b, top_k), dtype=torch.float32),
+                   queries.new_empty((b,), dtype=torch.int32))
         st = _lib.current_stream(self.device) if stream is None else stream
         check(self._lib.crag_search_device(self._h, queries.data_ptr(), b, int(top_k), float(symbol_boost),
                                            None if q_hashes is None else q_hashes.data_ptr(),
@@ -371,13 +370,12 @@ def search_multi_device(collections: List[GpuCollection], queries, top_k: int = 
         if not c._finalized:
             c.finalize()
     collections[0]._check_tensor(queries)
-    dev = queries.device
     hs = (C.c_void_p * b)(*[c.handle for c in collections])
     if out is None:
-        out = (torch.empty((b, top_k), dtype=torch.int64, device=dev),
-               torch.empty((b, top_k), dtype=torch.float64, device=dev),
-               torch.empty((b, top_k), dtype=torch.float32, device=dev),
-               torch.empty((b,), dtype=torch.int32, device=dev))
+        out = (queries.new_empty((b, top_k), dtype=torch.int64),
+               queries.new_empty((b, top_k), dtype=torch.float64),
+               queries.new_empty((b, top_k), dtype=torch.float32),
+               queries.new_empty((b,), dtype=torch.int32))
     st = _lib.current_stream(collections[0].device) if stream is None else stream
     check(lib.crag_search_multi_device(hs, queries.data_ptr(), b, int(top_k), float(symbol_boost),
                                        None if q_hashes is None else q_hashes.data_ptr(),
