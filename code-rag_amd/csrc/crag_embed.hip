@@ -164,10 +164,10 @@ struct Row {
         }
     }
 };
-// rows in flight per group of lanes
+// rows in flight per group of lanes: what leaves registers for three waves a SIMD (516 float32 elements: four 99 us, two 90)
 template <int DT, int VEC, int NV>
 constexpr int rows_ahead() {
-    return Raw<DT, VEC>::WORDS * NV <= 4 ? 8 : (Raw<DT, VEC>::WORDS * NV <= 24 ? 4 : 2);
+    return Raw<DT, VEC>::WORDS * NV <= 4 ? 8 : (Raw<DT, VEC>::WORDS * NV <= 12 ? 4 : 2);
 }
 
 // Last entry of off[0 .. n] that is <= p, as its index (-1: none)
@@ -238,11 +238,17 @@ __device__ __forceinline__ void zero_absent(const CragSegArgs& a, long long bloc
     }
 }
 
+// Waves a SIMD that k_segsum is built for (rows of up to twelve elements a lane fit by themselves) and its shares are cut for.
+// With three, rows of 24 elements a lane keep a few values in
+// scratch, and still two waves with a second round of shares half empty are slower (8192 bags of 300 tokens x 768 bf16: 262 us
+// against 279); four cost too many (1070).
+constexpr int SEG_WAVES = 3;
+
 // One group of lpr lanes walks the positions [g * share, (g + 1) * share).  A segment that lies whole in a share is stored:
 // backward that is the token's gradient, forward a plain sum for k_embed_finish (scale, norm and count would cost this
 // kernel's registers half of its waves).
 template <int DT, bool BWD, int VEC, int NV>
-__global__ __launch_bounds__(256) void k_segsum(CragSegArgs a) {
+__global__ __launch_bounds__(256, VEC * NV > 12 && VEC * NV <= 24 ? SEG_WAVES : 1) void k_segsum(CragSegArgs a) {
     constexpr int U = rows_ahead<DT, VEC, NV>();
     if constexpr (BWD) {
         if ((long long)blockIdx.x >= a.sum_blocks) {
@@ -1047,7 +1053,7 @@ int vec_of(int dim, int esz, const void* p) {
 // positions each: a segment that crosses a border costs a row written and read again, and a second round of waves that is
 // not full costs half a round (1M tokens of 384 float32: 168 positions a group 120 us, 128 141 us).
 int share_of(long long n, int lpr) {
-    const long long groups = 256ll * 12 * (64 / lpr);
+    const long long groups = 256ll * 4 * SEG_WAVES * (64 / lpr);
     return (int)std::max<long long>(8, ((n + groups - 1) / groups + 7) / 8 * 8);
 }
 
