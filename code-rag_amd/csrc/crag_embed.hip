@@ -246,7 +246,9 @@ constexpr int SEG_WAVES = 3;
 
 // One group of lpr lanes walks the positions [g * share, (g + 1) * share).  A segment that lies whole in a share is stored:
 // backward that is the token's gradient, forward a plain sum for k_embed_finish (scale, norm and count would cost this
-// kernel's registers half of its waves).
+// kernel's registers half of its waves).  Bound by what the caches deliver to a gather, 13 .. 15 TB/s of rows where tokens are
+// as uneven as text's, and for bf16 rows by the vector units as well, which unpack (busy two thirds of the cycles): 1M tokens
+// of 384 float32 147 us, 2.5M of 768 bf16 246; backward 1M positions of 384 with 400 MB of gradient 120.
 template <int DT, bool BWD, int VEC, int NV>
 __global__ __launch_bounds__(256, VEC * NV > 12 && VEC * NV <= 24 ? SEG_WAVES : 1) void k_segsum(CragSegArgs a) {
     constexpr int U = rows_ahead<DT, VEC, NV>();
@@ -467,7 +469,7 @@ __device__ __forceinline__ int join_rows(const CragSegArgs& a, int n, int grp, i
 }
 
 // Forward, after k_segsum: every bag, from its sum or, where it crosses borders of shares, from its partial sums.  `gp` groups
-// of lanes per bag.
+// of lanes per bag.  (1024 bags of 384: 9 us, 8192 of 768: 16.)
 template <int VEC, int NV>
 __global__ __launch_bounds__(256) void k_embed_finish(CragSegArgs a, int gp) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -613,7 +615,7 @@ __global__ __launch_bounds__(BAG_THREADS) void k_embed_bag(CragSegArgs a) {
 
 // Backward, after k_segsum: a token whose first partial sum is share g's tail goes on through the heads of the shares behind
 // it.  A block looks at four shares, one to a wave; a wave joins up to JOIN_ALONE rows by itself, longer ones (frequent tokens)
-// take the whole block.
+// take the whole block.  (1M tokens, one of them a twentieth of all: 12.5 us, most of it that one's.)
 constexpr int JOIN_ALONE = 16;
 template <int VEC, int NV>
 __global__ __launch_bounds__(256) void k_segjoin(CragSegArgs a) {
@@ -715,7 +717,8 @@ __device__ __forceinline__ unsigned long long same_digit(uint32_t d, int bits, b
 }
 
 // Up to SORT_SMALL positions: block 0 makes the keys and sorts (key, position) in LDS, stable, 8 bits a pass; the other blocks
-// do dp.  One launch for all that comes in front of the sums.
+// do dp.  One launch for all that comes in front of the sums.  (3200 positions: 14 us, two passes of five barriers each in the
+// one workgroup; the launches of the general sort alone would take longer.)
 constexpr int SORT_SMALL = 8192;
 __global__ __launch_bounds__(1024) void k_bwd_start_small(BwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -797,7 +800,8 @@ __global__ __launch_bounds__(1024) void k_bwd_start_small(BwdArgs a) {
 }
 
 // More: stable least-significant-digit radix sort with digits of up to SORT_BITS bits -- counts per tile, prefix per digit,
-// ordered scatter.  The first launch makes the keys and counts their first digit; its other blocks do dp.
+// ordered scatter.  The first launch makes the keys and counts their first digit; its other blocks do dp.  (1M positions, 18-bit
+// keys: 16 us for that launch, then two passes of 5 + 17 us, the second with 10 for its counts.)
 constexpr int SORT_BITS = 10, SORT_TILE = 2048, SORT_PER = SORT_TILE / 256;
 __global__ __launch_bounds__(256) void k_bwd_start(BwdArgs a) {
     __shared__ uint32_t h[1 << SORT_BITS];
@@ -950,7 +954,10 @@ __device__ __forceinline__ float add_lanes(float v, int lpr) {
     return v;
 }
 
-// dw_t = <dp_b, E[id_t]>; groups of lanes over shares of the positions, as in k_segsum
+// dw_t = <dp_b, E[id_t]>; groups of lanes over shares of the positions, as in k_segsum.  In the order of the positions, where
+// dp_b stays in registers and the caches may hold the forward pass's rows of the table (1M tokens of 384 float32: 111 us =
+// 14 TB/s).  Taken along by k_segsum over the sorted positions, which has dp_b at hand and a table row for several positions,
+// the two together took 270 us instead of 231: the sums across lanes leave too few loads in flight.
 template <int DT, int VEC, int NV>
 __global__ __launch_bounds__(256) void k_embed_dweights(CragSegArgs a, const void* __restrict__ table, const int* __restrict__ ids,
                                                         float* __restrict__ dw) {
