@@ -247,7 +247,7 @@ constexpr int SEG_WAVES = 3;
 // One group of lpr lanes walks the positions [g * share, (g + 1) * share).  A segment that lies whole in a share is stored:
 // backward that is the token's gradient, forward a plain sum for k_embed_finish (scale, norm and count would cost this
 // kernel's registers half of its waves).  Bound by what the caches deliver to a gather, 13 .. 15 TB/s of rows where tokens are
-// as uneven as text's, and for bf16 rows by the vector units as well, which unpack (busy two thirds of the cycles): 1M tokens
+// as uneven as text's, and for bf16 rows by the vector units as well, which unpack (busy 60 % of the cycles): 1M tokens
 // of 384 float32 147 us, 2.5M of 768 bf16 246; backward 1M positions of 384 with 400 MB of gradient 120.
 template <int DT, bool BWD, int VEC, int NV>
 __global__ __launch_bounds__(256, VEC * NV > 12 && VEC * NV <= 24 ? SEG_WAVES : 1) void k_segsum(CragSegArgs a) {
