@@ -189,6 +189,34 @@ def test_awkward_rows_in_batches_of_every_size(kind, b, top_k):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("b,top_k", [(300, 10), (300, 200), (1030, 1), (5, 25), (1, 200)])
+@pytest.mark.parametrize("rows", ["all equal", "five of each", "one step apart", "seven"])
+def test_small_collections_that_are_selected_from_their_scores(rows, b, top_k):
+    """up to 8192 rows: no threshold in between, with ties that fill the room for them and queries that are not certified"""
+    import torch
+    x = {"all equal": lambda: np.repeat(unit(1, 96, 1), 8000, 0), "five of each": lambda: np.repeat(unit(1638, 96, 2), 5, 0),
+         "one step apart": lambda: np.repeat(unit(1, 96, 3), 8192, 0) + np.eye(96, dtype=np.float32)[np.arange(8192) % 96] * 0.02,
+         "seven": lambda: unit(7, 96, 4)}[rows]()
+    col = collection(x)
+    ref = ch.GpuCollection(96, "f32")
+    ref.add(col.rows_host())
+    q = torch.from_numpy(unit(b, 96, 9)).cuda()
+    for got, want in zip(col.search_device(q, top_k), ref.search_device(q, top_k)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("sizes", [(0, 5, 8192, 8000, 33, 1), (0, 20000, 5, 8192)])
+def test_collections_of_all_sizes_in_one_call(sizes):
+    import torch
+    cols = [collection(unit(n, 64, n)) for n in sizes] * 60     # one query each: more queries than CUs
+    q = torch.from_numpy(unit(len(cols), 64, 3)).cuda()
+    got = ch.search_multi_device(cols, q, 10)
+    for i, c in enumerate(cols):
+        want = c.search_device(q[i:i + 1], 10)
+        for a, w in zip(got, want):
+            assert torch.equal(a[i:i + 1], w), (i, len(c))
+
+
 def test_rows_added_in_pieces_and_profiled():
     import torch
     rows, cls = unit(9000, 100, 4), (np.arange(9000) % 3).astype(np.uint8)
