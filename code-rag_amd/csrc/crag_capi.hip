@@ -586,6 +586,14 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     const bool segmented = P.mfma && (can_q16 || fp4_seg > 0);
     const bool cascade = P.mfma;
     // ---- descriptors ----
+    // 4-bit rows: where every collection is small, k_finalize selects from the scores of all rows, without thresholds and further
+    // levels in between (1 x 8000 x 384: two selections 20.0 us, one 17.3; searches of 20 000 x 384, 1 query top 10 58 against 53 us,
+    // 100 queries top 100 86 against 69, 64 collections of them 119 against 110).  Scores of more than
+    // 4M rows for all queries together are not worth their way through memory.
+    long long n_most = 0;
+    for (int b = 0; b < B; ++b) n_most = std::max<long long>(n_most, hs[b]->n_rows);
+    const bool sample_is_all = fp4 && (n_most <= 8192 || (n_most <= CRAG_FP4_DENSE_ROWS && B <= h0->n_cus && !ws->arena && n_most * B <= (4ll << 20)));
+    const long long dense_rows = sample_is_all ? n_most : 0;
     SmallVec<QueryDesc, 64> qd;
     qd.resize((size_t)B);
     SmallVec<GroupDesc, 64> gd;
@@ -597,7 +605,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         d.name_hash = (const unsigned long long*)h->name_hash;
         d.path_class = h->path_class;
         d.n_rows = h->n_rows;
-        d.n_sample = level0_rows(h->n_rows, fp4 ? 0 : P.M);
+        d.n_sample = fp4 && h->n_rows <= dense_rows ? h->n_rows : level0_rows(h->n_rows, fp4 ? 0 : P.M);
         // (4-bit rows: a level costs more than the survivors it saves; 64 collections x 20k rows 146 -> 130 us without level 1)
         d.n_mid = level1_rows(h->n_rows, d.n_sample, P.M, P.mfma || fp4 ? CRAG_CAND_CAP / 8 : std::max(32.0, 2048.0 / B));
         d.id_base = h->id_base;
@@ -714,11 +722,6 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
     Fp4Args fa = {};
     const float* qres = nullptr;
     const int many = fp4 && B > h0->n_cus && P.sample_stride <= 8192;
-    // 4-bit rows: where no collection has more rows than its sample, k_finalize selects from the sample itself, without a pass
-    // for a threshold in between (1 x 8000 x 384: 20.0 us in two launches, 17.3 in one).  The fallback still wants that pass.
-    bool sample_is_all = fp4 && P.sample_stride <= 8192;
-    for (int b = 0; b < B; ++b) sample_is_all = sample_is_all && qd[(size_t)b].n_rows <= qd[(size_t)b].n_sample;
-    KthArgs kth0 = {};
     if (fp4) {
         const bool narrow = !P.mfma || B <= CRAG_FP4_GROUP_Q;
         const int n_blocks = P.mfma ? crag_fp4_query_blocks(B, h0->dim_pad) : (int)gd.size();
@@ -834,7 +837,6 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         k.seed_n_seg = n_seg;
         k.seed_seg_cap = seg_cap;
         k.seed_stride = cand_stride;
-        kth0 = k;
         if (!sample_is_all && crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         // filter levels [n0, n1), [n1, n2), ..., [.., N): each tightens tau from everything found so far
         const LevelBounds nb = cascade_bounds(N, n0, P.M, fp4);
@@ -896,7 +898,6 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
             k.many = many;
             k.seed_cand = cand;  // later passes continue behind the sample rows
             k.seed_cnt = cnt;
-            kth0 = k;
             if (!sample_is_all && crag_launch_kth(k, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         }
         // level 1: filtered scan of rows [n0, n1) -> tau1 (tightens tau0; never loosens it)
@@ -1009,7 +1010,6 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         if (noalloc)  // the exact scan needs 8 bytes per row of the collection: not in a fixed scratch array
             return fail(CRAG_E_INEXACT, "crag_search_device_noalloc: a query failed its exactness certificate and needs the exact "
                                         "fallback scan (8 bytes of workspace per row); call crag_search_device for this batch");
-        if (sample_is_all && crag_launch_kth(kth0, st)) return fail(CRAG_E_HIP, "kth (level 0) launch failed");
         // device list of the failed queries (tier 1 takes the uncertified ones first, tier 2 whatever is left)
         const size_t nf = failed.size();
         if ((rc = ws->ensure_pinned(sizeof(int) * nf))) return rc;
@@ -1025,7 +1025,7 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         // beyond the slack at the cost of a few thousand row reads per query.
         SmallVec<int, 64> t1;
         for (int b : failed)
-            if (hst[(size_t)b] == CRAG_ST_UNCERTIFIED) t1.push_back(b);
+            if (hst[(size_t)b] == CRAG_ST_UNCERTIFIED && !sample_is_all) t1.push_back(b);  // (no buffer was filled there)
         if (!t1.empty()) {
             if ((rc = upload_qmap(t1))) return rc;
             FinalizeArgs g = f;

@@ -185,6 +185,7 @@ struct KthArgs {
     int many;  // 4-bit rows (samples of at most 8192), more queries than CUs: blocks of 256 threads
 };
 int crag_launch_kth(const KthArgs& a, hipStream_t s);
+constexpr int CRAG_FP4_DENSE_ROWS = 28672;  // scores that k_finalize can hold beside the candidates it gathers from them
 struct FinalizeArgs {
     const QueryDesc* qd;
     const void* queries;
@@ -211,8 +212,9 @@ struct FinalizeArgs {
     double symbol_boost;
     const int* qmap;                  // null: block b serves query b; else block b serves query qmap[b] (fallback passes)
     int many;                         // 4-bit rows, more queries than CUs, trusted == 0: smaller blocks
-    // 4-bit rows, trusted == 0, may be null: no collection of the batch has more rows than its sample (at most 8192).  The
-    // candidates are then all rows, and their ordered scores are here, [B][sample_stride]; cand, cnt and tau are not read
+    // 4-bit rows, trusted == 0, may be null: no collection of the batch has more rows than its sample (at most
+    // CRAG_FP4_DENSE_ROWS, 8192 with `many`).  The candidates are then all rows, and their ordered scores are here,
+    // [B][sample_stride]; cand, cnt and tau are not read
     const uint32_t* sample;
     long long sample_stride;
 };

@@ -623,7 +623,8 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
     int c_sorted = c;
     if (a.sample) {
         // every row: its score into LDS, the m + 1 smallest scores and their ties from there, behind them
-        uint32_t* scores = (uint32_t*)skeys;  // [8192]
+        uint32_t* scores = (uint32_t*)skeys;  // [2 * (KEYS - FIN_GATHER)]
+        static_assert(!ALL || 2 * (KEYS - FIN_GATHER) == CRAG_FP4_DENSE_ROWS, "rows whose scores fit");
         unsigned long long* gathered = skeys + KEYS - FIN_GATHER;
         const uint32_t* __restrict__ src = a.sample + (long long)q * a.sample_stride;
         for (int i0 = tid; i0 < c; i0 += 8 * T) {
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(T) void k_finalize(FinalizeArgs a) {
             }
             __syncthreads();
             const uint32_t L = *sel_count;
-            if (ALL && L > FIN_GATHER) {  // ties: all rows are sorted
+            if (ALL && L > FIN_GATHER && c <= KEYS / 2) {  // ties: all rows are sorted
                 __syncthreads();
                 for (int i = tid; i < c; i += T) skeys[KEYS / 2 + i] = ((unsigned long long)scores[i] << 32) | (uint32_t)i;
                 __syncthreads();

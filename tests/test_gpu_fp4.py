@@ -205,6 +205,19 @@ def test_small_collections_that_are_selected_from_their_scores(rows, b, top_k):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("b,top_k", [(1, 10), (17, 200), (140, 25), (150, 3)])
+@pytest.mark.parametrize("n,copies", [(8193, 1), (20000, 5), (28672, 1), (28672, 28672), (28673, 1), (20000, 2500)])
+def test_collections_around_the_limit_of_that(n, copies, b, top_k):
+    import torch
+    x = np.repeat(unit(n // copies, 70, n), copies, 0)
+    col = collection(x)
+    ref = ch.GpuCollection(70, "f32")
+    ref.add(col.rows_host())
+    q = torch.from_numpy(unit(b, 70, 9)).cuda()
+    for got, want in zip(col.search_device(q, top_k), ref.search_device(q, top_k)):
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("sizes", [(0, 5, 8192, 8000, 33, 1), (0, 20000, 5, 8192)])
 def test_collections_of_all_sizes_in_one_call(sizes):
     import torch
