@@ -366,6 +366,33 @@ def test_gradients_of_every_form():
         y.sum().backward()
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f32", 3000000), ("bf16", 6000000)])
+def test_rows_behind_four_gib(dtype, vocab):
+    import torch
+    dim = 768
+    table = torch.zeros((vocab, dim), dtype=torch.float32 if dtype == "f32" else torch.bfloat16, device="cuda")
+    r = np.random.default_rng(3)
+    used = np.unique(np.concatenate([[0, 1, vocab // 2, vocab - 2, vocab - 1], r.integers(0, vocab, 400)]))
+    small = torch.from_numpy(r.standard_normal((len(used), dim)).astype(np.float32)).to(table.dtype)
+    table[torch.from_numpy(used).cuda()] = small.cuda()
+    at = r.integers(0, len(used), 9000)
+    offsets = np.arange(0, 9001, 300)
+    w = r.standard_normal(9000).astype(np.float32)
+    grad = torch.from_numpy(r.standard_normal((30, dim)).astype(np.float32))
+    (y, yb), (de, deb), (dw, dwb) = plain(small, at.astype(np.int32), offsets, w, "mean", 1.0, True, grad)
+    table.requires_grad_(True)
+    _, ids, off, wd = gpu(small, used[at].astype(np.int32), offsets, w)
+    wd.requires_grad_(True)
+    got = ch.embed_bags(table, ids, off, wd)
+    within(got, y, yb)
+    g, gw = torch.autograd.grad(got, (table, wd), grad.cuda())
+    within(gw, dw, dwb)
+    rows = torch.from_numpy(used).cuda()
+    within(g[rows], de, deb, bf16=dtype == "bf16")
+    assert int((g != 0).any(1).sum()) <= len(used)
+    del g
+
+
 def test_two_threads_on_streams_of_their_own():
     import threading
     import torch

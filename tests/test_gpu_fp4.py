@@ -230,6 +230,30 @@ def test_collections_of_all_sizes_in_one_call(sizes):
             assert torch.equal(a[i:i + 1], w), (i, len(c))
 
 
+@pytest.mark.parametrize("b", [1, 40, 260])
+def test_rows_behind_four_gib(b):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = torch.randn((1000000, 768), generator=g, device="cuda")
+    col = ch.GpuCollection(768, "fp4")
+    q = torch.randn((b, 768), generator=g, device="cuda")
+    for i in range(11):
+        col.add_device(rows * (1 + 0.01 * i))
+    near = q.repeat_interleave(12, 0) * torch.linspace(1.0, 0.9, 12, device="cuda").repeat(b)[:, None]
+    rows[-len(near):] = near                       # the last rows of all: twelve near each query, ever farther
+    col.add_device(rows)
+    assert len(col) * (384 + 24) > 2 ** 32
+    ids, _, dist, count = col.search_device(q, 6)
+    first = 12000000 - len(near) + 12 * torch.arange(b, device="cuda")
+    assert count.eq(6).all()
+    held = torch.from_numpy(col.rows_host(12000000 - len(near), len(near))).cuda().double().view(b, 12, 768)
+    exact = ((held - q.double()[:, None]) ** 2).sum(2)
+    order = exact.argsort(1)[:, :6]
+    assert torch.equal(ids, first[:, None] + order)
+    # float32 of a float64 sum: one rounding, and the sum's own
+    assert ((dist.double() - exact.gather(1, order)).abs() <= exact.gather(1, order) * (2.0 ** -24 + 2.0 ** -40) + 1e-30).all()
+
+
 def test_rows_added_in_pieces_and_profiled():
     import torch
     rows, cls = unit(9000, 100, 4), (np.arange(9000) % 3).astype(np.uint8)
