@@ -728,9 +728,15 @@ int search_entries_chunk_launch(crag_index* const* hs, bool same_handle, const v
         const size_t piece_bytes = (size_t)crag_fp4_query_bytes(n_blocks, h0->dim_pad, narrow);
         if ((rc = ws->qscan.ensure(piece_bytes + sizeof(float) * (size_t)B))) return rc;
         float* res = (float*)((char*)ws->qscan.p + piece_bytes);
-        if (crag_launch_fp4_split(q_dev, P.mfma ? nullptr : gd_dev, n_blocks, B, h0->dim_pad, h0->metric, narrow, ws->qscan.p, res,
-                                  fp4_desc ? &qd[0] : nullptr, fp4_desc ? (QueryDesc*)desc_dev : nullptr, st))
+        if (fp4_desc && h0->n_rows > 0 && crag_fp4_splits_itself(B, h0->dim_pad)) {
+            fa.raw = (const float*)q_dev;  // (taken by the sample's scan only)
+            fa.residual = res;
+            fa.desc = qd[0];
+            fa.desc_out = (QueryDesc*)desc_dev;
+        } else if (crag_launch_fp4_split(q_dev, P.mfma ? nullptr : gd_dev, n_blocks, B, h0->dim_pad, h0->metric, narrow, ws->qscan.p, res,
+                                         fp4_desc ? &qd[0] : nullptr, fp4_desc ? (QueryDesc*)desc_dev : nullptr, st)) {
             return fail(CRAG_E_HIP, "query split launch failed");
+        }
         qres = res;
         fa.queries = ws->qscan.p;
         fa.metric = h0->metric;

@@ -271,6 +271,12 @@ struct Fp4Args {
     // several collections (crag_launch_scan_fp4_groups): query block g holds the queries of group g, at most 16
     const GroupDesc* groups;
     int n_groups, pass;
+    // the first scan of a few queries may split them itself (crag_fp4_splits_itself): the queries as they are, and where their
+    // pieces (`queries`), what these leave over and the descriptors go
+    const float* raw;
+    float* residual;
+    QueryDesc desc;
+    QueryDesc* desc_out;
 };
 #define CRAG_FP4_GROUP_Q 16  // most queries of the narrow form
 int crag_fp4_dim_pad(int dim);  // 0: too long
@@ -281,6 +287,7 @@ int crag_launch_fp4_split(const void* queries, const GroupDesc* groups, int n_bl
                           float* residual, const QueryDesc* desc, QueryDesc* desc_out, hipStream_t s);
 int crag_fp4_segments(int B, int dim_pad, int n_cus);
 int crag_launch_scan_fp4(const Fp4Args& a, int dim_pad, bool filter, int n_cus, hipStream_t s);
+bool crag_fp4_splits_itself(int B, int dim_pad);
 int crag_launch_scan_fp4_groups(const Fp4Args& a, int dim_pad, int blocks, hipStream_t s);
 int crag_launch_fp4_quantize(const float* src, long long n, int dim, int dim_pad, long long first, void* dst, hipStream_t s);
 int crag_launch_fp4_dequantize(const void* rows, long long first, long long n, int dim, int dim_pad, float* out, hipStream_t s);

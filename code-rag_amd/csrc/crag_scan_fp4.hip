@@ -380,38 +380,6 @@ __global__ __launch_bounds__(64 * Ring<KS>::WAVES, Ring<KS>::WAVES / 4) void k_s
     }
 }
 
-// Up to 16 queries on one collection (groups == null), or several collections with groups of up to 16 queries each
-// (GroupDesc, as the float32 and bf16 scans have them).  Bound by HBM: 3.5M rows of 384, the last level of a search through 4M,
-// 107 us = 6.7 TB/s, with both pieces of sixteen queries for the products of one.
-template <int KS, bool FILTER>
-__global__ __launch_bounds__(256) void k_scan_fp4_narrow(Fp4Args a) {
-    __shared__ __attribute__((aligned(16))) unsigned char stage[4 * 1024 * chunk_steps(KS, 1)];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int bid = blockIdx.x, c = lane & 31;
-    Query<KS, 1> q[1];
-    if (!a.groups) {
-        q[0].load((const unsigned char*)a.queries, lane);
-        const int qid[1] = {c < 16 && c < a.n_queries ? c : -1};
-        const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[c] : __builtin_nanf("")};
-        walk<KS, 1, 1, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + (long long)bid * 4 + wave, (long long)gridDim.x * 4, (a.row_end + 31) >> 5,
-                               a.row_end, a, q, tau, qid, lane, stage + wave * 1024 * chunk_steps(KS, 1));
-        return;
-    }
-    int g = 0;
-    for (int hi = a.n_groups; hi - g > 1;) {  // the last group whose first block is <= bid
-        const int mid = (g + hi) >> 1;
-        if (a.groups[mid].blk_first[a.pass] <= bid) g = mid; else hi = mid;
-    }
-    const GroupDesc& G = a.groups[g];
-    const long long row_end = a.pass == 0 ? G.n_sample : (a.pass == 1 ? G.n_mid : G.n_rows);
-    q[0].load((const unsigned char*)a.queries + g * crag_fp4_qblock_bytes(KS, 1), lane);
-    const int qid[1] = {c < 16 && c < G.nq ? G.q_first + c : -1};
-    const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[G.q_first + c] : __builtin_nanf("")};
-    const long long first = (long long)(bid - G.blk_first[a.pass]) * 4 + wave;
-    walk<KS, 1, 1, FILTER>(G.rows, G.xnorm, (G.from[a.pass] >> 5) + first, (long long)G.n_blk[a.pass] * 4, (row_end + 31) >> 5, row_end, a, q, tau, qid,
-                           lane, stage + wave * 1024 * chunk_steps(KS, 1));
-}
-
 // ---- queries: float32 -> two E2M3 pieces ---------------------------------------------------------------------------------
 // nearest E2M3 value of t (|t| <= 7.5), its code
 __device__ __forceinline__ float e2m3(float t, uint32_t* code) {
@@ -435,6 +403,126 @@ __device__ __forceinline__ float e2m3(float t, uint32_t* code) {
     return t < 0.f ? -r : r;
 }
 
+// Elements 4 t .. 4 t + 3 of -q, eight lanes to a group of 32: their codes and scales into column `col` of the operand block at
+// `base`.  Returns |what is left of them|^2.
+__device__ __forceinline__ double split_four(f32x4_t v, int t, int ks, int narrow, int col, int metric, unsigned char* base) {
+    const int pieces = narrow ? 1 : 2;
+    const int grp = t >> 3, part = t & 7;
+    int k, half;
+    crag_fp4_step(ks, grp, &k, &half);
+    half *= 32;
+    float big = 0.f;
+    int huge = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        huge |= fabsf(v[j]) <= 1.329227995784916e36f ? 0 : 1;  // 2^120: beyond it nothing is split, and everything left over
+        big = fmaxf(big, fabsf(v[j]));
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            big = fmaxf(big, __shfl_xor(big, o));
+            huge |= __shfl_xor(huge, o);
+        }
+        int ex;
+        const float m = frexpf(big, &ex);
+        int e = ex - (m > 0.9375f ? 2 : 3);  // the smallest with big <= 7.5 * 2^e
+        e = e < -120 || huge ? -120 : e;
+        const float down = ldexpf(1.f, -e), up = ldexpf(1.f, e);
+        uint32_t w = 0;  // 24 bits: this lane's four codes
+        float rest = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t c = 0;
+            if (!huge) {
+                const float r = e2m3(v[j] * down, &c);
+                v[j] -= r * up;
+                rest = fmaxf(rest, fabsf(v[j]));
+            }
+            w |= c << (6 * j);
+        }
+        big = rest;
+        // four lanes' 24 bits are three words
+        const uint32_t w1 = __shfl_down(w, 1, 8), w2 = __shfl_down(w, 2, 8), w3 = __shfl_down(w, 3, 8);
+        const int i = narrow ? k : 2 * k + p, at = half + (narrow ? 16 * p + col : col);
+        if ((part & 3) == 0) {
+            uint32_t* o = (uint32_t*)(base + ((long long)i * 64 + at) * 24 + (part >> 2) * 12);
+            o[0] = w | (w1 << 24);
+            o[1] = (w1 >> 8) | (w2 << 16);
+            o[2] = (w2 >> 16) | (w3 << 8);
+        }
+        // -2q is -q with a scale twice as large
+        if (part == 0)
+            base[64ll * 24 * ks * pieces + (long long)at * 4 * crag_fp4_qsw(ks, pieces) + i] = (unsigned char)(e + 127 + (metric == CRAG_L2 ? 1 : 0));
+    }
+    double left = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) left += (double)v[j] * (double)v[j];
+    return left;
+}
+
+constexpr int SPLIT_QUERIES = 4, SPLIT_ELEMS = 1024, SPLIT_KS = 16;  // one round of a workgroup: with four of them (7 x 1M x 500) nothing is gained
+
+// Up to 16 queries on one collection (groups == null), or several collections with groups of up to 16 queries each
+// (GroupDesc, as the float32 and bf16 scans have them).  Bound by HBM: 3.5M rows of 384, the last level of a search through 4M,
+// 107 us = 6.7 TB/s, with both pieces of sixteen queries for the products of one.
+// SPLIT: the first scan of a search for few queries.  Every workgroup splits them for itself, all together leave the pieces for
+// the scans that follow, the first one what is left over and the descriptors: no launch in front (1 x 8000 x 384: 6.5 us instead of 4.5 and 4.0 and the gap between them).
+template <int KS, bool FILTER, bool SPLIT = false>
+__global__ __launch_bounds__(256) void k_scan_fp4_narrow(Fp4Args a) {
+    __shared__ __attribute__((aligned(16))) unsigned char stage[4 * 1024 * chunk_steps(KS, 1)];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int bid = blockIdx.x, c = lane & 31;
+    Query<KS, 1> q[1];
+    if (!a.groups) {
+        if constexpr (SPLIT) {
+            constexpr int WORDS = (int)crag_fp4_qblock_bytes(KS, 1) / 16;
+            __shared__ __attribute__((aligned(16))) unsigned char block[WORDS * 16];
+            __shared__ double left[SPLIT_QUERIES * 2 * KS];
+            const int tid = threadIdx.x;
+            for (int i = tid; i < WORDS; i += 256) ((u32x4_t*)block)[i] = (u32x4_t){0, 0, 0, 0};
+            __syncthreads();
+            for (int i = tid; i < a.n_queries * 16 * KS; i += 256) {  // whole groups of eight lanes
+                const int col = i / (16 * KS), t = i % (16 * KS);
+                double r = split_four(-*(const f32x4_t*)(a.raw + i * 4), t, KS, 1, col, a.metric, block);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) r += __shfl_xor(r, o);
+                if ((t & 7) == 0) left[col * 2 * KS + (t >> 3)] = r;
+            }
+            __syncthreads();
+            for (int i = bid * 256 + tid; i < WORDS; i += gridDim.x * 256) ((u32x4_t*)const_cast<void*>(a.queries))[i] = ((const u32x4_t*)block)[i];
+            if (bid == 0 && tid < a.n_queries) {
+                double sum = 0.0;
+                for (int g = 0; g < 2 * KS; ++g) sum += left[tid * 2 * KS + g];
+                a.residual[tid] = nextafterf((float)sqrt(sum), __builtin_inff());
+                a.desc_out[tid] = a.desc;
+            }
+            q[0].load(block, lane);
+        } else {
+            q[0].load((const unsigned char*)a.queries, lane);
+        }
+        const int qid[1] = {c < 16 && c < a.n_queries ? c : -1};
+        const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[c] : __builtin_nanf("")};
+        walk<KS, 1, 1, FILTER>(a.rows, a.xnorm, (a.row_begin >> 5) + (long long)bid * 4 + wave, (long long)gridDim.x * 4, (a.row_end + 31) >> 5,
+                               a.row_end, a, q, tau, qid, lane, stage + wave * 1024 * chunk_steps(KS, 1));
+        return;
+    }
+    int g = 0;
+    for (int hi = a.n_groups; hi - g > 1;) {  // the last group whose first block is <= bid
+        const int mid = (g + hi) >> 1;
+        if (a.groups[mid].blk_first[a.pass] <= bid) g = mid; else hi = mid;
+    }
+    const GroupDesc& G = a.groups[g];
+    const long long row_end = a.pass == 0 ? G.n_sample : (a.pass == 1 ? G.n_mid : G.n_rows);
+    q[0].load((const unsigned char*)a.queries + g * crag_fp4_qblock_bytes(KS, 1), lane);
+    const int qid[1] = {c < 16 && c < G.nq ? G.q_first + c : -1};
+    const float tau[1] = {FILTER && qid[0] >= 0 ? a.tau[G.q_first + c] : __builtin_nanf("")};
+    const long long first = (long long)(bid - G.blk_first[a.pass]) * 4 + wave;
+    walk<KS, 1, 1, FILTER>(G.rows, G.xnorm, (G.from[a.pass] >> 5) + first, (long long)G.n_blk[a.pass] * 4, (row_end + 31) >> 5, row_end, a, q, tau, qid,
+                           lane, stage + wave * 1024 * chunk_steps(KS, 1));
+}
+
 // One block per query slot, eight lanes per group of 32 elements, four elements each.  Wide: slot = query, 32 to a block of the
 // operand.  Narrow: 16 slots to a block; with `groups`, block g holds the queries of group g.
 // (1 query of 384 4.5 us, 1024 of 1024 7.8: a launch and three trips to memory.)
@@ -456,57 +544,7 @@ __global__ __launch_bounds__(512) void k_fp4_split(const float* __restrict__ que
     if (tid * 4 < dim_pad) {  // whole groups of eight lanes
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
         if (q >= 0) v = -*(const f32x4_t*)(queries + (long long)q * dim_pad + tid * 4);
-        const int grp = tid >> 3, part = tid & 7;
-        int k, half;
-        crag_fp4_step(ks, grp, &k, &half);
-        half *= 32;
-        float big = 0.f;
-        int huge = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            huge |= fabsf(v[j]) <= 1.329227995784916e36f ? 0 : 1;  // 2^120: beyond it nothing is split, and everything left over
-            big = fmaxf(big, fabsf(v[j]));
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) {
-                big = fmaxf(big, __shfl_xor(big, o));
-                huge |= __shfl_xor(huge, o);
-            }
-            int ex;
-            const float m = frexpf(big, &ex);
-            int e = ex - (m > 0.9375f ? 2 : 3);  // the smallest with big <= 7.5 * 2^e
-            e = e < -120 || huge ? -120 : e;
-            const float down = ldexpf(1.f, -e), up = ldexpf(1.f, e);
-            uint32_t w = 0;  // 24 bits: this lane's four codes
-            float rest = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t c = 0;
-                if (!huge) {
-                    const float r = e2m3(v[j] * down, &c);
-                    v[j] -= r * up;
-                    rest = fmaxf(rest, fabsf(v[j]));
-                }
-                w |= c << (6 * j);
-            }
-            big = rest;
-            // four lanes' 24 bits are three words
-            const uint32_t w1 = __shfl_down(w, 1, 8), w2 = __shfl_down(w, 2, 8), w3 = __shfl_down(w, 3, 8);
-            const int i = narrow ? k : 2 * k + p, at = half + (narrow ? 16 * p + col : col);
-            if ((part & 3) == 0) {
-                uint32_t* o = (uint32_t*)(base + ((long long)i * 64 + at) * 24 + (part >> 2) * 12);
-                o[0] = w | (w1 << 24);
-                o[1] = (w1 >> 8) | (w2 << 16);
-                o[2] = (w2 >> 16) | (w3 << 8);
-            }
-            // -2q is -q with a scale twice as large
-            if (part == 0)
-                base[64ll * 24 * ks * pieces + (long long)at * 4 * crag_fp4_qsw(ks, pieces) + i] = (unsigned char)(e + 127 + (metric == CRAG_L2 ? 1 : 0));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) left += (double)v[j] * (double)v[j];
+        left = split_four(v, tid, ks, narrow, col, metric, base);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) left += __shfl_xor(left, o);
@@ -659,6 +697,12 @@ int launch_wide(const Fp4Args& a, int qb, int blocks, bool filter, hipStream_t s
 }
 template <int KS>
 int launch_narrow(const Fp4Args& a, int blocks, bool filter, hipStream_t s) {
+    if constexpr (KS <= SPLIT_KS) {
+        if (!filter && a.raw) {
+            hipLaunchKernelGGL((k_scan_fp4_narrow<KS, false, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+            return (int)hipGetLastError();
+        }
+    }
     if (filter) hipLaunchKernelGGL((k_scan_fp4_narrow<KS, true>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_scan_fp4_narrow<KS, false>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     return (int)hipGetLastError();
@@ -705,6 +749,10 @@ static long long ring_streams(int B, int ks, int n_cus) {
 int crag_fp4_segments(int B, int dim_pad, int n_cus) {
     const int ks = dim_pad >> 6;
     return use_ring(B, ks) ? (int)ring_streams(B, ks, n_cus) * 2 : 0;
+}
+
+bool crag_fp4_splits_itself(int B, int dim_pad) {
+    return B <= SPLIT_QUERIES && B <= CRAG_FP4_GROUP_Q && B * dim_pad <= SPLIT_ELEMS && dim_pad <= 64 * SPLIT_KS;
 }
 
 int crag_launch_scan_fp4(const Fp4Args& args, int dim_pad, bool filter, int n_cus, hipStream_t s) {
