@@ -125,8 +125,8 @@ def _ptr(t):
 def _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, want_coef):
     import torch
     dev, n_bags, (vocab, dim) = table.device, offsets.numel() - 1, table.shape
-    out = torch.empty((n_bags, dim), dtype=out_dtype, device=dev)
-    coef = torch.empty((n_bags,), dtype=torch.float32, device=dev) if want_coef else None
+    out = table.new_empty((n_bags, dim), dtype=out_dtype)
+    coef = table.new_empty((n_bags,), dtype=torch.float32) if want_coef else None
     n = ids.numel()
     ws, ws_ptr, ws_bytes = _workspace(n, n_bags, dim, False, dev)
     check(_lib.load().crag_embed_forward_device(
@@ -204,7 +204,7 @@ def embed_bags(table, ids, offsets, weights=None, mode: str = "mean", scale: flo
             for node, _ in y.grad_fn.next_functions:
                 if node is not None:
                     node.metadata.setdefault("coderag_stream", stream)
-        return y.to(out_dtype)
+        return y if out_dtype == torch.float32 else y.to(out_dtype)
     return _forward(table, ids, offsets, weights, mode, scale, normalize, out_dtype, False)[0]
 
 
