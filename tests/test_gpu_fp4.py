@@ -366,6 +366,28 @@ def test_noalloc_and_sharded_entry_points(coracle):
         assert np.array_equal(a, b)
 
 
+@pytest.mark.parametrize("n,d", [(7, 100), (8000, 384), (25000, 384), (30000, 768), (31000, 500), (40000, 1024), (9000, 2048)])
+def test_few_queries_by_every_entry_and_path(n, d):
+    import torch
+    col = collection(unit(n, d, 1))
+    q = unit(7, d, 2)
+    qd = torch.from_numpy(q).cuda()
+    want = numpy_of(col.search_device(qd, 10))
+    for b in (1, 2, 3, 7):
+        for path in ("auto", "gemv", "mfma", "tiled"):
+            col.set_path(path)
+            for got in (numpy_of(col.search_device(qd[:b].contiguous(), 10)), col.search(q[:b], 10)):
+                for x, w in zip(got, want):
+                    assert np.array_equal(x, w[:b]), (b, path)
+        col.set_path("auto")
+        out = [torch.empty((b, 10), dtype=t, device="cuda") for t in (torch.int64, torch.float64, torch.float32)] + [torch.empty(b, dtype=torch.int32, device="cuda")]
+        rc = ch.load().crag_search_device_noalloc(col.handle, qd.data_ptr(), b, 10, C.c_double(2.0), None, None, *[t.data_ptr() for t in out], None)
+        assert rc == 0
+        torch.cuda.synchronize()
+        for x, w in zip(numpy_of(out), want):
+            assert np.array_equal(x, w[:b]), (b, "noalloc")
+
+
 def test_two_threads_and_a_stream_of_the_callers():
     import torch
     col = collection(unit(30000, 384, 1))
