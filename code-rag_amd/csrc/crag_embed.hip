@@ -1056,23 +1056,24 @@ int vec_of(int dim, int esz, const void* p) {
         if (dim % vec == 0 && (uintptr_t)p % (size_t)(vec * esz) == 0) return vec;
     return 1;
 }
-// Positions a group of lanes walks: as many groups as the chip holds at once (about twelve waves a CU), at least eight
-// positions each: a segment that crosses a border costs a row written and read again, and a second round of waves that is
-// not full costs half a round (1M tokens of 384 float32: 168 positions a group 120 us, 128 141 us).
-int share_of(long long n, int lpr) {
-    const long long groups = 256ll * 4 * SEG_WAVES * (64 / lpr);
+// Positions a group of lanes walks: as many groups as `waves` waves a SIMD hold, at least eight positions each: a segment that
+// crosses a border costs a row written and read again, and a second round of waves that is not full costs half a round (1M tokens
+// of 384 float32 backward: 168 positions a group 120 us, 128 141 us).
+int share_of(long long n, int lpr, int waves) {
+    const long long groups = 256ll * 4 * waves * (64 / lpr);
     return (int)std::max<long long>(8, ((n + groups - 1) / groups + 7) / 8 * 8);
 }
+constexpr int MOST_WAVES = 5;
 
 struct Walk {  // how a gather of n rows is cut up
     Shape sh;
     int share;
     long long n_share, blocks;
 };
-Walk plan_walk(long long n, int dim, int dtype, const void* src) {
+Walk plan_walk(long long n, int dim, int dtype, const void* src, int waves = SEG_WAVES) {
     Walk w;
     w.sh = row_shape(dim, vec_of(dim, dtype == CRAG_F32 ? 4 : 2, src));
-    w.share = share_of(n, w.sh.lpr);
+    w.share = share_of(n, w.sh.lpr, waves);
     w.n_share = (n + w.share - 1) / w.share;
     const int per_block = 4 * (64 / w.sh.lpr);
     w.blocks = (w.n_share + per_block - 1) / per_block;
@@ -1103,6 +1104,30 @@ int launch_segsum(CragSegArgs a, const Walk& w, hipStream_t s) {
     CRAG_SEG_CASES(X)
 #undef X
     return -1;
+}
+// Forward: the waves a SIMD really holds.  With fewer, the first CUs get all they can and the others nothing (1M tokens of 128
+// float32: three waves 82 us, four 46).
+template <int DT>
+int forward_waves(const Shape& sh) {
+#define X(V, N)                                                                                                                      \
+    if (sh.vec == V && sh.nv == N) {                                                                                                  \
+        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                                  \
+            static std::atomic<int> known{0};                                                                                         \
+            int waves = known.load(std::memory_order_relaxed);                                                                        \
+            if (!waves) {                                                                                                             \
+                if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&waves, k_segsum<DT, false, V, N>, 256, 0) != hipSuccess || waves < 1) {  \
+                    (void)hipGetLastError();                                                                                          \
+                    waves = SEG_WAVES;                                                                                                \
+                }                                                                                                                     \
+                waves = std::min(waves, MOST_WAVES);                                                                                  \
+                known.store(waves, std::memory_order_relaxed);                                                                        \
+            }                                                                                                                         \
+            return waves;                                                                                                             \
+        }                                                                                                                             \
+    }
+    CRAG_SEG_CASES(X)
+#undef X
+    return SEG_WAVES;
 }
 template <int DT>
 int launch_bag(const CragSegArgs& a, const Shape& sh, hipStream_t s) {
@@ -1183,7 +1208,7 @@ struct Carve {
 long long most_shares(long long n, int dim) {
     long long most = 1;
     for (int vec : {1, 2, 4, 8}) {
-        const int share = share_of(n, row_shape(dim, vec).lpr);
+        const int share = share_of(n, row_shape(dim, vec).lpr, MOST_WAVES);
         most = std::max(most, (n + share - 1) / share);
     }
     return most;
@@ -1235,7 +1260,12 @@ size_t crag_embed_ws_bytes(long long n, int n_bags, int dim, bool backward) {
 int crag_launch_embed_forward(const CragEmbedArgs& e, hipStream_t s) {
     Carve c{(char*)e.workspace};
     const FwdWs ws = carve_fwd(c, e.n, e.n_bags, e.dim);
-    const Walk w = plan_walk(e.n, e.dim, e.dtype, e.table);
+    const Shape sh = row_shape(e.dim, vec_of(e.dim, e.dtype == CRAG_F32 ? 4 : 2, e.table));
+    int waves = e.dtype == CRAG_F32 ? forward_waves<CRAG_F32>(sh) : forward_waves<CRAG_BF16>(sh);
+    // long bags in long shares: a third more shares than fit even out what the first round leaves uneven (384 float32, bags of
+    // 1000 tokens, 1M in all: 135 -> 113 us; bags of 150: 72 -> 79, bags of 2000, 200 k in all: 32 -> 36)
+    if (waves == 3 && sh.vec * sh.nv <= 12 && e.n_bags > 0 && e.n / e.n_bags >= 512 && share_of(e.n, sh.lpr, 4) >= 96) waves = 4;
+    const Walk w = plan_walk(e.n, e.dim, e.dtype, e.table, waves);
     CragSegArgs a = {};
     apply(a, w);
     a.src = e.table;
