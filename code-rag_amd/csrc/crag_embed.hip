@@ -248,7 +248,7 @@ constexpr int SEG_WAVES = 3;
 // backward that is the token's gradient, forward a plain sum for k_embed_finish (scale, norm and count would cost this
 // kernel's registers half of its waves).  Bound by what the caches deliver to a gather, 13 .. 15 TB/s of rows where tokens are
 // as uneven as text's, and for bf16 rows by the vector units as well, which unpack (busy 60 % of the cycles): 1M tokens
-// of 384 float32 147 us, 2.5M of 768 bf16 246; backward 1M positions of 384 with 400 MB of gradient 120.
+// of 384 float32 134 us, 2.5M of 768 bf16 246; backward 1M positions of 384 with 400 MB of gradient 120.
 template <int DT, bool BWD, int VEC, int NV>
 __global__ __launch_bounds__(256, VEC * NV > 12 && VEC * NV <= 24 ? SEG_WAVES : 1) void k_segsum(CragSegArgs a) {
     constexpr int U = rows_ahead<DT, VEC, NV>();
@@ -1105,25 +1105,30 @@ int launch_segsum(CragSegArgs a, const Walk& w, hipStream_t s) {
 #undef X
     return -1;
 }
-// Forward: the waves a SIMD really holds.  With fewer, the first CUs get all they can and the others nothing (1M tokens of 128
-// float32: three waves 82 us, four 46).
-template <int DT>
-int forward_waves(const Shape& sh) {
-#define X(V, N)                                                                                                                      \
-    if (sh.vec == V && sh.nv == N) {                                                                                                  \
-        if constexpr (!(DT == CRAG_F32 && V == 8)) {                                                                                  \
-            static std::atomic<int> known{0};                                                                                         \
-            int waves = known.load(std::memory_order_relaxed);                                                                        \
-            if (!waves) {                                                                                                             \
-                if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&waves, k_segsum<DT, false, V, N>, 256, 0) != hipSuccess || waves < 1) {  \
-                    (void)hipGetLastError();                                                                                          \
-                    waves = SEG_WAVES;                                                                                                \
-                }                                                                                                                     \
-                waves = std::min(waves, MOST_WAVES);                                                                                  \
-                known.store(waves, std::memory_order_relaxed);                                                                        \
-            }                                                                                                                         \
-            return waves;                                                                                                             \
-        }                                                                                                                             \
+// The waves a SIMD really holds.  With fewer, the first CUs get all they can and the others nothing (1M tokens of 128 float32
+// forward: three waves 82 us, four 46).
+enum Gather { FORWARD, BACKWARD, WEIGHTS };
+template <Gather G, int DT, int V, int N>
+int occupancy() {
+    static std::atomic<int> known{0};
+    int waves = known.load(std::memory_order_relaxed);
+    if (waves) return waves;
+    hipError_t rc;
+    if constexpr (G == WEIGHTS) rc = hipOccupancyMaxActiveBlocksPerMultiprocessor(&waves, k_embed_dweights<DT, V, N>, 256, 0);
+    else rc = hipOccupancyMaxActiveBlocksPerMultiprocessor(&waves, k_segsum<DT, G == BACKWARD, V, N>, 256, 0);
+    if (rc != hipSuccess || waves < 1) {
+        (void)hipGetLastError();
+        waves = SEG_WAVES;
+    }
+    waves = std::min(waves, MOST_WAVES);
+    known.store(waves, std::memory_order_relaxed);
+    return waves;
+}
+template <Gather G, int DT>
+int waves_of(const Shape& sh) {
+#define X(V, N)                                                                           \
+    if (sh.vec == V && sh.nv == N) {                                                      \
+        if constexpr (!(DT == CRAG_F32 && V == 8)) return occupancy<G, DT, V, N>();       \
     }
     CRAG_SEG_CASES(X)
 #undef X
@@ -1261,7 +1266,7 @@ int crag_launch_embed_forward(const CragEmbedArgs& e, hipStream_t s) {
     Carve c{(char*)e.workspace};
     const FwdWs ws = carve_fwd(c, e.n, e.n_bags, e.dim);
     const Shape sh = row_shape(e.dim, vec_of(e.dim, e.dtype == CRAG_F32 ? 4 : 2, e.table));
-    int waves = e.dtype == CRAG_F32 ? forward_waves<CRAG_F32>(sh) : forward_waves<CRAG_BF16>(sh);
+    int waves = e.dtype == CRAG_F32 ? waves_of<FORWARD, CRAG_F32>(sh) : waves_of<FORWARD, CRAG_BF16>(sh);
     // long bags in long shares: a third more shares than fit even out what the first round leaves uneven (384 float32, bags of
     // 1000 tokens, 1M in all: 135 -> 113 us; bags of 150: 72 -> 79, bags of 2000, 200 k in all: 32 -> 36)
     if (waves == 3 && sh.vec * sh.nv <= 12 && e.n_bags > 0 && e.n / e.n_bags >= 512 && share_of(e.n, sh.lpr, 4) >= 96) waves = 4;
@@ -1338,7 +1343,9 @@ int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
     // out (109 us against 150 behind a pass that wrote 400 MB, 1M tokens of 384 elements)
     auto weights = [&]() -> int {
         if (!e.d_weights || e.n == 0) return (int)hipGetLastError();
-        const Walk k = plan_walk(e.n, e.dim, e.dtype, e.table);
+        const Shape sh = row_shape(e.dim, vec_of(e.dim, esz, e.table));
+        const int waves = e.dtype == CRAG_BF16 ? waves_of<WEIGHTS, CRAG_BF16>(sh) : (sh.vec * sh.nv <= 8 ? waves_of<WEIGHTS, CRAG_F32>(sh) : SEG_WAVES);
+        const Walk k = plan_walk(e.n, e.dim, e.dtype, e.table, waves);
         apply(a, k);
         return e.dtype == CRAG_F32 ? launch_dweights<CRAG_F32>(a, k, e.table, e.ids, e.d_weights, s)
                                    : launch_dweights<CRAG_BF16>(a, k, e.table, e.ids, e.d_weights, s);
@@ -1369,7 +1376,10 @@ int crag_launch_embed_backward(const CragEmbedArgs& args, hipStream_t s) {
         }
     }
     if ((rc = (int)hipGetLastError()) || !e.d_table) return rc;
-    const Walk k = plan_walk(e.n, e.dim, CRAG_F32, w.dp);
+    // (longer float32 rows, here and above: a fourth wave's shares are worth less than their borders cost; 1M tokens of 256 float32
+    // 251 -> 215 us, of 768 556 -> 593)
+    const Shape sh = row_shape(e.dim, vec_of(e.dim, 4, w.dp));
+    const Walk k = plan_walk(e.n, e.dim, CRAG_F32, w.dp, sh.vec * sh.nv <= 8 ? waves_of<BACKWARD, CRAG_F32>(sh) : SEG_WAVES);
     apply(a, k);
     a.pairs = w.pairs[cur];
     a.partial = w.partial;
